@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libaipu_q4k.so")
 AIPU_OK, AIPU_EINVAL, AIPU_ECUDA, AIPU_ETIMEOUT, AIPU_ENCCL, AIPU_ENOMEM = 0, -1, -2, -3, -4, -5
 # weight types
 Q4_K, Q6_K, Q8_0, F16, F32 = 0, 1, 2, 3, 4
-DT_F32, DT_BF16 = 0, 1
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 MODE_FAST, MODE_STRICT = 0, 1
 FLAG_PDL = 1
 FLAG_STRICT = 2
@@ -41,6 +41,15 @@ class MoeWeights(ctypes.Structure):
         ("gate_wtype", ctypes.c_int32), ("up_wtype", ctypes.c_int32), ("down_wtype", ctypes.c_int32),
         ("gate_w", c_void_p), ("up_w", c_void_p), ("down_w", c_void_p),
         ("shared_gate_w", c_void_p), ("shared_up_w", c_void_p), ("shared_down_w", c_void_p),
+    ]
+
+
+class Lora(ctypes.Structure):
+    """aipu_lora (include/aipu_q4k.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("n_adapters", ctypes.c_int32), ("rank", c_int64), ("in_features", c_int64),
+        ("out_features", c_int64), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p), ("ranks", c_void_p),
     ]
 
 
@@ -81,6 +90,12 @@ SIGNATURES = {
     "aipu_ep_connect": (c_int, [c_void_p, c_void_p]),
     "aipu_ep_moe_layer": (c_int, [c_void_p, ctypes.POINTER(MoeWeights), c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "aipu_ep_destroy": (c_int, [c_void_p]),
+    "aipu_lora_workspace": (c_int64, [c_int64, c_int64]),
+    "aipu_lora_add": (c_int, [c_void_p, ctypes.POINTER(Lora), c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
+                              c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p]),
+    "aipu_q4k_gemm_lora_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64, c_int64]),
+    "aipu_q4k_gemm_lora": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                   ctypes.POINTER(Lora), c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

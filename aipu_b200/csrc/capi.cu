@@ -14,6 +14,7 @@
 #include "gemv.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "lora.cuh"
 
 namespace aipu {
 
@@ -1315,4 +1316,145 @@ extern "C" int aipu_q4k_gemm_tc(aipu_ctx* c, int wtype, const void* w, int64_t N
   p.y = static_cast<uint16_t*>(y);
   p.status = c->status;
   return tc_gemm_launch(p, 128, 1, static_cast<int>((M + 127) / 128), c->num_sms, s, true);
+}
+
+// ------------------------------------------------------------------ low-rank adapters
+static int lora_params(const aipu_lora* ad, const int32_t* ids, int64_t M, LoraParams& p, const char* bad) {
+  if (!ad || (M > 0 && !ids) || !ad->a || !ad->b || (ad->dtype != AIPU_DT_BF16 && ad->dtype != AIPU_DT_F16) || ad->n_adapters < 1 ||
+      ad->n_adapters > 32768 || ad->rank < 1 || ad->rank > 128 || ad->in_features < 1 || ad->in_features > (1 << 24) ||
+      ad->out_features < 1 || ad->out_features > (1 << 24) || M < 0 || M > (1 << 24))
+    return set_error(EINVAL_, bad);
+  p.a = ad->a;
+  p.b = ad->b;
+  p.scale = ad->scale;
+  p.ranks = ad->ranks;
+  p.adtype = ad->dtype == AIPU_DT_F16 ? AD_F16 : AD_BF16;
+  p.L = ad->n_adapters;
+  p.R = static_cast<int>(ad->rank);
+  p.K = static_cast<int>(ad->in_features);
+  p.N = static_cast<int>(ad->out_features);
+  p.M = static_cast<int>(M);
+  p.ids = ids;
+  return OK;
+}
+
+extern "C" int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters) {
+  if (M < 0 || M > (1 << 24) || n_adapters < 1 || n_adapters > 32768) return 0;
+  return static_cast<int64_t>(lora_plan_bytes(M, n_adapters));
+}
+
+extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
+                             const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,
+                             int64_t ws_bytes, void* stream) {
+  LoraParams p = {};
+  if (!c) return set_error(EINVAL_, "lora_add: null context");
+  int rc = lora_params(ad, ids, M, p, "lora_add: bad adapters (bf16 or fp16, 1 to 32768 of rank 1 to 128) or row count");
+  if (rc) return rc;
+  if (M == 0) return OK;
+  if (!x || !y || !out || ldx < p.K || ldy < p.N || ldo < p.N) return set_error(EINVAL_, "lora_add: null pointer or row stride below the row length");
+  if ((y_dtype != AIPU_DT_F32 && y_dtype != AIPU_DT_BF16) || (out_dtype != AIPU_DT_F32 && out_dtype != AIPU_DT_BF16) ||
+      (y_dtype == AIPU_DT_BF16 && out_dtype == AIPU_DT_F32))
+    return set_error(EINVAL_, "lora_add: y and out must be bf16, fp32, or fp32 and bf16");
+  if (out == y && (y_dtype != out_dtype || ldy != ldo))
+    return set_error(EINVAL_, "lora_add: in place needs the same type and row stride");
+  if ((reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < aipu_lora_workspace(M, p.L) || (!ws && aipu_lora_workspace(M, p.L) > 0))
+    return set_error(EINVAL_, "lora_add: workspace missing, too small or not 16-byte aligned");
+  p.x = static_cast<const uint16_t*>(x);
+  p.ldx = ldx;
+  p.y = y;
+  p.ldy = ldy;
+  p.out = out;
+  p.ldo = ldo;
+  p.y_f32 = y_dtype == AIPU_DT_F32;
+  p.out_f32 = out_dtype == AIPU_DT_F32;
+  p.status = c->status;
+  DeviceGuard dg(c->device);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if ((rc = lora_plan_launch(p, ws, s, false))) return rc;
+  return lora_launch(p, c->num_sms, s, (c->flags & AIPU_FLAG_PDL) != 0);
+}
+
+// rows from which the projection runs on the tcgen05 GEMM
+static bool gemm_lora_tc(int wtype, int64_t M) { return (wtype == AIPU_Q4_K || wtype == AIPU_Q6_K) && M >= 64; }
+
+extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters) {
+  if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
+      n_adapters > 32768)
+    return 0;
+  size_t b = al256x(lora_plan_bytes(M, n_adapters)) + al256x(4 * static_cast<size_t>(M) * N);
+  if (gemm_lora_tc(wtype, M)) b += al256x(xt_bytes(M, K)) + al256x(4 * M);
+  return static_cast<int64_t>(b);
+}
+
+extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,
+                                  const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes,
+                                  void* stream) {
+  LoraParams p = {};
+  if (!c) return set_error(EINVAL_, "gemm_lora: null context");
+  int rc = lora_params(ad, ids, M, p, "gemm_lora: bad adapters (bf16 or fp16, 1 to 32768 of rank 1 to 128) or row count");
+  if (rc) return rc;
+  if (!w || (M > 0 && (!x || !y)) || wtype == AIPU_F32 || aipu_row_bytes(wtype, K) == 0 || K % 256 || ad->in_features != K ||
+      ad->out_features != N)
+    return set_error(EINVAL_, "gemm_lora: bad arguments (GGUF rows, K % 256 == 0, adapters of the same K and N)");
+  if (M == 0) return OK;
+  if ((reinterpret_cast<uintptr_t>(w) & 15u) || (reinterpret_cast<uintptr_t>(x) & 15u))
+    return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned");
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L))
+    return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
+  if ((N + 15) / 16 > c->ws[0].max_tiles) return set_error(EINVAL_, "gemm_lora: N too large for the workspace");
+  DeviceGuard dg(c->device);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  void* plan = b;
+  b += al256x(lora_plan_bytes(M, p.L));
+  float* y32 = reinterpret_cast<float*>(b);
+  b += al256x(4 * static_cast<size_t>(M) * N);
+  p.x = static_cast<const uint16_t*>(x);
+  p.ldx = K;
+  p.y = y32;
+  p.ldy = p.ldo = N;
+  p.out = y;
+  p.y_f32 = 1;
+  p.status = c->status;
+  if ((rc = lora_plan_launch(p, plan, s, false))) return rc;
+  if (gemm_lora_tc(wtype, M)) {
+    uint8_t* xt = b;
+    int* shift = reinterpret_cast<int*>(xt + al256x(xt_bytes(M, K)));
+    rc = prescale_tiled_launch(p.x, p.M, p.K, nullptr, 0, static_cast<int>((M + 7) & ~7LL), nullptr, xt, shift, s, false);
+    if (rc) return rc;
+    TcParams t = {};
+    t.wt = wtype;
+    t.shared_id = -1;
+    t.w[0] = static_cast<const uint8_t*>(w);
+    t.row_bytes = row_bytes_of(wtype, K);
+    t.N = p.N;
+    t.K = p.K;
+    t.M = p.M;
+    t.xt = xt;
+    t.xshift = shift;
+    t.y32 = y32;
+    t.status = c->status;
+    rc = tc_gemm_launch(t, 128, 1, static_cast<int>((M + 127) / 128), c->num_sms, s, true);
+  } else {
+    for (int64_t m0 = 0; m0 < M && !rc; m0 += 8) {
+      GemvParams g = {};
+      g.w0 = static_cast<const uint8_t*>(w);
+      g.row_bytes = row_bytes_of(wtype, K);
+      g.n_groups = 1;
+      g.N = p.N;
+      g.K = p.K;
+      g.x = p.x + m0 * K;
+      g.M = static_cast<int>(std::min<int64_t>(8, M - m0));
+      g.y32 = y32 + m0 * N;
+      g.partials = c->ws[0].partials;
+      g.counters = c->ws[0].counters;
+      g.status = c->status;
+      // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
+      // kernel behind it may read x, the ids and the adapters without waiting for it
+      rc = gemv_launch(wtype, XT_BF16, EPI_STORE, g, c->num_sms, s, false);
+    }
+  }
+  if (rc) return rc;
+  p.wait_y = 1;
+  return lora_launch(p, c->num_sms, s, true);
 }

@@ -325,3 +325,114 @@ def moe_combine(sel: torch.Tensor, sel_w: torch.Tensor, experts_per_piece: int, 
     check(lib().aipu_moe_combine(ctx.handle, M, H, T, _ptr(sel), _ptr(sel_w), experts_per_piece, _ptr(pieces),
                                  _ptr(y_shared), _ptr(out), _stream(pieces.device)))
     return out
+
+
+# ------------------------------------------------------------------------------------ per-request adapters
+def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
+    """Elements between the rows of a 2-D CUDA tensor whose rows are contiguous (columns of a wider tensor too)."""
+    if t.dim() != 2 or t.shape[1] != width:
+        raise ValueError(f"{name} must be [rows, {width}]")
+    if not t.is_cuda:
+        raise ValueError("aipu_b200 runs on CUDA tensors only (no CPU fallback)")
+    ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    if t.shape[0] and ((width > 1 and t.stride(1) != 1) or ld < width):
+        raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
+    return ld
+
+
+def _one_device(ctx: Context, *ts):
+    index = ctx.device.index if ctx.device.index is not None else 0
+    for t in ts:
+        if t is not None and t.device.index != index:
+            raise ValueError(f"all tensors must be on the context's device ({ctx.device}), got {t.device}")
+
+
+@dataclass
+class LoraAdapters:
+    """Low-rank adapters of one projection of K inputs and N outputs, on the GPU: a [L, R, K] and b [L, N, R] (bf16 or
+    fp16), scale fp32 [L] (1 if None), ranks int32 [L] (R if None; rows of a and columns of b from an adapter's rank
+    on are not used). R <= 128, L <= 32768."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+    ranks: Optional[torch.Tensor] = None
+
+    def cstruct(self) -> L.Lora:
+        a, b = self.a, self.b
+        _need_cuda(a, b, self.scale, self.ranks)
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("adapters must be a [L, R, K] and b [L, N, R]")
+        if a.dtype != b.dtype or a.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("adapters must be bf16 or fp16, both the same")
+        if self.scale is not None and (self.scale.dtype != torch.float32 or self.scale.shape != a.shape[:1]):
+            raise ValueError("scale must be fp32 [L]")
+        if self.ranks is not None and (self.ranks.dtype != torch.int32 or self.ranks.shape != a.shape[:1]):
+            raise ValueError("ranks must be int32 [L]")
+        s = L.Lora()
+        s.dtype = L.DT_BF16 if a.dtype == torch.bfloat16 else L.DT_F16
+        s.n_adapters, s.rank, s.in_features = a.shape
+        s.out_features = b.shape[1]
+        s.a, s.b = a.data_ptr(), b.data_ptr()
+        s.scale = self.scale.data_ptr() if self.scale is not None else None
+        s.ranks = self.ranks.data_ptr() if self.ranks is not None else None
+        return s
+
+
+def _lora_inputs(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor) -> L.Lora:
+    _need_cuda(ids)
+    if x.dtype != torch.bfloat16:
+        raise ValueError("adapter activations must be bf16")
+    if ids.dtype != torch.int32 or ids.dim() != 1 or x.dim() != 2 or ids.shape[0] != x.shape[0]:
+        raise ValueError("ids must be int32 [M], one for each row of x")
+    return ad.cstruct()
+
+
+def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None,
+             ctx: Optional[Context] = None) -> torch.Tensor:
+    """out[m] = y[m] + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m], for the rows of many requests at once: beside any
+    projection that gave y (bf16 or fp32 [M, N]). x bf16 [M, K]; a negative id leaves the row as it is (an id >= L too,
+    with bit 4 of the context's status set). Sums in fp32, one rounding. out: bf16 or y's type (default: like y); out=y
+    adds in place. x, y and out may be columns of wider tensors (stride(1) == 1)."""
+    cs = _lora_inputs(ad, ids, x)
+    ctx = ctx or Context.default(x.device)
+    M = x.shape[0]
+    if y.dim() != 2 or y.shape[0] != M:
+        raise ValueError("y must have a row for each row of x")
+    ldx, ldy = _rows_of(x, "x", cs.in_features), _rows_of(y, "y", cs.out_features)
+    if out is None:
+        out = torch.empty((M, cs.out_features), dtype=y.dtype, device=y.device)
+    ldo = _rows_of(out, "out", cs.out_features)
+    if out.shape[0] != M or y.dtype not in _DTYPE or out.dtype not in (torch.bfloat16, y.dtype):
+        raise ValueError("y must be bf16 or fp32 and out bf16 or y's type, with a row for each row of x")
+    _one_device(ctx, ad.a, ad.b, ad.scale, ad.ranks, ids, x, y, out)
+    n = lib().aipu_lora_workspace(M, cs.n_adapters)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    check(lib().aipu_lora_add(ctx.handle, ctypes.byref(cs), _ptr(ids), _ptr(x), ldx, M, _ptr(y), _DTYPE[y.dtype], ldy,
+                              _ptr(out), _DTYPE[out.dtype], ldo, _ptr(ws), n, _stream(x.device)))
+    return out
+
+
+def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: LoraAdapters, ids: torch.Tensor,
+              ctx: Optional[Context] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[m] bf16 = x[m] W^T + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m]: a shared quantised projection (W = N GGUF rows
+    of K weights, as in gemm) and the adapters of its rows, rounded once. Few rows run on the decode GEMV, 64 and more of
+    Q4_K or Q6_K on the tensor-core GEMM."""
+    _need_cuda(w, x, out)
+    cs = _lora_inputs(ad, ids, x)
+    if x.dim() != 2 or x.shape[1] != K or cs.in_features != K or cs.out_features != N:
+        raise ValueError("x must be [M, K], a [L, R, K] and b [L, N, R]")
+    if w.numel() * w.element_size() < N * row_bytes(wtype, K):
+        raise ValueError("weight buffer smaller than N * row_bytes")
+    ctx = ctx or Context.default(x.device)
+    M = x.shape[0]
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
+        raise ValueError("out must be bf16 [M, N]")
+    _one_device(ctx, w, ad.a, ad.b, ad.scale, ad.ranks, ids, x, out)
+    n = lib().aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    check(lib().aipu_q4k_gemm_lora(ctx.handle, wtype, _ptr(w), N, K, _ptr(x), M, ctypes.byref(cs), _ptr(ids), _ptr(out),
+                                   _ptr(ws), n, _stream(x.device)))
+    return out

@@ -43,6 +43,7 @@ extern "C" {
 /* activation / output dtypes */
 #define AIPU_DT_F32 0
 #define AIPU_DT_BF16 1
+#define AIPU_DT_F16 2 /* adapters only */
 
 #define AIPU_MODE_FAST 0
 #define AIPU_MODE_STRICT 1
@@ -253,6 +254,46 @@ int aipu_ep_connect(aipu_ep* ep, const void* handles);
 int aipu_ep_moe_layer(aipu_ep* ep, const aipu_moe_weights* w_local, int64_t expert_lo, const void* x, int64_t M,
                       void* y, void* stream);
 int aipu_ep_destroy(aipu_ep* ep);
+
+/* Low-rank adapters of one projection of K inputs and N outputs: adapter l has a[l] (R rows of K),
+ * b[l] (N rows of R), a factor and a rank <= R (rows of a[l] and columns of b[l] from the rank on are
+ * not used, whatever they hold). All device pointers; a, b 2-byte aligned (16-byte rows are fastest). */
+typedef struct aipu_lora {
+  int32_t dtype;        /* of a and b: AIPU_DT_BF16 or AIPU_DT_F16 */
+  int32_t n_adapters;   /* 1 .. 32768 */
+  int64_t rank;         /* R: 1 .. 128 */
+  int64_t in_features;  /* K */
+  int64_t out_features; /* N */
+  const void* a;        /* [n_adapters, R, K] */
+  const void* b;        /* [n_adapters, N, R] */
+  const float* scale;   /* [n_adapters] or NULL (1) */
+  const int32_t* ranks; /* [n_adapters] or NULL (R); values outside 0 .. R act as the nearer bound */
+} aipu_lora;
+
+/* Adapters of many requests beside a projection: for every row m of x[M, K] (bf16), with l = ids[m]:
+ *   out[m, n] = round(y[m, n] + sum_r (scale[l] * sum_k x[m, k] a[l][r, k]) * b[l][n, r])
+ * sums in fp32, one rounding to the type of out. A negative id means no adapter: out[m] = y[m]. An
+ * id >= n_adapters acts as -1 and sets bit 4 of the context's status word. y and out are both bf16, both
+ * fp32, or fp32 and bf16; out may be y (same type and stride: rows without an adapter are then not
+ * touched), otherwise they must not overlap. ldx, ldy, ldo: elements between rows (>= K, N, N), so
+ * columns of a wider tensor can be passed.
+ * ws: device scratch of aipu_lora_workspace(M, n_adapters) bytes (NULL when that is 0), in use until
+ * the call's work on `stream` is done. Nothing else is shared, so calls with their own ws may run at the
+ * same time. Equal calls give equal bits. No counterpart in the reference. */
+int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters);
+int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
+                  const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,
+                  int64_t ws_bytes, void* stream);
+
+/* The quantised projection with the adapters of its rows: y[m, n] (bf16) = bf16(x[m] W^T + the adapter
+ * term of aipu_lora_add); x[M, K] bf16, 16-byte aligned, W = N GGUF rows of K weights (Q4_K, Q6_K, Q8_0,
+ * F16; K a multiple of 256, 16-byte aligned). The projection's fp32 sums (those of AIPU_MODE_FAST, or of
+ * the tcgen05 GEMM for many rows of Q4_K / Q6_K) are not rounded before the adapter term is added.
+ * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Uses the context's
+ * stream-K workspace (one context per concurrently used stream). No counterpart in the reference. */
+int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters);
+int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,
+                       const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
