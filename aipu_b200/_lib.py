@@ -53,6 +53,16 @@ class Lora(ctypes.Structure):
     ]
 
 
+class LogitCtl(ctypes.Structure):
+    """aipu_logit_ctl (include/aipu_q4k.h)."""
+
+    _fields_ = [
+        ("tokens", c_void_p), ("n_tokens", c_int64), ("spans", c_void_p), ("penalties", c_void_p),
+        ("bias_begin", c_void_p), ("bias_ids", c_void_p), ("bias_vals", c_void_p), ("n_bias", c_int64),
+        ("mask", c_void_p), ("mask_rows", c_void_p), ("n_masks", c_int64),
+    ]
+
+
 # name -> (restype, argtypes); every function the header declares
 SIGNATURES = {
     "aipu_version": (c_int, []),
@@ -90,6 +100,8 @@ SIGNATURES = {
     "aipu_ep_connect": (c_int, [c_void_p, c_void_p]),
     "aipu_ep_moe_layer": (c_int, [c_void_p, ctypes.POINTER(MoeWeights), c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "aipu_ep_destroy": (c_int, [c_void_p]),
+    "aipu_logits_process": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, ctypes.POINTER(LogitCtl),
+                                    c_void_p, c_int64, c_void_p, c_void_p]),
     "aipu_lora_workspace": (c_int64, [c_int64, c_int64]),
     "aipu_lora_add": (c_int, [c_void_p, ctypes.POINTER(Lora), c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
                               c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p]),

@@ -14,6 +14,7 @@
 #include "gemv.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "logits.cuh"
 #include "lora.cuh"
 
 namespace aipu {
@@ -1347,18 +1348,18 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
                              const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,
                              int64_t ws_bytes, void* stream) {
   LoraParams p = {};
-  if (!c) return set_error(EINVAL_, "lora_add: null context");
   int rc = lora_params(ad, ids, M, p, "lora_add: bad adapters (bf16 or fp16, 1 to 32768 of rank 1 to 128) or row count");
   if (rc) return rc;
-  if (M == 0) return OK;
-  if (!x || !y || !out || ldx < p.K || ldy < p.N || ldo < p.N) return set_error(EINVAL_, "lora_add: null pointer or row stride below the row length");
+  if ((M > 0 && (!x || !y || !out)) || ldx < p.K || ldy < p.N || ldo < p.N) return set_error(EINVAL_, "lora_add: null pointer or row stride below the row length");
   if ((y_dtype != AIPU_DT_F32 && y_dtype != AIPU_DT_BF16) || (out_dtype != AIPU_DT_F32 && out_dtype != AIPU_DT_BF16) ||
       (y_dtype == AIPU_DT_BF16 && out_dtype == AIPU_DT_F32))
     return set_error(EINVAL_, "lora_add: y and out must be bf16, fp32, or fp32 and bf16");
-  if (out == y && (y_dtype != out_dtype || ldy != ldo))
+  if (out && out == y && (y_dtype != out_dtype || ldy != ldo))
     return set_error(EINVAL_, "lora_add: in place needs the same type and row stride");
   if ((reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < aipu_lora_workspace(M, p.L) || (!ws && aipu_lora_workspace(M, p.L) > 0))
     return set_error(EINVAL_, "lora_add: workspace missing, too small or not 16-byte aligned");
+  if (!c) return set_error(EINVAL_, "lora_add: null context");
+  if (M == 0) return OK;
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = ldx;
   p.y = y;
@@ -1390,17 +1391,17 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
                                   const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes,
                                   void* stream) {
   LoraParams p = {};
-  if (!c) return set_error(EINVAL_, "gemm_lora: null context");
   int rc = lora_params(ad, ids, M, p, "gemm_lora: bad adapters (bf16 or fp16, 1 to 32768 of rank 1 to 128) or row count");
   if (rc) return rc;
   if (!w || (M > 0 && (!x || !y)) || wtype == AIPU_F32 || aipu_row_bytes(wtype, K) == 0 || K % 256 || ad->in_features != K ||
       ad->out_features != N)
     return set_error(EINVAL_, "gemm_lora: bad arguments (GGUF rows, K % 256 == 0, adapters of the same K and N)");
-  if (M == 0) return OK;
   if ((reinterpret_cast<uintptr_t>(w) & 15u) || (reinterpret_cast<uintptr_t>(x) & 15u))
     return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned");
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L))
+  if ((M > 0 && !ws) || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L))
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
+  if (!c) return set_error(EINVAL_, "gemm_lora: null context");
+  if (M == 0) return OK;
   if ((N + 15) / 16 > c->ws[0].max_tiles) return set_error(EINVAL_, "gemm_lora: N too large for the workspace");
   DeviceGuard dg(c->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1457,4 +1458,50 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   if (rc) return rc;
   p.wait_y = 1;
   return lora_launch(p, c->num_sms, s, true);
+}
+
+// ------------------------------------------------------------------ logits
+extern "C" int aipu_logits_process(aipu_ctx* c, const void* logits, int dtype, int64_t ld, int64_t M, int64_t V,
+                                   const aipu_logit_ctl* ctl, float* out, int64_t ldo, int32_t* token, void* stream) {
+  if (M < 0 || M > (1 << 24) || V < 1 || V > (1 << 28) || (dtype != AIPU_DT_F32 && dtype != AIPU_DT_BF16) || ld < V ||
+      (out && ldo < V) || (M > 0 && (!logits || (!out && !token))))
+    return set_error(EINVAL_, "logits_process: bad shape, type or pointer");
+  if (out == logits && out && (dtype != AIPU_DT_F32 || ld != ldo))
+    return set_error(EINVAL_, "logits_process: in place needs fp32 logits and one row stride");
+  if (ctl) {
+    if ((ctl->spans != nullptr) != (ctl->penalties != nullptr) || ctl->n_tokens < 0 || ctl->n_tokens > INT32_MAX ||
+        (ctl->n_tokens > 0 && !ctl->tokens))
+      return set_error(EINVAL_, "logits_process: penalties need spans, and tokens for them (at most 2^31 - 1)");
+    if (ctl->n_bias < 0 || (ctl->bias_begin && ctl->n_bias > 0 && (!ctl->bias_ids || !ctl->bias_vals)))
+      return set_error(EINVAL_, "logits_process: biases need ids and values");
+    if ((ctl->mask != nullptr) != (ctl->mask_rows != nullptr) || (ctl->mask && (ctl->n_masks < 1 || ctl->n_masks > INT32_MAX)))
+      return set_error(EINVAL_, "logits_process: masks need mask_rows and at least one mask");
+  }
+  if (!c) return set_error(EINVAL_, "logits_process: null context");
+  if (M == 0) return OK;
+  LogitParams p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.f32 = dtype == AIPU_DT_F32;
+  p.M = static_cast<int>(M);
+  p.V = static_cast<int>(V);
+  p.out = out;
+  p.ldo = ldo;
+  p.token = token;
+  p.status = c->status;
+  if (ctl) {
+    p.tokens = ctl->tokens;
+    p.n_tokens = ctl->n_tokens;
+    p.spans = ctl->spans;
+    p.penalties = ctl->penalties;
+    p.bias_begin = ctl->bias_begin;
+    p.bias_ids = ctl->bias_ids;
+    p.bias_vals = ctl->bias_vals;
+    p.n_bias = ctl->n_bias;
+    p.mask = ctl->mask;
+    p.mask_rows = ctl->mask_rows;
+    p.n_masks = static_cast<int>(ctl->n_masks);
+  }
+  DeviceGuard dg(c->device);
+  return logits_launch(p, c->num_sms, static_cast<cudaStream_t>(stream), (c->flags & AIPU_FLAG_PDL) != 0);
 }

@@ -23,6 +23,33 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# The per-request operators are called several times a layer with little work each, so their front end is kept
+# short: raw pointers and the raw stream handle, and one pass over the tensors' devices.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on(ctx: Optional["Context"], *ts) -> tuple:
+    """(context, device index) of tensors that all have to be on one GPU, the context's."""
+    index = ts[0].get_device()
+    if index < 0:
+        raise ValueError("aipu_b200 runs on CUDA tensors only (no CPU fallback)")
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"all tensors must be on one CUDA device: cuda:{index} and {t.device}")
+    if ctx is None:
+        ctx = Context._default.get(index) or Context.default(ts[0].device)
+    elif (ctx.device.index or 0) != index:
+        raise ValueError(f"the context is on {ctx.device}, the tensors on cuda:{index}")
+    return ctx, index
+
+
+def _contiguous(**ts):
+    for name, t in ts.items():
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
 def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
@@ -328,23 +355,17 @@ def moe_combine(sel: torch.Tensor, sel_w: torch.Tensor, experts_per_piece: int, 
 
 
 # ------------------------------------------------------------------------------------ per-request adapters
-def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
-    """Elements between the rows of a 2-D CUDA tensor whose rows are contiguous (columns of a wider tensor too)."""
-    if t.dim() != 2 or t.shape[1] != width:
-        raise ValueError(f"{name} must be [rows, {width}]")
-    if not t.is_cuda:
-        raise ValueError("aipu_b200 runs on CUDA tensors only (no CPU fallback)")
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
-    if t.shape[0] and ((width > 1 and t.stride(1) != 1) or ld < width):
+def _row_stride(t: torch.Tensor, name: str, rows: int, width: int) -> int:
+    """Elements between the rows of a [rows, width] tensor whose rows are contiguous (columns of a wider tensor too)."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != width:
+        raise ValueError(f"{name} must be [{rows}, {width}]")
+    ld, step = t.stride()
+    if rows <= 1:
+        ld = max(ld, width)
+    if rows and ((width > 1 and step != 1) or ld < width):
         raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
     return ld
-
-
-def _one_device(ctx: Context, *ts):
-    index = ctx.device.index if ctx.device.index is not None else 0
-    for t in ts:
-        if t is not None and t.device.index != index:
-            raise ValueError(f"all tensors must be on the context's device ({ctx.device}), got {t.device}")
 
 
 @dataclass
@@ -359,33 +380,32 @@ class LoraAdapters:
     ranks: Optional[torch.Tensor] = None
 
     def cstruct(self) -> L.Lora:
-        a, b = self.a, self.b
-        _need_cuda(a, b, self.scale, self.ranks)
-        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+        a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
+        sa, sb = a.shape, b.shape
+        if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2]:
             raise ValueError("adapters must be a [L, R, K] and b [L, N, R]")
-        if a.dtype != b.dtype or a.dtype not in (torch.bfloat16, torch.float16):
+        dtype = a.dtype
+        if b.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("adapters must be bf16 or fp16, both the same")
-        if self.scale is not None and (self.scale.dtype != torch.float32 or self.scale.shape != a.shape[:1]):
+        if scale is not None and (scale.dtype != torch.float32 or scale.shape != sa[:1]):
             raise ValueError("scale must be fp32 [L]")
-        if self.ranks is not None and (self.ranks.dtype != torch.int32 or self.ranks.shape != a.shape[:1]):
+        if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != sa[:1]):
             raise ValueError("ranks must be int32 [L]")
-        s = L.Lora()
-        s.dtype = L.DT_BF16 if a.dtype == torch.bfloat16 else L.DT_F16
-        s.n_adapters, s.rank, s.in_features = a.shape
-        s.out_features = b.shape[1]
-        s.a, s.b = a.data_ptr(), b.data_ptr()
-        s.scale = self.scale.data_ptr() if self.scale is not None else None
-        s.ranks = self.ranks.data_ptr() if self.ranks is not None else None
-        return s
+        if not (a.is_contiguous() and b.is_contiguous()):
+            raise ValueError("a and b must be contiguous")
+        _contiguous(scale=scale, ranks=ranks)
+        return L.Lora(L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F16, sa[0], sa[1], sa[2], sb[1], a.data_ptr(),
+                      b.data_ptr(), scale.data_ptr() if scale is not None else None,
+                      ranks.data_ptr() if ranks is not None else None)
 
 
-def _lora_inputs(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor) -> L.Lora:
-    _need_cuda(ids)
-    if x.dtype != torch.bfloat16:
-        raise ValueError("adapter activations must be bf16")
-    if ids.dtype != torch.int32 or ids.dim() != 1 or x.dim() != 2 or ids.shape[0] != x.shape[0]:
-        raise ValueError("ids must be int32 [M], one for each row of x")
-    return ad.cstruct()
+def _lora_inputs(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor) -> int:
+    """Rows of x; checks x and the rows' adapters."""
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise ValueError("adapter activations must be bf16 [M, K]")
+    if ids.dtype != torch.int32 or ids.dim() != 1 or len(ids) != len(x) or not ids.is_contiguous():
+        raise ValueError("ids must be int32 [M], contiguous, one for each row of x")
+    return len(x)
 
 
 def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -393,23 +413,23 @@ def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tens
     """out[m] = y[m] + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m], for the rows of many requests at once: beside any
     projection that gave y (bf16 or fp32 [M, N]). x bf16 [M, K]; a negative id leaves the row as it is (an id >= L too,
     with bit 4 of the context's status set). Sums in fp32, one rounding. out: bf16 or y's type (default: like y); out=y
-    adds in place. x, y and out may be columns of wider tensors (stride(1) == 1)."""
-    cs = _lora_inputs(ad, ids, x)
-    ctx = ctx or Context.default(x.device)
-    M = x.shape[0]
-    if y.dim() != 2 or y.shape[0] != M:
-        raise ValueError("y must have a row for each row of x")
-    ldx, ldy = _rows_of(x, "x", cs.in_features), _rows_of(y, "y", cs.out_features)
+    adds in place, otherwise out must not overlap the inputs. x, y and out may be columns of wider tensors."""
+    M = _lora_inputs(ad, ids, x)
+    cs = ad.cstruct()
+    N = cs.out_features
+    ldx, ldy = _row_stride(x, "x", M, cs.in_features), _row_stride(y, "y", M, N)
+    ydt = y.dtype
     if out is None:
-        out = torch.empty((M, cs.out_features), dtype=y.dtype, device=y.device)
-    ldo = _rows_of(out, "out", cs.out_features)
-    if out.shape[0] != M or y.dtype not in _DTYPE or out.dtype not in (torch.bfloat16, y.dtype):
-        raise ValueError("y must be bf16 or fp32 and out bf16 or y's type, with a row for each row of x")
-    _one_device(ctx, ad.a, ad.b, ad.scale, ad.ranks, ids, x, y, out)
+        out = torch.empty_like(y, memory_format=torch.contiguous_format)
+    ldo = _row_stride(out, "out", M, N)
+    odt = out.dtype
+    if ydt not in _DTYPE or odt not in (torch.bfloat16, ydt):
+        raise ValueError("y must be bf16 or fp32, out bf16 or y's type")
+    ctx, index = _on(ctx, x, ids, y, out, ad.a, ad.b, ad.scale, ad.ranks)
     n = lib().aipu_lora_workspace(M, cs.n_adapters)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    check(lib().aipu_lora_add(ctx.handle, ctypes.byref(cs), _ptr(ids), _ptr(x), ldx, M, _ptr(y), _DTYPE[y.dtype], ldy,
-                              _ptr(out), _DTYPE[out.dtype], ldo, _ptr(ws), n, _stream(x.device)))
+    check(lib().aipu_lora_add(ctx.handle, cs, ids.data_ptr(), x.data_ptr(), ldx, M, y.data_ptr(), _DTYPE[ydt], ldy,
+                              out.data_ptr(), _DTYPE[odt], ldo, ws.data_ptr() if n else None, n, _raw_stream(index)))
     return out
 
 
@@ -418,21 +438,113 @@ def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: 
     """y[m] bf16 = x[m] W^T + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m]: a shared quantised projection (W = N GGUF rows
     of K weights, as in gemm) and the adapters of its rows, rounded once. Few rows run on the decode GEMV, 64 and more of
     Q4_K or Q6_K on the tensor-core GEMM."""
-    _need_cuda(w, x, out)
-    cs = _lora_inputs(ad, ids, x)
-    if x.dim() != 2 or x.shape[1] != K or cs.in_features != K or cs.out_features != N:
+    M = _lora_inputs(ad, ids, x)
+    cs = ad.cstruct()
+    if x.shape[1] != K or cs.in_features != K or cs.out_features != N:
         raise ValueError("x must be [M, K], a [L, R, K] and b [L, N, R]")
+    _contiguous(w=w, x=x, out=out)
     if w.numel() * w.element_size() < N * row_bytes(wtype, K):
         raise ValueError("weight buffer smaller than N * row_bytes")
-    ctx = ctx or Context.default(x.device)
-    M = x.shape[0]
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
+        out = x.new_empty((M, N))
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
         raise ValueError("out must be bf16 [M, N]")
-    _one_device(ctx, w, ad.a, ad.b, ad.scale, ad.ranks, ids, x, out)
+    ctx, index = _on(ctx, x, w, ids, out, ad.a, ad.b, ad.scale, ad.ranks)
     n = lib().aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    check(lib().aipu_q4k_gemm_lora(ctx.handle, wtype, _ptr(w), N, K, _ptr(x), M, ctypes.byref(cs), _ptr(ids), _ptr(out),
-                                   _ptr(ws), n, _stream(x.device)))
+    check(lib().aipu_q4k_gemm_lora(ctx.handle, wtype, w.data_ptr(), N, K, x.data_ptr(), M, cs, ids.data_ptr(),
+                                   out.data_ptr(), ws.data_ptr() if n else None, n, _raw_stream(index)))
     return out
+
+
+# ------------------------------------------------------------------------------------ logits
+@dataclass
+class LogitControls:
+    """Controls of the M rows of a batch of logits [M, V], on the GPU; each group may be left out.
+
+    Penalties: row m's context is tokens[begin:end], tokens[gen:end] of it generated, (begin, gen, end) = spans[m]
+    (int64 [M, 3]; tokens int32 [T]; contexts may overlap, as the rows of a verify pass do). penalties fp32 [M, 3]:
+    repetition (divides positive and multiplies other logits of the context's tokens; 1: none), presence (subtracted
+    from the generated tokens) and frequency (subtracted as often as they were generated).
+    Biases: row m adds bias_vals[i] (fp32) to token bias_ids[i] (int32), bias_begin[m] <= i < bias_begin[m + 1]
+    (int64 [M + 1]).
+    Masks: bit v % 32 of word v // 32 of mask[mask_rows[m]] (int32 [G, ceil(V / 32)], int32 [M]) allows token v;
+    a negative mask row has no mask."""
+
+    tokens: Optional[torch.Tensor] = None
+    spans: Optional[torch.Tensor] = None
+    penalties: Optional[torch.Tensor] = None
+    bias_begin: Optional[torch.Tensor] = None
+    bias_ids: Optional[torch.Tensor] = None
+    bias_vals: Optional[torch.Tensor] = None
+    mask: Optional[torch.Tensor] = None
+    mask_rows: Optional[torch.Tensor] = None
+
+    def tensors(self) -> tuple:
+        return (self.tokens, self.spans, self.penalties, self.bias_begin, self.bias_ids, self.bias_vals, self.mask,
+                self.mask_rows)
+
+    def cstruct(self, M: int, V: int) -> L.LogitCtl:
+        def need(t, name, dtype, shape):
+            if t is None or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
+            return t.data_ptr()
+
+        s = L.LogitCtl()
+        if self.spans is not None or self.penalties is not None or self.tokens is not None:
+            s.spans = need(self.spans, "spans", torch.int64, (M, 3))
+            s.penalties = need(self.penalties, "penalties", torch.float32, (M, 3))
+            n = self.tokens.numel() if self.tokens is not None else 0
+            s.tokens, s.n_tokens = need(self.tokens, "tokens", torch.int32, (n,)), n
+        if self.bias_begin is not None or self.bias_ids is not None or self.bias_vals is not None:
+            s.bias_begin = need(self.bias_begin, "bias_begin", torch.int64, (M + 1,))
+            n = self.bias_ids.numel() if self.bias_ids is not None else 0
+            s.bias_ids, s.n_bias = need(self.bias_ids, "bias_ids", torch.int32, (n,)), n
+            s.bias_vals = need(self.bias_vals, "bias_vals", torch.float32, (n,))
+        if self.mask is not None or self.mask_rows is not None:
+            n = self.mask.shape[0] if self.mask is not None else 0
+            s.mask, s.n_masks = need(self.mask, "mask", torch.int32, (n, (V + 31) // 32)), n
+            s.mask_rows = need(self.mask_rows, "mask_rows", torch.int32, (M,))
+        return s
+
+
+def _logits(logits, controls, ctx, out, want_out):
+    if logits.dim() != 2 or logits.dtype not in _DTYPE:
+        raise ValueError("logits must be bf16 or fp32 [M, V]")
+    M, V = logits.shape
+    ld = _row_stride(logits, "logits", M, V)
+    cs = controls.cstruct(M, V) if controls is not None else None
+    if out is None and want_out:
+        out = torch.empty((M, V), dtype=torch.float32, device=logits.device)
+    ldo = _row_stride(out, "out", M, V) if want_out else 0
+    if want_out and out.dtype != torch.float32:
+        raise ValueError("out must be fp32 [M, V]")
+    token = torch.empty(M, dtype=torch.int32, device=logits.device)
+    ctx, index = _on(ctx, logits, out, *(controls.tensors() if controls is not None else ()))
+    check(lib().aipu_logits_process(ctx.handle, logits.data_ptr(), _DTYPE[logits.dtype], ld, M, V, cs,
+                                    out.data_ptr() if want_out else None, ldo, token.data_ptr(), _raw_stream(index)))
+    return out, token
+
+
+def process_logits(logits: torch.Tensor, controls: Optional[LogitControls] = None, out: Optional[torch.Tensor] = None,
+                   ctx: Optional[Context] = None):
+    """(fp32 [M, V], int32 [M]): the logits (bf16 or fp32 [M, V], rows may be columns of a wider tensor) after each row's
+    penalties, biases and mask, in this order, and the greedy token of each row: the lowest index of the largest value, -1
+    where nothing is above -inf. Every step rounds to fp32. out=logits works in place (fp32)."""
+    return _logits(logits, controls, ctx, out, True)
+
+
+def greedy_tokens(logits: torch.Tensor, controls: Optional[LogitControls] = None,
+                  ctx: Optional[Context] = None) -> torch.Tensor:
+    """int32 [M]: the greedy tokens of process_logits, without writing the processed logits."""
+    return _logits(logits, controls, ctx, None, False)[1]
+
+
+def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
+    """int32 [G, ceil(V / 32)] mask words of a bool [G, V] tensor (True: the token is allowed)."""
+    if allowed.dtype != torch.bool or allowed.dim() != 2:
+        raise ValueError("allowed must be bool [G, V]")
+    G, V = allowed.shape
+    bits = torch.nn.functional.pad(allowed, (0, -V % 32)).view(G, -1, 32)
+    one = torch.ones(32, dtype=torch.int32, device=allowed.device) << torch.arange(32, dtype=torch.int32, device=allowed.device)
+    return torch.where(bits, one, 0).sum(2, dtype=torch.int32)

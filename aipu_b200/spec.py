@@ -16,11 +16,16 @@ the KV-cache write-back of the accepted rows and the AIPUDevice.step backend tha
 maps [rows, H] bf16 hidden states to the next ones, so a caller that owns those parts plugs them in.
 Every row is computed independently and bit-exactly, so a row's result does not depend on how many
 rows share the pass (M = K + 1 rows give the same bits as K + 1 single-row passes).
+
+A Request carries what one request asks of its tokens: its adapter on the LM head (ops.lora_add), and
+penalties, biases and a mask on the logits before the argmax (ops.greedy_tokens). Row j of a pass is
+then judged by the request's context with the drafts before it, so the committed stream equals greedy
+decoding under the same controls.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
@@ -54,14 +59,60 @@ class SpecStats:
         return self.committed / self.passes if self.passes else 0.0
 
 
+@dataclass
+class Request:
+    """One request: its context (the last token is the next pass's input), of which the first n_prompt tokens were
+    given and the rest generated, and the controls of its tokens. mask(context) gives the packed mask words (int32
+    [ceil(V / 32)], ops.pack_mask) of the token that follows a context, or None for no mask. adapter: its row in the
+    verifier's head adapters, negative for none."""
+
+    context: List[int]
+    n_prompt: int = 0
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: Dict[int, float] = field(default_factory=dict)
+    mask: Optional[Callable[[Sequence[int]], Optional[torch.Tensor]]] = None
+    adapter: int = -1
+
+    def controls(self, drafts: Sequence[int], device) -> ops.LogitControls:
+        """Controls of the rows {context, context + d_1, ..}: one shared run of tokens, each row's context ends at its
+        own input token."""
+        M, n = len(drafts) + 1, len(self.context)
+        tokens = list(self.context) + [int(d) for d in drafts]
+        spans = [[0, min(self.n_prompt, n), n + j] for j in range(M)]
+        c = ops.LogitControls(
+            tokens=torch.tensor(tokens, dtype=torch.int32, device=device),
+            spans=torch.tensor(spans, dtype=torch.int64, device=device),
+            penalties=torch.tensor([[self.repetition, self.presence, self.frequency]] * M, dtype=torch.float32, device=device))
+        if self.bias:
+            b = len(self.bias)
+            c.bias_begin = torch.arange(M + 1, device=device) * b
+            c.bias_ids = torch.tensor(list(self.bias.keys()) * M, dtype=torch.int32, device=device)
+            c.bias_vals = torch.tensor(list(self.bias.values()) * M, dtype=torch.float32, device=device)
+        if self.mask is not None:
+            words = [self.mask(tokens[:n + j]) for j in range(M)]
+            live = [w for w in words if w is not None]
+            if live:
+                rows, at = [], 0
+                for w in words:
+                    rows.append(-1 if w is None else at)
+                    at += w is not None
+                c.mask = torch.stack([w.to(device) for w in live]).contiguous()
+                c.mask_rows = torch.tensor(rows, dtype=torch.int32, device=device)
+        return c
+
+
 class SpecVerifier:
     """Verify passes of K drafts over the MoE decode stack.
 
     emb: bf16 [V, H] token rows; lm_head: bf16 [V, H] (rows of the output projection);
-    stack: list of ops.MoeLayerWeights (applied in turn on one GPU) or a callable [M, H] -> [M, H].
+    stack: list of ops.MoeLayerWeights (applied in turn on one GPU) or a callable [M, H] -> [M, H];
+    head_adapters: low-rank adapters of the LM head (a [L, R, H], b [L, V, R]) that requests name.
     """
 
-    def __init__(self, emb: torch.Tensor, lm_head: torch.Tensor, stack, ctx: Optional[ops.Context] = None):
+    def __init__(self, emb: torch.Tensor, lm_head: torch.Tensor, stack, ctx: Optional[ops.Context] = None,
+                 head_adapters: Optional[ops.LoraAdapters] = None):
         if emb.dtype != torch.bfloat16 or lm_head.dtype != torch.bfloat16 or emb.dim() != 2 or lm_head.dim() != 2:
             raise ValueError("emb and lm_head must be bf16 [V, H]")
         if emb.shape[1] != lm_head.shape[1]:
@@ -69,6 +120,7 @@ class SpecVerifier:
         self.emb = emb
         self.lm_head = lm_head
         self.ctx = ctx
+        self.head_adapters = head_adapters
         if callable(stack):
             self._stack: Callable[[torch.Tensor], torch.Tensor] = stack
         else:
@@ -82,18 +134,34 @@ class SpecVerifier:
             self._stack = run
         self.stats = SpecStats()
 
-    def greedy_tokens(self, rows: Sequence[int]) -> List[int]:
-        """m_j = argmax of the LM head over the stack's output for token row j (lowest index on ties)."""
+    def greedy_tokens(self, rows: Sequence[int], request: Optional[Request] = None) -> List[int]:
+        """m_j = argmax of the LM head over the stack's output for token row j (lowest index on ties); for a request, of
+        its adapted logits under its controls (-1 where its mask leaves nothing)."""
         idx = torch.as_tensor(list(rows), dtype=torch.long, device=self.emb.device)
         h = self._stack(self.emb.index_select(0, idx).contiguous())
         logits = ops.bf16_dot_gemv(self.lm_head, h, ctx=self.ctx)
-        return [int(v) for v in logits.float().argmax(dim=1).cpu().tolist()]
+        if request is None:
+            return [int(v) for v in logits.float().argmax(dim=1).cpu().tolist()]
+        if self.head_adapters is not None and request.adapter >= 0:
+            ids = torch.full((len(rows),), request.adapter, dtype=torch.int32, device=h.device)
+            logits = ops.lora_add(self.head_adapters, ids, h, logits, out=logits, ctx=self.ctx)
+        return ops.greedy_tokens(logits, request.controls(rows[1:], h.device), ctx=self.ctx).cpu().tolist()
 
-    def verify(self, cur_tok: int, drafts: Sequence[int]):
-        """One pass over {cur_tok, d_1..d_K}: returns (committed tokens m_1..m_{p+1}, p)."""
-        truth = self.greedy_tokens([cur_tok] + list(drafts))
+    def verify(self, cur_tok: int, drafts: Sequence[int], request: Optional[Request] = None):
+        """One pass over {cur_tok, d_1..d_K}: returns (committed tokens m_1..m_{p+1}, p). A request's context must end
+        with cur_tok; the committed tokens are added to it. Where its mask leaves no token, the committed ones end."""
+        if request is not None:
+            if not request.context or request.context[-1] != cur_tok:
+                raise ValueError("a request's context must end with cur_tok")
+            if request.adapter >= 0 and (self.head_adapters is None or request.adapter >= self.head_adapters.a.shape[0]):
+                raise ValueError("the request names an adapter that the verifier does not have")
+        truth = self.greedy_tokens([cur_tok] + list(drafts), request)
         p = longest_accepted_prefix(drafts, truth)
         committed = truth[:p + 1]
+        if request is not None:
+            if committed[-1] < 0:
+                committed.pop()
+            request.context.extend(committed)
         s = self.stats
         s.passes += 1
         s.drafted += len(drafts)
@@ -102,13 +170,18 @@ class SpecVerifier:
         s.accepted_per_pass.append(p)
         return committed, p
 
-    def generate(self, cur_tok: int, n_tokens: int, draft_fn: Callable[[int, int], Sequence[int]], k: int):
+    def generate(self, cur_tok: int, n_tokens: int, draft_fn: Callable[[int, int], Sequence[int]], k: int,
+                 request: Optional[Request] = None):
         """Commit n_tokens tokens after cur_tok with K-draft verify passes; draft_fn(tok, k) proposes
-        the next k tokens after tok."""
+        the next k tokens after tok. With a request, fewer where its mask leaves none."""
         out: List[int] = []
         tok = cur_tok
         while len(out) < n_tokens:
-            committed, _ = self.verify(tok, list(draft_fn(tok, k))[:k])
+            committed, _ = self.verify(tok, list(draft_fn(tok, k))[:k], request)
+            if not committed:
+                break
             out.extend(committed)
             tok = committed[-1]
+        if request is not None and len(out) > n_tokens:  # committed by the last pass, but not asked for
+            del request.context[n_tokens - len(out):]
         return out[:n_tokens]

@@ -295,6 +295,41 @@ int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M,
 int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,
                        const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes, void* stream);
 
+/* Controls of the rows of a batch of logits. A group that is not used is NULL. */
+typedef struct aipu_logit_ctl {
+  /* penalties: row m's context is tokens[begin, end), of which tokens[gen, end) were generated, with
+   * (begin, gen, end) = spans[3 m ..]; contexts may overlap. penalties[3 m ..] = repetition, presence,
+   * frequency (1, 0, 0: none). Tokens outside 0 .. V - 1 count for nothing. */
+  const int32_t* tokens;
+  int64_t n_tokens;
+  const int64_t* spans;     /* [M, 3] */
+  const float* penalties;   /* [M, 3] */
+  /* biases: row m adds bias_vals[i] to token bias_ids[i] for bias_begin[m] <= i < bias_begin[m + 1] */
+  const int64_t* bias_begin; /* [M + 1] */
+  const int32_t* bias_ids;
+  const float* bias_vals;
+  int64_t n_bias;
+  /* masks: token v is allowed in row m if bit v % 32 of word v / 32 of mask mask_rows[m] is set; a
+   * negative row has no mask */
+  const uint32_t* mask;     /* [n_masks, ceil(V / 32)] */
+  const int32_t* mask_rows; /* [M] */
+  int64_t n_masks;
+} aipu_logit_ctl;
+
+/* Processed logits out[M, V] (fp32; NULL: not written) and greedy tokens token[M] (NULL: not wanted) of
+ * logits[M, V] (bf16 or fp32, ld elements between rows). Steps, each rounded to fp32:
+ *   z = z > 0 ? z / repetition : z * repetition   if the token occurs in the row's context
+ *   z = z - frequency * count, z = z - presence   if it occurs count > 0 times in the generated part
+ *   z = z + bias                                  every entry of the row for the token, in list order
+ *   z = -inf                                      if the row's mask does not allow it
+ * token = the lowest index of the largest z (NaN is never the largest), -1 if no z is above -inf (a mask
+ * that leaves nothing). ctl may be NULL. out may be logits (fp32, same stride). A span or bias range that
+ * leaves its array is cut to it, and a mask row >= n_masks acts as -1; both set bit 4 of the context's
+ * status word. No scratch: calls may run at the same time. Equal calls give equal bits. No counterpart in
+ * the reference (its sampler takes the argmax, as ctl = NULL does). */
+int aipu_logits_process(aipu_ctx* ctx, const void* logits, int dtype, int64_t ld, int64_t M, int64_t V,
+                        const aipu_logit_ctl* ctl, float* out, int64_t ldo, int32_t* token, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
