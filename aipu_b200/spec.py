@@ -155,7 +155,8 @@ class SpecVerifier:
                 raise ValueError("a request's context must end with cur_tok")
             if request.adapter >= 0 and (self.head_adapters is None or request.adapter >= self.head_adapters.a.shape[0]):
                 raise ValueError("the request names an adapter that the verifier does not have")
-        truth = self.greedy_tokens([cur_tok] + list(drafts), request)
+        rows = [cur_tok] + list(drafts)
+        truth = self.greedy_tokens(rows) if request is None else self.greedy_tokens(rows, request)
         p = longest_accepted_prefix(drafts, truth)
         committed = truth[:p + 1]
         if request is not None:
