@@ -135,10 +135,28 @@ def test_a_long_context_and_many_rows():
     _run(200, 777, history=300, bias=7, masks=5)
 
 
+@pytest.mark.parametrize("n", [32767, 32768, 70000])
+def test_counts_that_pass_sixteen_bits(n):
+    """One token generated n times beside others, and n times in the prompt of another row."""
+    d = _dev()
+    V = 45000
+    rng = np.random.default_rng(n)
+    x, x_np = _logits(rng, 2, V, torch.float32, d)
+    gen = np.full(n, 4321, np.int32)
+    c = dict(tokens=np.concatenate([gen, [4320, 4322, 44999, 4321]]).astype(np.int32),
+             spans=np.array([[0, 0, n + 3], [0, n + 3, n + 4]], np.int64),
+             penalties=np.array([[1.1, 0.5, 2.0 ** -9], [1.2, 0.25, 1.0]], F32))
+    out, tok = ops.process_logits(x, _dev_controls(c, d))
+    z, t = oracle(x_np, **c)
+    np.testing.assert_array_equal(out.cpu().numpy(), z)
+    np.testing.assert_array_equal(tok.cpu().numpy(), t)
+
+
 def test_a_vocabulary_of_several_windows():
     """More tokens than a cluster counts at once: the context is scanned for each part."""
     _run(2, 250001, torch.float32, history=900, bias=300, masks=1)
     _run(1, 600000, history=900, bias=300, repeat=True, masks=1)
+    _run(1, 400003, history=300000, bias=30, seed=5)
 
 
 def test_rows_a_mask_leaves_nothing_of_and_values_that_are_not_finite():
