@@ -102,10 +102,10 @@ SIGNATURES = {
     "aipu_ep_destroy": (c_int, [c_void_p]),
     "aipu_logits_process": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, ctypes.POINTER(LogitCtl),
                                     c_void_p, c_int64, c_void_p, c_void_p]),
-    "aipu_lora_workspace": (c_int64, [c_int64, c_int64]),
+    "aipu_lora_workspace": (c_int64, [c_int64, c_int64, c_int64]),
     "aipu_lora_add": (c_int, [c_void_p, ctypes.POINTER(Lora), c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
                               c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p]),
-    "aipu_q4k_gemm_lora_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64, c_int64]),
+    "aipu_q4k_gemm_lora_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64, c_int64, c_int64]),
     "aipu_q4k_gemm_lora": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                    ctypes.POINTER(Lora), c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
 }

@@ -1339,9 +1339,9 @@ static int lora_params(const aipu_lora* ad, const int32_t* ids, int64_t M, LoraP
   return OK;
 }
 
-extern "C" int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters) {
-  if (M < 0 || M > (1 << 24) || n_adapters < 1 || n_adapters > 32768) return 0;
-  return static_cast<int64_t>(lora_plan_bytes(M, n_adapters));
+extern "C" int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters, int64_t rank) {
+  if (M < 0 || M > (1 << 24) || n_adapters < 1 || n_adapters > 32768 || rank < 1 || rank > 128) return 0;
+  return static_cast<int64_t>(lora_plan_bytes(M, n_adapters, rank));
 }
 
 extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
@@ -1356,7 +1356,8 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
     return set_error(EINVAL_, "lora_add: y and out must be bf16, fp32, or fp32 and bf16");
   if (out && out == y && (y_dtype != out_dtype || ldy != ldo))
     return set_error(EINVAL_, "lora_add: in place needs the same type and row stride");
-  if ((reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < aipu_lora_workspace(M, p.L) || (!ws && aipu_lora_workspace(M, p.L) > 0))
+  const int64_t need = aipu_lora_workspace(M, p.L, p.R);
+  if ((reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < need || (!ws && need > 0))
     return set_error(EINVAL_, "lora_add: workspace missing, too small or not 16-byte aligned");
   if (!c) return set_error(EINVAL_, "lora_add: null context");
   if (M == 0) return OK;
@@ -1371,18 +1372,19 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
   p.status = c->status;
   DeviceGuard dg(c->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if ((rc = lora_plan_launch(p, ws, s, false))) return rc;
-  return lora_launch(p, c->num_sms, s, (c->flags & AIPU_FLAG_PDL) != 0);
+  const bool pdl = (c->flags & AIPU_FLAG_PDL) != 0;
+  if ((rc = lora_begin(p, ws, s, pdl))) return rc;
+  return lora_finish(p, s, pdl || p.tiles);
 }
 
 // rows from which the projection runs on the tcgen05 GEMM
 static bool gemm_lora_tc(int wtype, int64_t M) { return (wtype == AIPU_Q4_K || wtype == AIPU_Q6_K) && M >= 64; }
 
-extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters) {
+extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank) {
   if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
-      n_adapters > 32768)
+      n_adapters > 32768 || rank < 1 || rank > 128)
     return 0;
-  size_t b = al256x(lora_plan_bytes(M, n_adapters)) + al256x(4 * static_cast<size_t>(M) * N);
+  size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * static_cast<size_t>(M) * N);
   if (gemm_lora_tc(wtype, M)) b += al256x(xt_bytes(M, K)) + al256x(4 * M);
   return static_cast<int64_t>(b);
 }
@@ -1398,7 +1400,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     return set_error(EINVAL_, "gemm_lora: bad arguments (GGUF rows, K % 256 == 0, adapters of the same K and N)");
   if ((reinterpret_cast<uintptr_t>(w) & 15u) || (reinterpret_cast<uintptr_t>(x) & 15u))
     return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned");
-  if ((M > 0 && !ws) || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L))
+  if ((M > 0 && !ws) || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L, p.R))
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
   if (!c) return set_error(EINVAL_, "gemm_lora: null context");
   if (M == 0) return OK;
@@ -1407,7 +1409,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* b = static_cast<uint8_t*>(ws);
   void* plan = b;
-  b += al256x(lora_plan_bytes(M, p.L));
+  b += al256x(lora_plan_bytes(M, p.L, p.R));
   float* y32 = reinterpret_cast<float*>(b);
   b += al256x(4 * static_cast<size_t>(M) * N);
   p.x = static_cast<const uint16_t*>(x);
@@ -1417,7 +1419,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   p.out = y;
   p.y_f32 = 1;
   p.status = c->status;
-  if ((rc = lora_plan_launch(p, plan, s, false))) return rc;
+  if ((rc = lora_begin(p, plan, s, false))) return rc;
   if (gemm_lora_tc(wtype, M)) {
     uint8_t* xt = b;
     int* shift = reinterpret_cast<int*>(xt + al256x(xt_bytes(M, K)));
@@ -1457,7 +1459,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   }
   if (rc) return rc;
   p.wait_y = 1;
-  return lora_launch(p, c->num_sms, s, true);
+  return lora_finish(p, s, true);
 }
 
 // ------------------------------------------------------------------ logits

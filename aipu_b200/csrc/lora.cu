@@ -8,7 +8,8 @@
 // before the tensor pipe; mma.sync, whose fragments come straight from global memory, feeds it without
 // a trip through shared memory or TMEM.
 //
-// One cluster of CTAs takes one tile: up to 8 * NT rows that share an adapter.
+// Up to kDirectRows rows: ONE launch. A cluster of CTAs takes a tile of up to 8 rows that share an adapter
+// (found by two ballots over the ids).
 //   1. CTA c and its 8 warps each take a share of K. Rank rows are the 16 MMA rows, token rows the 8
 //      MMA columns; a lane loads 8 consecutive k of its rows (16 bytes) and uses them as two MMA steps
 //      whose k order is permuted the same way on both sides.
@@ -16,8 +17,11 @@
 //      shared memory, always in the same order (no atomics: equal calls give equal bits).
 //   3. CTA c and its warps each take 64-column blocks of N. The MMA's rows are columns of y, ordered so
 //      that a lane ends with 8 consecutive columns of a row: y is read and written 16 bytes at a time.
-// So a call is one launch (and a plan of the rows by adapter when there are more than kDirectRows), h
-// never leaves the chip, and the reads of B do not wait for the sums of A.
+//   h never leaves the chip, and the reads of B and y do not wait for the sums of A.
+// More rows: a plan (rows ordered by adapter, tiles of up to 64 of them), the first product (a tile and a
+// share of K a CTA: x and A stream through a ring of asynchronous copies in shared memory, partial sums to
+// global memory), the second product (a tile and a share of N a CTA: step 3 above). As one cluster kernel
+// this took 119 us for 4096 rows, because its phases followed one another with one CTA an SM.
 //
 // Rounding: bf16 x and A products are exact in the MMA, sums are fp32. h is not rounded to 16 bits: it
 // enters the second product as 2 (bf16 result) or 3 (fp32 result) bf16 pieces, 16 and 24 bits. fp16
@@ -34,7 +38,8 @@ namespace aipu {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kDirectRows = 64;      // rows for which every cluster finds its tile itself
+constexpr int kDirectRows = 64;      // rows of the one-launch kernel
+constexpr int kDirectCtas = 8;       // CTAs of its clusters
 constexpr int kMaxAdapters = 32768;  // counters of the plan kernel in shared memory
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -103,17 +108,18 @@ __device__ __forceinline__ void split4_f16(const uint4& v, uint4& hi, uint4& lo)
   split_f16(v.w, hi.w, lo.w);
 }
 
-template <int MT, int NT>
+constexpr int kDirectTile = 8;  // rows of a tile of the one-launch kernel
+template <int MT>
 struct LoraCfg {
-  static constexpr int TM = 8 * NT;                  // rows of a tile
+  static constexpr int TM = kDirectTile;
   static constexpr int RP = 16 * MT;                 // rank rows
   static constexpr int RF = RP < 32 ? 32 : RP;       // rank columns of the second product (steps of 32)
   static constexpr int HPITCH = RF + 8;              // bf16 pitch of a token's h (16-byte rows, banks spread)
-  static constexpr int COPIES = NT == 1 ? kLoraWarps : kLoraWarps / 2;
-  static constexpr int OFF_HP = 0;                   // fp32 [TM][RP]: this CTA's sums
-  static constexpr int OFF_HF = OFF_HP + TM * RP * 4;  // bf16 [3][TM][HPITCH]: scale * h
+  static constexpr int PITCH = RP + 4;               // fp32 pitch of a token's sums (banks spread)
+  static constexpr int OFF_HP = 0;                   // fp32 [TM][PITCH]: this CTA's sums
+  static constexpr int OFF_HF = OFF_HP + TM * PITCH * 4;  // bf16 [3][TM][HPITCH]: scale * h
   static constexpr int OFF_RED = OFF_HF + 3 * TM * HPITCH * 2;
-  static constexpr int TOTAL = OFF_RED + COPIES * TM * RP * 4;
+  static constexpr int TOTAL = OFF_RED + kLoraWarps * TM * PITCH * 4;
 };
 
 struct LoraTile {
@@ -122,14 +128,15 @@ struct LoraTile {
 };
 
 // ------------------------------------------------------------------ first product: this warp's k range
-template <int MT, int NT, int AT, bool VEC>
+template <int MT, int AT, bool VEC>
 __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, const LoraTile& tl, int c0, int c1, int lane,
-                                       float (&acc)[MT][NT][4]) {
-  constexpr int U = NT > 1 ? 1 : (MT == 1 ? 4 : MT == 2 ? 2 : 1);  // k chunks loaded ahead
+                                       float (&acc)[MT][4]) {
+  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1;  // k chunks loaded ahead
   const int g = lane >> 2, t = lane & 3;
   const uint16_t* abase = static_cast<const uint16_t*>(p.a) + static_cast<int64_t>(tl.id) * p.R * p.K;
+  const uint16_t* xrow = p.x + static_cast<int64_t>(tok[g]) * p.ldx;
   for (int c = c0; c < c1; c += U) {
-    uint4 va[U][MT][2], vx[U][NT];
+    uint4 va[U][MT][2], vx[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (c + u) * 32 + 8 * t;
@@ -141,11 +148,7 @@ __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, cons
           const int r = 16 * i + 8 * h + g;
           va[u][i][h] = load8<VEC>(abase + static_cast<int64_t>(r) * p.K + k, r < tl.rank ? valid : 0, p.wa);
         }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int m = 8 * j + g;
-        vx[u][j] = load8<VEC>(p.x + static_cast<int64_t>(tok[m]) * p.ldx + k, m < tl.rows ? valid : 0, p.wx);
-      }
+      vx[u] = load8<VEC>(xrow + k, g < tl.rows ? valid : 0, p.wx);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -156,28 +159,41 @@ __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, cons
           uint4 ah, al, bh, bl;
           split4_f16(va[u][i][0], ah, al);
           split4_f16(va[u][i][1], bh, bl);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (NT > 1 && 8 * j >= tl.rows) continue;
-            mma_pair(acc[i][j], ah, bh, vx[u][j]);
-            mma_pair(acc[i][j], al, bl, vx[u][j]);
-          }
+          mma_pair(acc[i], ah, bh, vx[u]);
+          mma_pair(acc[i], al, bl, vx[u]);
         } else {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (NT > 1 && 8 * j >= tl.rows) continue;
-            mma_pair(acc[i][j], va[u][i][0], va[u][i][1], vx[u][j]);
-          }
+          mma_pair(acc[i], va[u][i][0], va[u][i][1], vx[u]);
         }
       }
   }
 }
 
 // ------------------------------------------------------------------ second product and the result rows
-// acc2[j][nt]: MMA j's rows g and g + 8 are columns n0 + 8 g + 2 j and + 2 j + 1 of y
-template <int NT>
+// acc[q][j]: MMA q's rows g and g + 8 are columns n0 + 8 g + 2 q and + 2 q + 1 of y, its columns 2 t and
+// 2 t + 1 the rows 8 (nt0 + j) + 2 t (+ 1) of the tile. Rows of y, 8 columns a lane, loaded ahead:
+template <int NT, bool Y32>
+struct YTile {
+  uint4 v[NT][2][Y32 ? 2 : 1];
+  __device__ __forceinline__ void load(const LoraParams& p, const int* tok, int rows, int n0, int lane, int nt0) {
+    const int g = lane >> 2, t = lane & 3, n = n0 + 8 * g;
+    if (!p.vy || n + 8 > p.N) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int m = 8 * (nt0 + j) + 2 * t + e;
+        if (m >= rows) continue;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.y) +
+                                                          (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < (Y32 ? 2 : 1); ++i) v[j][e][i] = src[i];
+      }
+  }
+};
+
+template <int NT, bool Y32>
 __device__ __forceinline__ void store_rows(const LoraParams& p, const int* tok, int rows, int n0, int lane,
-                                           const float (&acc)[4][NT][4], int nt0) {
+                                           const float (&acc)[4][NT][4], const YTile<NT, Y32>& yt, int nt0) {
   const int g = lane >> 2, t = lane & 3;
   const int n = n0 + 8 * g;
   if (n >= p.N) return;
@@ -196,43 +212,48 @@ __device__ __forceinline__ void store_rows(const LoraParams& p, const int* tok, 
         d[2 * q + 1] = acc[q][j][2 + e];
       }
       if (p.vy && cols == 8) {
-        if (p.y_f32) {
-          const float4* yp = reinterpret_cast<const float4*>(static_cast<const float*>(p.y) + row * p.ldy + n);
-          const float4 v0 = yp[0], v1 = yp[1];
-          d[0] = __fadd_rn(v0.x, d[0]); d[1] = __fadd_rn(v0.y, d[1]); d[2] = __fadd_rn(v0.z, d[2]); d[3] = __fadd_rn(v0.w, d[3]);
-          d[4] = __fadd_rn(v1.x, d[4]); d[5] = __fadd_rn(v1.y, d[5]); d[6] = __fadd_rn(v1.z, d[6]); d[7] = __fadd_rn(v1.w, d[7]);
-        } else {
-          const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.y) + row * p.ldy + n);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(yt.v[j][e]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            d[2 * i] = __fadd_rn(__uint_as_float(w[i] << 16), d[2 * i]);
-            d[2 * i + 1] = __fadd_rn(__uint_as_float(w[i] & 0xFFFF0000u), d[2 * i + 1]);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float y = Y32 ? __uint_as_float(w[Y32 ? i : 0])
+                              : __uint_as_float((i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+          d[i] = __fadd_rn(y, d[i]);
         }
-        if (p.out_f32) {
+        if (Y32 && p.out_f32) {
           float4* op = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + n);
           op[0] = make_float4(d[0], d[1], d[2], d[3]);
           op[1] = make_float4(d[4], d[5], d[6], d[7]);
         } else {
-          uint32_t w[4];
+          uint32_t o[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            w[i] = bf16_rne_bits(d[2 * i]) | (static_cast<uint32_t>(bf16_rne_bits(d[2 * i + 1])) << 16);
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + n) = make_uint4(w[0], w[1], w[2], w[3]);
+            o[i] = bf16_rne_bits(d[2 * i]) | (static_cast<uint32_t>(bf16_rne_bits(d[2 * i + 1])) << 16);
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + n) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (i >= cols) break;
-          const float y = p.y_f32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
-                                  : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
+          const float y = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
+                              : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
           const float v = __fadd_rn(y, d[i]);
-          if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + n + i] = v;
+          if (Y32 && p.out_f32) static_cast<float*>(p.out)[row * p.ldo + n + i] = v;
           else static_cast<uint16_t*>(p.out)[row * p.ldo + n + i] = bf16_rne_bits(v);
         }
       }
     }
+}
+
+// scale * h of one token and two ranks as packed bf16 pieces
+__device__ __forceinline__ void pieces(float2 v, int ns, uint32_t (&w)[3]) {
+  float r0, r1, q0, q1;
+  w[0] = piece(v.x, r0) | (piece(v.y, r1) << 16);
+  if (ns == 2) {
+    w[1] = bf16_rne_bits(r0) | (static_cast<uint32_t>(bf16_rne_bits(r1)) << 16);
+  } else {
+    w[1] = piece(r0, q0) | (piece(r1, q1) << 16);
+    w[2] = (__float_as_uint(q0) >> 16) | (__float_as_uint(q1) & 0xFFFF0000u);
+  }
 }
 
 // B rows n0 + 8 g + 2 j (+ 1) for j = 0..3, rank columns r .. r + 7 (past the rank: 0, whatever is stored)
@@ -289,10 +310,20 @@ __device__ __forceinline__ void expand_step(float (&acc)[4][NTG][4], const uint4
   }
 }
 
-template <int MT, int NT, int AT, bool VEC>
+// Adapter, rank and factor of a tile (id < 0: none)
+__device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int id, int rows) {
+  LoraTile tl = {id, rows, 0, 1.f};
+  if (id >= 0) {
+    tl.rank = p.ranks ? min(max(p.ranks[id], 0), p.R) : p.R;
+    if (p.scale) tl.scale = p.scale[id];
+  }
+  return tl;
+}
+
+template <int MT, int AT, bool VEC, bool Y32>
 __global__ void __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
-  using C = LoraCfg<MT, NT>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  using C = LoraCfg<MT>;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[C::TM];
   float* hp = reinterpret_cast<float*>(smem + C::OFF_HP);
   uint16_t* hf = reinterpret_cast<uint16_t*>(smem + C::OFF_HF);
@@ -300,219 +331,378 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t crank = cluster_rank(), csize = cluster_size();
-  const int n_clusters = gridDim.x / csize, cl = blockIdx.x / csize;
+  const int lead = blockIdx.x / csize;  // the row that this cluster's tile would begin with
   const int ns = p.out_f32 ? 3 : 2;
   constexpr int HS = C::TM * C::HPITCH;  // elements of one piece
   // x (and the ids) may come from the kernel before the one that writes y, so they wait too unless the
   // launch says that only y does
   if (!p.wait_y) pdl_wait();
-  for (int i = tid; i < 3 * HS / 2; i += kLoraThreads) reinterpret_cast<uint32_t*>(hf)[i] = 0;
 
-  const int total = p.tiles ? *p.n_tiles : p.M;
-  bool pending = false;  // a cluster_arrive whose wait is still due
-  for (int ti = cl; ti < total; ti += n_clusters) {
-    // ---- the tile: rows that share an adapter
-    LoraTile tl;
-    if (p.tiles) {
-      const int4 v = p.tiles[ti];
-      tl.id = v.x;
-      tl.rows = v.z;
-      __syncthreads();  // the last tile's readers of tok are done
-      for (int i = tid; i < C::TM; i += kLoraThreads) tok[i] = i < v.z ? p.perm[v.y + i] : 0;
-    } else {
-      // row ti leads a tile if the number of earlier rows with its id is a multiple of the tile's rows;
-      // the tile is that row and the following ones of the id (at most kDirectRows rows in all)
-      const int n0 = lane < p.M ? p.ids[lane] : -2, n1 = lane + 32 < p.M ? p.ids[lane + 32] : -2;
-      const int mine = p.ids[ti];
-      int id = mine;
-      if (id < 0 || id >= p.L) {
-        if (id >= p.L && crank == 0 && tid == 0 && p.status) atomicOr(p.status, ST_BAD_ARGS);
-        id = -1;
-      }
-      auto same = [&](int v, int row) { return row < p.M && (id < 0 ? (v < 0 || v >= p.L) : v == id); };
-      const uint32_t b0 = __ballot_sync(0xffffffffu, same(n0, lane));
-      const uint32_t b1 = __ballot_sync(0xffffffffu, same(n1, lane + 32));
-      const uint64_t all = static_cast<uint64_t>(b1) << 32 | b0;
-      const uint64_t below = (1ull << ti) - 1;
-      if (__popcll(all & below) % C::TM != 0) continue;  // the same for every thread of the cluster
-      tl.id = id;
-      const uint64_t rest = all & ~below;
-      tl.rows = min(C::TM, __popcll(rest));
-      __syncthreads();
-      if (warp == 0) {
-        for (int i = lane; i < C::TM; i += 32) tok[i] = 0;
-        __syncwarp();
-        for (int h = 0; h < 2; ++h) {
-          const int row = lane + 32 * h;
-          if ((rest >> row) & 1) {
-            const int at = __popcll(rest & ((1ull << row) - 1));
-            if (at < C::TM) tok[at] = row;
-          }
-        }
+  // row `lead` leads a tile if the number of earlier rows with its id is a multiple of the tile's rows; the
+  // tile is that row and the following ones of the id
+  const int n0 = lane < p.M ? p.ids[lane] : -2, n1 = lane + 32 < p.M ? p.ids[lane + 32] : -2;
+  int id = p.ids[lead];
+  if (id < 0 || id >= p.L) {
+    if (id >= p.L && crank == 0 && tid == 0 && p.status) atomicOr(p.status, ST_BAD_ARGS);
+    id = -1;
+  }
+  const LoraTile own = lora_tile(p, id, 0);
+  auto same = [&](int v, int row) { return row < p.M && (id < 0 ? (v < 0 || v >= p.L) : v == id); };
+  const uint32_t b0 = __ballot_sync(0xffffffffu, same(n0, lane));
+  const uint32_t b1 = __ballot_sync(0xffffffffu, same(n1, lane + 32));
+  const uint64_t all = static_cast<uint64_t>(b1) << 32 | b0;
+  const uint64_t below = (1ull << lead) - 1;
+  // (the same for every thread of the cluster)
+  if (__popcll(all & below) % C::TM != 0 || (id < 0 && p.skip_plain)) {
+    pdl_launch_dependents();
+    if (p.wait_y) pdl_wait();  // a cluster without a tile may not end before what it depends on
+    return;
+  }
+  const uint64_t rest = all & ~below;
+  LoraTile tl = own;
+  tl.rows = min(C::TM, __popcll(rest));
+  if (warp == 0) {
+    if (lane < C::TM) tok[lane] = 0;
+    __syncwarp();
+    for (int h = 0; h < 2; ++h) {
+      const int row = lane + 32 * h;
+      if ((rest >> row) & 1) {
+        const int at = __popcll(rest & ((1ull << row) - 1));
+        if (at < C::TM) tok[at] = row;
       }
     }
+  }
+  if (C::RF > C::RP)  // rank columns that the second product reads and the first does not give
+    for (int i = tid; i < 3 * C::TM * (C::HPITCH - C::RP); i += kLoraThreads)
+      hf[(i / (C::HPITCH - C::RP)) * C::HPITCH + C::RP + i % (C::HPITCH - C::RP)] = 0;
+  __syncthreads();
+
+  const int nblk = (p.N + 63) / 64;
+  const int gw = crank * kLoraWarps + warp, nw = csize * kLoraWarps;
+  uint4 vb[8];
+  YTile<1, Y32> yt;
+  if (!p.wait_y && gw < nblk) yt.load(p, tok, tl.rows, gw * 64, lane, 0);
+  bool pending = false;
+  if (tl.rank > 0) {
+    // ---- first product: this warp's share of K
+    float acc[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[i][q] = 0.f;
+    const int chunks = (p.K + 31) / 32;
+    const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * gw / nw);
+    const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (gw + 1) / nw);
+    shrink<MT, AT, VEC>(p, tok, tl, c0, c1, lane, acc);
+    // the first block's B rows are on the way while the sums are joined
+    if (gw < nblk) load_b<VEC>(p, tl, gw * 64, 8 * t, g, vb);
+    // ---- sums over the warps of the CTA, in warp order
+    float* mine = red + warp * C::TM * C::PITCH;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mine[(2 * t + (q & 1)) * C::PITCH + 16 * i + g + 8 * (q >> 1)] = acc[i][q];
     __syncthreads();
-    if (tl.id < 0 && p.skip_plain) continue;  // uniform over the cluster
-    tl.rank = 0;
-    tl.scale = 1.f;
-    if (tl.id >= 0) {
-      tl.rank = p.ranks ? min(max(p.ranks[tl.id], 0), p.R) : p.R;
-      if (p.scale) tl.scale = p.scale[tl.id];
+    for (int e = tid; e < C::TM * C::PITCH; e += kLoraThreads) {
+      float v = red[e];
+#pragma unroll
+      for (int w = 1; w < kLoraWarps; ++w) v = __fadd_rn(v, red[w * C::TM * C::PITCH + e]);
+      hp[e] = v;
     }
-
-    const int nblk = (p.N + 63) / 64;
-    const int gw = crank * kLoraWarps + warp, nw = csize * kLoraWarps;
-    uint4 vb[8];
-    if (tl.rank > 0) {
-      // ---- first product: this warp's share of K
-      float acc[MT][NT][4];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
-      const int chunks = (p.K + 31) / 32;
-      const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * gw / nw);
-      const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (gw + 1) / nw);
-      shrink<MT, NT, AT, VEC>(p, tok, tl, c0, c1, lane, acc);
-      // the first block's B rows are on the way while the sums are joined
-      if (NT == 1 && gw < nblk) load_b<VEC>(p, tl, gw * 64, 8 * t, g, vb);
-
-      // ---- sums over the warps of the CTA, in warp order (fixed tree for the large tile)
-      auto put = [&](float* dst) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              dst[(8 * j + 2 * t + (q & 1)) * C::RP + 16 * i + g + 8 * (q >> 1)] = acc[i][j][q];
-      };
-      if (pending) {  // the other CTAs have read the last tile's sums
-        cluster_wait();
-        pending = false;
+    // ---- sums over the CTAs of the cluster, in rank order; h as bf16 pieces in every CTA
+    cluster_arrive();
+    cluster_wait();
+    const uint32_t hpa = smem_u32(hp);
+    for (int e = tid; e < tl.rows * C::RP / 2; e += kLoraThreads) {
+      const int m = (2 * e) / C::RP, r = 2 * e - m * C::RP;
+      float2 v = make_float2(0.f, 0.f);
+      for (uint32_t c = 0; c < csize; ++c) {
+        const float2 o = ld_cluster_f2(map_rank(hpa + 4 * (m * C::PITCH + r), c));
+        v.x = __fadd_rn(v.x, o.x);
+        v.y = __fadd_rn(v.y, o.y);
       }
-      if (NT == 1) {
-        put(red + warp * C::TM * C::RP);
-        __syncthreads();
-        for (int e = tid; e < C::TM * C::RP; e += kLoraThreads) {
-          float v = red[e];
-#pragma unroll
-          for (int w = 1; w < kLoraWarps; ++w) v = __fadd_rn(v, red[w * C::TM * C::RP + e]);
-          hp[e] = v;
-        }
-      } else {
-#pragma unroll
-        for (int half = kLoraWarps / 2; half >= 1; half >>= 1) {
-          if (warp >= half && warp < 2 * half) put(red + (warp - half) * C::TM * C::RP);
-          __syncthreads();
-          if (warp < half) {
-            const float* src = red + warp * C::TM * C::RP;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  acc[i][j][q] = __fadd_rn(acc[i][j][q],
-                                           src[(8 * j + 2 * t + (q & 1)) * C::RP + 16 * i + g + 8 * (q >> 1)]);
-          }
-          __syncthreads();
-        }
-        if (warp == 0) put(hp);
-      }
-      // ---- sums over the CTAs of the cluster, in rank order; h as bf16 pieces in every CTA
-      cluster_arrive();
-      cluster_wait();
-      const uint32_t hpa = smem_u32(hp), hfa = smem_u32(hf);
-      const int pairs = tl.rows * C::RP / 2;
-      const bool all = pairs <= 2 * kLoraThreads;  // few: every CTA sums all of them (one barrier less)
-      const int e0 = all ? 0 : static_cast<int>(pairs * crank / csize);
-      const int e1 = all ? pairs : static_cast<int>(pairs * (crank + 1) / csize);
-      for (int e = e0 + tid; e < e1; e += kLoraThreads) {
-        float2 v = make_float2(0.f, 0.f);
-        for (uint32_t c = 0; c < csize; ++c) {
-          const float2 o = ld_cluster_f2(map_rank(hpa + 8 * e, c));
-          v.x = __fadd_rn(v.x, o.x);
-          v.y = __fadd_rn(v.y, o.y);
-        }
-        const int m = (2 * e) / C::RP, r = 2 * e - m * C::RP;
-        // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
-        v.x = r < tl.rank ? __fmul_rn(v.x, tl.scale) : 0.f;
-        v.y = r + 1 < tl.rank ? __fmul_rn(v.y, tl.scale) : 0.f;
-        float r0, r1, q0, q1;
-        uint32_t w[3];
-        w[0] = piece(v.x, r0) | (piece(v.y, r1) << 16);
-        if (ns == 2) {
-          w[1] = bf16_rne_bits(r0) | (static_cast<uint32_t>(bf16_rne_bits(r1)) << 16);
-        } else {
-          w[1] = piece(r0, q0) | (piece(r1, q1) << 16);
-          w[2] = (__float_as_uint(q0) >> 16) | (__float_as_uint(q1) & 0xFFFF0000u);
-        }
-        for (int s = 0; s < ns; ++s) {
-          const uint32_t at = hfa + 2 * (s * HS + m * C::HPITCH + r);
-          if (all) reinterpret_cast<uint32_t*>(hf)[(s * HS + m * C::HPITCH + r) >> 1] = w[s];
-          else
-            for (uint32_t c = 0; c < csize; ++c) st_cluster_u32(map_rank(at, c), w[s]);
-        }
-      }
-      cluster_arrive();
-      pending = true;
-      if (all) {
-        __syncthreads();
-      } else {
-        cluster_wait();
-        pending = false;
-      }
+      // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
+      v.x = r < tl.rank ? __fmul_rn(v.x, tl.scale) : 0.f;
+      v.y = r + 1 < tl.rank ? __fmul_rn(v.y, tl.scale) : 0.f;
+      uint32_t w[3];
+      pieces(v, ns, w);
+      for (int s = 0; s < ns; ++s) reinterpret_cast<uint32_t*>(hf)[(s * HS + m * C::HPITCH + r) >> 1] = w[s];
     }
-    if (p.wait_y) pdl_wait();
-    // ---- second product: 64-column blocks
-    // items: 64-column blocks times groups of NTG token tiles (one pass over the accumulators each)
-    constexpr int NTG = NT > 4 ? 4 : NT;
-    const int rchunks = (tl.rank + 31) / 32;
-    const int items = nblk * ((tl.rows + 8 * NTG - 1) / (8 * NTG));
-    for (int it = gw; it < items; it += nw) {
-      const int nb = NT > NTG ? it % nblk : it, nt0 = NT > NTG ? (it / nblk) * NTG : 0;
-      float acc[4][NTG][4];
+    cluster_arrive();  // no CTA ends before the others have read its sums
+    pending = true;
+    __syncthreads();
+  }
+  if (p.wait_y) {
+    pdl_wait();
+    if (gw < nblk) yt.load(p, tok, tl.rows, gw * 64, lane, 0);
+  }
+  // ---- second product: 64-column blocks
+  const int rchunks = (tl.rank + 31) / 32;
+  for (int nb = gw; nb < nblk; nb += nw) {
+    float acc[4][1][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int j = 0; j < NTG; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[q][j][i] = -0.f;  // y + -0 is y, also for y = -0
-      for (int rc = 0; rc < rchunks; ++rc) {
-        if (NT != 1 || it != gw || rc != 0) load_b<VEC>(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
-        expand_step<NTG, AT>(acc, vb, hf, C::HPITCH, HS, ns, nt0, tl.rows, rc, lane);
-      }
-      store_rows<NTG>(p, tok, tl.rows, nb * 64, lane, acc, nt0);
+      for (int i = 0; i < 4; ++i) acc[q][0][i] = -0.f;  // y + -0 is y, also for y = -0
+    if (nb != gw) yt.load(p, tok, tl.rows, nb * 64, lane, 0);
+    for (int rc = 0; rc < rchunks; ++rc) {
+      if (nb != gw || rc != 0) load_b<VEC>(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
+      expand_step<1, AT>(acc, vb, hf, C::HPITCH, HS, ns, 0, tl.rows, rc, lane);
     }
-    if (!p.tiles) break;  // a cluster per row: this was its only tile
+    store_rows<1, Y32>(p, tok, tl.rows, nb * 64, lane, acc, yt, 0);
   }
   pdl_launch_dependents();
-  if (p.wait_y) pdl_wait();  // a cluster without a tile may not end before what it depends on
   if (pending) cluster_wait();
+}
+
+// ------------------------------------------------------------------ many rows: first product
+constexpr int kTile = 64;    // rows of a tile
+constexpr int kStages = 4;   // ring of 64-wide k chunks
+constexpr int kMaxSplit = 8; // shares of K
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+// 8 values (those below `valid`, the rest 0) of a row to a 16-byte place in shared memory
+template <bool VEC>
+__device__ __forceinline__ void stage8(uint32_t dst, const uint16_t* src, int valid, int w) {
+  if (VEC) {
+    cp_async16(dst, src, valid >= 8 ? 16 : 0);
+  } else if (w >= 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = valid - 2 * i;  // (a row of even length: its last pair is whole)
+      cp_async4(dst + 4 * i, n > 0 ? src + 2 * i : src, n > 0 ? 4 : 0);
+    }
+  } else {
+    const uint4 v = load8<false>(src, valid, 1);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  }
+}
+
+// CTA (tile, share of K): sums[share][position][rank], positions in the plan's order. Warp w takes 16 rows
+// and half the rank; operands by ldmatrix from rows of 128 bytes whose 16-byte chunks are XORed with the row.
+template <int MT, int AT, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int RP = 16 * MT, STAGE = (kTile + RP) * 128;
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_wait();
+  const int ti = blockIdx.x / p.ksplit, ks = blockIdx.x - ti * p.ksplit;
+  if (ti >= *p.n_tiles) return;
+  const int4 tile = p.tiles[ti];
+  if (tile.x < 0) return;
+  const LoraTile tl = lora_tile(p, tile.x, tile.z);
+  if (tl.rank == 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int chunks = (p.K + 63) / 64;
+  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * ks / p.ksplit);
+  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (ks + 1) / p.ksplit);
+  // this thread copies chunk tid % 8 of rows tid / 8 and + 32 of x and + 32 i of A
+  const int cc = tid & 7, cr = tid >> 3;
+  const uint16_t* xs[2];
+  int xok[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = cr + 32 * i;
+    xok[i] = m < tl.rows;
+    xs[i] = p.x + static_cast<int64_t>(xok[i] ? p.perm[tile.y + m] : 0) * p.ldx + 8 * cc;
+  }
+  const uint16_t* as = static_cast<const uint16_t*>(p.a) + (static_cast<int64_t>(tl.id) * p.R + cr) * p.K + 8 * cc;
+  const uint32_t base = smem_u32(smem);
+  auto issue = [&](int c) {
+    if (c < c1) {
+      const uint32_t st = base + (c - c0) % kStages * STAGE;
+      const int k = 64 * c, valid = p.K - k - 8 * cc;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int m = cr + 32 * i;
+        const bool in = xok[i] && valid > 0;
+        stage8<VEC>(st + m * 128 + ((cc ^ (m & 7)) << 4), in ? xs[i] + k : p.x, in ? valid : 0, p.wx);
+      }
+#pragma unroll
+      for (int i = 0; i < (RP + 31) / 32; ++i) {
+        const int r = cr + 32 * i;
+        const bool in = r < tl.rank && valid > 0;
+        if (RP % 32 == 0 || r < RP)
+          stage8<VEC>(st + (kTile + r) * 128 + ((cc ^ (r & 7)) << 4),
+                      in ? as + static_cast<int64_t>(32 * i) * p.K + k : static_cast<const uint16_t*>(p.a), in ? valid : 0, p.wa);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(c0 + i);
+  float acc[MT][4];  // 8-rank groups of this warp's half
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[i][q] = 0.f;
+  const int tg = 16 * (warp & 3), r0 = 8 * MT * (warp >> 2);
+  const int xr = tg + (lane & 15), xh = lane >> 4;             // x rows and k halves that this lane addresses
+  const int ar = (lane & 7) + ((lane >> 4) << 3), ah = (lane >> 3) & 1;  // A: two groups of 8 ranks, k halves
+  for (int c = c0; c < c1; ++c) {
+    cp_wait<kStages - 2>();
+    __syncthreads();
+    issue(c + kStages - 1);
+    const uint32_t st = base + (c - c0) % kStages * STAGE;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t x[4];
+      ldsm4(st + xr * 128 + (((2 * k + xh) ^ (xr & 7)) << 4), x);
+#pragma unroll
+      for (int i = 0; i < MT; i += 2) {
+        // (one group of 8 only: its lines are addressed twice)
+        const int r = r0 + 8 * i + (MT == 1 ? (lane & 7) : ar);
+        uint32_t w[4];
+        ldsm4(st + (kTile + r) * 128 + (((2 * k + ah) ^ (r & 7)) << 4), w);
+#pragma unroll
+        for (int h = 0; h < (MT == 1 ? 1 : 2); ++h) {
+          if (AT == AD_F16) {
+            uint32_t h0, l0, h1, l1;
+            split_f16(w[2 * h], h0, l0);
+            split_f16(w[2 * h + 1], h1, l1);
+            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], h0, h1);
+            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], l0, l1);
+          } else {
+            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], w[2 * h], w[2 * h + 1]);
+          }
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+  const int g = lane >> 2, t = lane & 3;
+  float* dst = p.sums + (static_cast<int64_t>(ks) * p.M + tile.y) * RP;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int m = tg + g + 8 * h;
+      if (m < tl.rows)
+        *reinterpret_cast<float2*>(dst + static_cast<int64_t>(m) * RP + r0 + 8 * i + 2 * t) =
+            make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+    }
+  pdl_launch_dependents();
+}
+
+// ------------------------------------------------------------------ many rows: second product
+// CTA (tile, share of N): the shares of K are summed in order, then warps take 64 columns x NT * 8 rows.
+template <int AT, bool VEC, bool Y32>
+__global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int NT = 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int tok[kTile];
+  uint16_t* hf = reinterpret_cast<uint16_t*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  pdl_wait();
+  const int ti = blockIdx.x / p.nsplit, np = blockIdx.x - ti * p.nsplit;
+  if (ti >= *p.n_tiles) return;
+  const int4 tile = p.tiles[ti];
+  if (tile.x < 0 && p.skip_plain) return;
+  const LoraTile tl = lora_tile(p, tile.x, tile.z);
+  const int ns = p.out_f32 ? 3 : 2;
+  const int rchunks = (tl.rank + 31) / 32;
+  const int hpitch = 32 * ((p.rp + 31) / 32) + 8, hs = kTile * hpitch;
+  if (tid < kTile) tok[tid] = tid < tl.rows ? p.perm[tile.y + tid] : 0;
+  for (int e = tid; e < tl.rows * rchunks * 16; e += kLoraThreads) {
+    const int m = e / (rchunks * 16), r = 2 * (e - m * rchunks * 16);
+    float2 v = make_float2(0.f, 0.f);
+    if (r < p.rp) {
+      const float* src = p.sums + static_cast<int64_t>(tile.y + m) * p.rp + r;
+#pragma unroll 4
+      for (int s = 0; s < p.ksplit; ++s) {
+        const float2 o = *reinterpret_cast<const float2*>(src + static_cast<int64_t>(s) * p.M * p.rp);
+        v.x = __fadd_rn(v.x, o.x);
+        v.y = __fadd_rn(v.y, o.y);
+      }
+    }
+    v.x = r < tl.rank ? __fmul_rn(v.x, tl.scale) : 0.f;
+    v.y = r + 1 < tl.rank ? __fmul_rn(v.y, tl.scale) : 0.f;
+    uint32_t w[3];
+    pieces(v, ns, w);
+    for (int s = 0; s < ns; ++s) reinterpret_cast<uint32_t*>(hf)[(s * hs + m * hpitch + r) >> 1] = w[s];
+  }
+  __syncthreads();
+  const int nblk = (p.N + 63) / 64;
+  const int nb0 = static_cast<int>(static_cast<int64_t>(nblk) * np / p.nsplit);
+  const int nb1 = static_cast<int>(static_cast<int64_t>(nblk) * (np + 1) / p.nsplit);
+  const int groups = (tl.rows + 8 * NT - 1) / (8 * NT);
+  for (int it = warp; it < (nb1 - nb0) * groups; it += kLoraWarps) {
+    const int nb = nb0 + it / groups, nt0 = (it % groups) * NT;
+    YTile<NT, Y32> yt;
+    yt.load(p, tok, tl.rows, nb * 64, lane, nt0);
+    float acc[4][NT][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[q][j][i] = -0.f;  // y + -0 is y, also for y = -0
+    for (int rc = 0; rc < rchunks; ++rc) {
+      uint4 vb[8];
+      load_b<VEC>(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
+      expand_step<NT, AT>(acc, vb, hf, hpitch, hs, ns, nt0, tl.rows, rc, lane);
+    }
+    store_rows<NT, Y32>(p, tok, tl.rows, nb * 64, lane, acc, yt, nt0);
+  }
+  pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ plan: rows ordered by adapter
 // Counting sort of the rows by id in one CTA: perm (rows of an adapter together), and tiles of at most
-// tm of them. The order inside an adapter follows the atomics; a row's result does not depend on its
-// place in a tile.
-__global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __restrict__ ids, int M, int L, int tm,
+// kTile of them. Rows of a warp that share an id take one atomic (the rows of a prompt all do). The order
+// inside an adapter follows the atomics; a row's result does not depend on its place in a tile.
+__global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __restrict__ ids, int M, int L,
                                                               int32_t* __restrict__ perm, int4* __restrict__ tiles,
                                                               int32_t* __restrict__ n_tiles, int* status) {
   extern __shared__ int cnt[];  // [L + 1]; L = rows without an adapter
   __shared__ int wsum[32], wtile[32];
+  constexpr int kHeld = 4;  // ids a thread keeps between the passes
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i <= L; i += 1024) cnt[i] = 0;
-  __syncthreads();
+  int held[kHeld];
   auto key = [&](int m) {
-    const int v = ids[m];
+    const int v = m < M ? ids[m] : -1;
     if (v >= L && status) atomicOr(status, ST_BAD_ARGS);
     return (v < 0 || v >= L) ? L : v;
   };
-  for (int m = tid; m < M; m += 1024) atomicAdd(&cnt[key(m)], 1);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = key(tid + 1024 * i);
+  for (int i = tid; i <= L; i += 1024) cnt[i] = 0;
+  __syncthreads();
+  // adds the rows of this warp's lanes to their counters: the lane's place in its counter
+  auto add = [&](int k, bool in) {
+    const uint32_t same = __match_any_sync(0xffffffffu, in ? k : -1);
+    const int first = __ffs(same) - 1;
+    int at = 0;
+    if (in && lane == first) at = atomicAdd(&cnt[k], __popc(same));
+    return __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1));
+  };
+  const int steps = (M + 1023) / 1024;
+  for (int i = 0; i < steps; ++i) {
+    const int m = tid + 1024 * i;
+    int k = 0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (j == i) k = held[j];
+    if (i >= kHeld) k = key(m);
+    add(k, m < M);
+  }
   __syncthreads();
   // exclusive sums over the keys of rows and of tiles; every thread takes a run of keys
   const int per = (L + 1 + 1023) / 1024;
@@ -520,7 +710,7 @@ __global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __r
   int rows = 0, tl = 0;
   for (int k = k0; k < k1; ++k) {
     rows += cnt[k];
-    tl += (cnt[k] + tm - 1) / tm;
+    tl += (cnt[k] + kTile - 1) / kTile;
   }
   int ir = rows, it = tl;
 #pragma unroll
@@ -555,57 +745,118 @@ __global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __r
   for (int k = k0; k < k1; ++k) {
     const int n = cnt[k];
     cnt[k] = r0;
-    for (int i = 0; i < n; i += tm) tiles[t0++] = make_int4(k == L ? -1 : k, r0 + i, min(tm, n - i), 0);
+    for (int i = 0; i < n; i += kTile) tiles[t0++] = make_int4(k == L ? -1 : k, r0 + i, min(kTile, n - i), 0);
     r0 += n;
   }
   __syncthreads();
-  for (int m = tid; m < M; m += 1024) {
-    const int v = ids[m];
-    perm[atomicAdd(&cnt[(v < 0 || v >= L) ? L : v], 1)] = m;
+  for (int i = 0; i < steps; ++i) {
+    const int m = tid + 1024 * i;
+    int k = 0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (j == i) k = held[j];
+    if (i >= kHeld && m < M) {
+      const int v = ids[m];
+      k = (v < 0 || v >= L) ? L : v;
+    }
+    const int at = add(k, m < M);
+    if (m < M) perm[at] = m;
   }
   pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ host
 static size_t al256l(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
-// tiles of 8 rows at least: never more than this
-static int64_t plan_max_tiles(int64_t M, int64_t L, int tm) { return M / tm + std::min<int64_t>(L + 1, M); }
-
-size_t lora_plan_bytes(int64_t M, int64_t L) {
-  if (M <= kDirectRows) return 0;
-  return 256 + al256l(4 * M) + al256l(16 * plan_max_tiles(M, L, 8));
+static int64_t max_tiles(int64_t M, int64_t L) { return M / kTile + std::min<int64_t>(L + 1, M); }
+static int padded_rank(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+// shares of K: about two CTAs an SM over the tiles that M rows and L adapters make (148 SMs)
+static int k_split(int64_t M, int64_t L) {
+  const int64_t tiles = std::max<int64_t>(1, M / kTile + std::min<int64_t>(L, M) / 2);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 296 / tiles)));
 }
 
-template <int MT, int NT, int AT, bool VEC>
-static int lora_launch_one(const LoraParams& p, int clusters, int csize, cudaStream_t s, bool pdl) {
-  using C = LoraCfg<MT, NT>;
-  auto kern = aipu_lora_kernel<MT, NT, AT, VEC>;
-  static bool attr[64] = {false};
-  const int rc = set_smem_attr_once(reinterpret_cast<const void*>(kern), C::TOTAL, attr, "cudaFuncSetAttribute(lora)");
-  if (rc) return rc;
+size_t lora_plan_bytes(int64_t M, int64_t L, int64_t R) {
+  if (M <= kDirectRows) return 0;
+  return 256 + al256l(4 * M) + al256l(16 * max_tiles(M, L)) +
+         al256l(static_cast<size_t>(4) * M * padded_rank(R) * k_split(M, L));
+}
+
+static int launch(const void* kern, int grid, int block, size_t smem, int cluster, cudaStream_t s, bool pdl, void** args,
+                  const char* what) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * csize);
-  cfg.blockDim = dim3(kLoraThreads);
-  cfg.dynamicSmemBytes = C::TOTAL;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = pdl ? 2 : 1;
-  return set_cuda_error(cudaLaunchKernelEx(&cfg, kern, p), "aipu_lora_kernel");
+  cfg.numAttrs = n;
+  return set_cuda_error(cudaLaunchKernelExC(&cfg, kern, args), what);
 }
 
-template <int MT, int NT>
-static int lora_launch_t(const LoraParams& p, bool vec, int clusters, int csize, cudaStream_t s, bool pdl) {
-  if (p.adtype == AD_F16)
-    return vec ? lora_launch_one<MT, NT, AD_F16, true>(p, clusters, csize, s, pdl)
-               : lora_launch_one<MT, NT, AD_F16, false>(p, clusters, csize, s, pdl);
-  return vec ? lora_launch_one<MT, NT, AD_BF16, true>(p, clusters, csize, s, pdl)
-             : lora_launch_one<MT, NT, AD_BF16, false>(p, clusters, csize, s, pdl);
+template <int MT, int AT, bool VEC, bool Y32>
+static int direct_launch(LoraParams& p, cudaStream_t s, bool pdl) {
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_kernel<MT, AT, VEC, Y32>);
+  static bool attr[64] = {false};
+  const int rc = set_smem_attr_once(kern, LoraCfg<MT>::TOTAL, attr, "cudaFuncSetAttribute(lora)");
+  if (rc) return rc;
+  void* args[1] = {&p};
+  // a cluster for every row that may lead a tile
+  return launch(kern, p.M * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, kDirectCtas, s, pdl, args, "aipu_lora_kernel");
+}
+template <int MT>
+static int direct_launch_t(LoraParams& p, bool vec, cudaStream_t s, bool pdl) {
+  if (p.adtype == AD_F16) {
+    if (vec) return p.y_f32 ? direct_launch<MT, AD_F16, true, true>(p, s, pdl) : direct_launch<MT, AD_F16, true, false>(p, s, pdl);
+    return p.y_f32 ? direct_launch<MT, AD_F16, false, true>(p, s, pdl) : direct_launch<MT, AD_F16, false, false>(p, s, pdl);
+  }
+  if (vec) return p.y_f32 ? direct_launch<MT, AD_BF16, true, true>(p, s, pdl) : direct_launch<MT, AD_BF16, true, false>(p, s, pdl);
+  return p.y_f32 ? direct_launch<MT, AD_BF16, false, true>(p, s, pdl) : direct_launch<MT, AD_BF16, false, false>(p, s, pdl);
+}
+
+template <int MT, int AT, bool VEC>
+static int shrink_launch(LoraParams& p, cudaStream_t s) {
+  constexpr int smem = kStages * (kTile + 16 * MT) * 128;
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_shrink_kernel<MT, AT, VEC>);
+  static bool attr[64] = {false};
+  const int rc = set_smem_attr_once(kern, smem, attr, "cudaFuncSetAttribute(lora shrink)");
+  if (rc) return rc;
+  void* args[1] = {&p};
+  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.ksplit, kLoraThreads, smem, 1, s, true, args,
+                "aipu_lora_shrink_kernel");
+}
+template <int MT>
+static int shrink_launch_t(LoraParams& p, bool vec, cudaStream_t s) {
+  if (p.adtype == AD_F16) return vec ? shrink_launch<MT, AD_F16, true>(p, s) : shrink_launch<MT, AD_F16, false>(p, s);
+  return vec ? shrink_launch<MT, AD_BF16, true>(p, s) : shrink_launch<MT, AD_BF16, false>(p, s);
+}
+
+template <int AT, bool VEC, bool Y32>
+static int expand_launch(LoraParams& p, cudaStream_t s, bool pdl) {
+  const int smem = 3 * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, VEC, Y32>);
+  static bool attr[64] = {false};
+  const int rc = set_smem_attr_once(kern, 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
+  if (rc) return rc;
+  void* args[1] = {&p};
+  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, 1, s, pdl, args,
+                "aipu_lora_expand_kernel");
+}
+template <int AT, bool VEC>
+static int expand_launch_t(LoraParams& p, cudaStream_t s, bool pdl) {
+  return p.y_f32 ? expand_launch<AT, VEC, true>(p, s, pdl) : expand_launch<AT, VEC, false>(p, s, pdl);
 }
 
 // widest load (elements of 16 bits) of rows `ld` elements apart from `ptr`
@@ -614,79 +865,58 @@ static int load_width(const void* ptr, int64_t ld) {
   return (a % 16 == 0 && ld % 8 == 0) ? 8 : (a % 4 == 0 && ld % 2 == 0) ? 2 : 1;
 }
 
-// Shape of the row tiles. Tiles of 8 rows where the rows of an adapter are few on average, else of 64
-// (32 for ranks above 64, whose sums take twice the registers).
-struct LoraShape {
-  int mt, tm;
-  bool wide;
-};
-static LoraShape lora_shape(const LoraParams& p) {
-  LoraShape sh;
-  sh.mt = p.R <= 16 ? 1 : p.R <= 32 ? 2 : p.R <= 64 ? 4 : 8;
-  sh.wide = p.M > kDirectRows && p.M / std::min(p.L, p.M) > 8;
-  sh.tm = !sh.wide ? 8 : sh.mt == 8 ? 32 : 64;
-  return sh;
-}
-
-int lora_plan_launch(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
+int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
+  if (p.L > kMaxAdapters || p.R > 128) return set_error(EINVAL_, "lora: at most 32768 adapters of rank 128");
+  p.skip_plain = (p.out == p.y && p.out_f32 == p.y_f32) ? 1 : 0;
+  p.rp = padded_rank(p.R);
+  // (an even row length is what the pairwise copies of the first product need of A and x)
+  p.wa = load_width(p.a, p.K);
+  p.wx = p.K % 2 ? 1 : load_width(p.x, p.ldx);
+  p.wb = load_width(p.b, p.R);
+  auto rows16 = [](const void* q, int64_t ld, int esz) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * esz % 16 == 0;
+  };
+  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2) && rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
   p.tiles = nullptr;
   if (p.M <= kDirectRows) return OK;
   uint8_t* b = static_cast<uint8_t*>(plan);
   p.n_tiles = reinterpret_cast<int32_t*>(b);
   p.perm = reinterpret_cast<int32_t*>(b + 256);
-  p.tiles = reinterpret_cast<int4*>(b + 256 + al256l(4 * static_cast<size_t>(p.M)));
+  b += 256 + al256l(4 * static_cast<size_t>(p.M));
+  p.tiles = reinterpret_cast<int4*>(b);
+  p.sums = reinterpret_cast<float*>(b + al256l(16 * max_tiles(p.M, p.L)));
+  p.ksplit = k_split(p.M, p.L);
+  // shares of N: about three CTAs an SM, of eight 64-column blocks at least
+  const int64_t likely = std::max<int64_t>(1, p.M / kTile + std::min(p.L, p.M) / 2);
+  p.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((p.N + 255) / 256, 444 / likely)));
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_plan_kernel);
   static bool attr[64] = {false};
-  const int rc = set_smem_attr_once(reinterpret_cast<const void*>(aipu_lora_plan_kernel), (kMaxAdapters + 1) * 4, attr,
-                                    "cudaFuncSetAttribute(lora plan)");
+  int rc = set_smem_attr_once(kern, (kMaxAdapters + 1) * 4, attr, "cudaFuncSetAttribute(lora plan)");
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(1);
-  cfg.blockDim = dim3(1024);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.L + 1) * 4;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return set_cuda_error(cudaLaunchKernelEx(&cfg, aipu_lora_plan_kernel, p.ids, p.M, p.L, lora_shape(p).tm, p.perm, p.tiles,
-                                           p.n_tiles, p.status),
-                        "aipu_lora_plan_kernel");
+  void* args[7] = {&p.ids, &p.M, &p.L, &p.perm, &p.tiles, &p.n_tiles, &p.status};
+  if ((rc = launch(kern, 1, 1024, static_cast<size_t>(p.L + 1) * 4, 1, s, pdl, args, "aipu_lora_plan_kernel"))) return rc;
+  const bool vec = p.wa == 8 && p.wx == 8;
+  switch (p.rp) {
+    case 16: return shrink_launch_t<1>(p, vec, s);
+    case 32: return shrink_launch_t<2>(p, vec, s);
+    case 64: return shrink_launch_t<4>(p, vec, s);
+    default: return shrink_launch_t<8>(p, vec, s);
+  }
 }
 
-int lora_launch(LoraParams p, int num_sms, cudaStream_t s, bool pdl) {
-  if (p.M <= 0 || p.N <= 0) return OK;
-  if (p.L > kMaxAdapters || p.R > 128) return set_error(EINVAL_, "lora: at most 32768 adapters of rank 128");
-  p.skip_plain = (p.out == p.y && p.out_f32 == p.y_f32) ? 1 : 0;
-  p.wa = load_width(p.a, p.K);
-  p.wx = load_width(p.x, p.ldx);
-  p.wb = load_width(p.b, p.R);
-  const bool vec = p.wa == 8 && p.wx == 8 && p.wb == 8;
-  auto rows16 = [](const void* q, int64_t ld, int esz) {
-    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * esz % 16 == 0;
-  };
-  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2) && rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
-  const LoraShape sh = lora_shape(p);
-  int clusters = p.M, csize = 8;
-  if (p.tiles) {
-    const int64_t tiles = plan_max_tiles(p.M, p.L, sh.tm);
-    csize = tiles >= 2 * num_sms ? 2 : tiles >= num_sms / 2 ? 4 : 8;
-    clusters = static_cast<int>(std::min<int64_t>(tiles, 4 * num_sms / csize));
-  }
-  if (sh.wide) {
-    switch (sh.mt) {
-      case 1: return lora_launch_t<1, 8>(p, vec, clusters, csize, s, pdl);
-      case 2: return lora_launch_t<2, 8>(p, vec, clusters, csize, s, pdl);
-      case 4: return lora_launch_t<4, 8>(p, vec, clusters, csize, s, pdl);
-      default: return lora_launch_t<8, 4>(p, vec, clusters, csize, s, pdl);
+int lora_finish(LoraParams& p, cudaStream_t s, bool pdl) {
+  if (!p.tiles) {
+    const bool vec = p.wa == 8 && p.wx == 8 && p.wb == 8;
+    switch (p.rp) {
+      case 16: return direct_launch_t<1>(p, vec, s, pdl);
+      case 32: return direct_launch_t<2>(p, vec, s, pdl);
+      case 64: return direct_launch_t<4>(p, vec, s, pdl);
+      default: return direct_launch_t<8>(p, vec, s, pdl);
     }
   }
-  switch (sh.mt) {
-    case 1: return lora_launch_t<1, 1>(p, vec, clusters, csize, s, pdl);
-    case 2: return lora_launch_t<2, 1>(p, vec, clusters, csize, s, pdl);
-    case 4: return lora_launch_t<4, 1>(p, vec, clusters, csize, s, pdl);
-    default: return lora_launch_t<8, 1>(p, vec, clusters, csize, s, pdl);
-  }
+  const bool vec = p.wb == 8;
+  if (p.adtype == AD_F16) return vec ? expand_launch_t<AD_F16, true>(p, s, pdl) : expand_launch_t<AD_F16, false>(p, s, pdl);
+  return vec ? expand_launch_t<AD_BF16, true>(p, s, pdl) : expand_launch_t<AD_BF16, false>(p, s, pdl);
 }
 
 }  // namespace aipu

@@ -23,20 +23,23 @@ struct LoraParams {
   int64_t ldo;
   int y_f32, out_f32;
   int* status;           // device status word (nullable)
-  // set by the launch
-  int32_t* perm;         // rows ordered by adapter
+  int wait_y;            // 1: y comes from the kernel launched just before lora_finish's (programmatic launch)
+  // set by lora_begin
+  int32_t* perm;         // rows ordered by adapter (more rows than one launch takes: tiles is set)
   int4* tiles;           // {adapter or -1, first position in perm, rows, 0}
   int32_t* n_tiles;
+  float* sums;           // [ksplit][M][rp] shares of h by position
+  int ksplit, nsplit;    // shares of K and of N
+  int rp;                // padded rank: 16, 32, 64 or 128
   int skip_plain;        // 1: in-place, rows without an adapter are not touched
   int wa, wx, wb;        // widest aligned load of A rows, x rows, B rows (elements: 8, 2 or 1)
   int vy;                // 1: 16-byte loads and stores of y and out
-  int wait_y;            // 1: y comes from the kernel launched just before (programmatic dependent launch)
 };
 
-// bytes of the row plan (0 when M rows need none)
-size_t lora_plan_bytes(int64_t M, int64_t L);
-// the plan of p.ids in `plan` (sets p's pointers to it; nothing to do for few rows)
-int lora_plan_launch(LoraParams& p, void* plan, cudaStream_t s, bool pdl);
-int lora_launch(LoraParams p, int num_sms, cudaStream_t s, bool pdl);
+// bytes of the scratch of M rows (0 when the one launch takes them)
+size_t lora_plan_bytes(int64_t M, int64_t L, int64_t R);
+// what does not need y: the row plan and the first product of many rows. Then the rest.
+int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl);
+int lora_finish(LoraParams& p, cudaStream_t s, bool pdl);
 
 }  // namespace aipu

@@ -426,7 +426,7 @@ def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tens
     if ydt not in _DTYPE or odt not in (torch.bfloat16, ydt):
         raise ValueError("y must be bf16 or fp32, out bf16 or y's type")
     ctx, index = _on(ctx, x, ids, y, out, ad.a, ad.b, ad.scale, ad.ranks)
-    n = lib().aipu_lora_workspace(M, cs.n_adapters)
+    n = lib().aipu_lora_workspace(M, cs.n_adapters, cs.rank)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     check(lib().aipu_lora_add(ctx.handle, cs, ids.data_ptr(), x.data_ptr(), ldx, M, y.data_ptr(), _DTYPE[ydt], ldy,
                               out.data_ptr(), _DTYPE[odt], ldo, ws.data_ptr() if n else None, n, _raw_stream(index)))
@@ -450,7 +450,7 @@ def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: 
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
         raise ValueError("out must be bf16 [M, N]")
     ctx, index = _on(ctx, x, w, ids, out, ad.a, ad.b, ad.scale, ad.ranks)
-    n = lib().aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters)
+    n = lib().aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters, cs.rank)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     check(lib().aipu_q4k_gemm_lora(ctx.handle, wtype, w.data_ptr(), N, K, x.data_ptr(), M, cs, ids.data_ptr(),
                                    out.data_ptr(), ws.data_ptr() if n else None, n, _raw_stream(index)))

@@ -277,10 +277,10 @@ typedef struct aipu_lora {
  * fp32, or fp32 and bf16; out may be y (same type and stride: rows without an adapter are then not
  * touched), otherwise they must not overlap. ldx, ldy, ldo: elements between rows (>= K, N, N), so
  * columns of a wider tensor can be passed.
- * ws: device scratch of aipu_lora_workspace(M, n_adapters) bytes (NULL when that is 0), in use until
+ * ws: device scratch of aipu_lora_workspace(M, n_adapters, rank) bytes (NULL when that is 0), in use until
  * the call's work on `stream` is done. Nothing else is shared, so calls with their own ws may run at the
  * same time. Equal calls give equal bits. No counterpart in the reference. */
-int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters);
+int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
                   const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,
                   int64_t ws_bytes, void* stream);
@@ -291,7 +291,7 @@ int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const 
  * the tcgen05 GEMM for many rows of Q4_K / Q6_K) are not rounded before the adapter term is added.
  * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Uses the context's
  * stream-K workspace (one context per concurrently used stream). No counterpart in the reference. */
-int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters);
+int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,
                        const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes, void* stream);
 

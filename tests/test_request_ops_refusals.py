@@ -130,11 +130,13 @@ def test_c_entry_refuses_a_projection(kw, text):
 
 def test_workspace_sizes():
     L = _lib.lib()
-    assert L.aipu_lora_workspace(64, 8) == 0 and L.aipu_lora_workspace(-1, 8) == 0 and L.aipu_lora_workspace(65, 0) == 0
-    # one int per row and room for tiles of 8 rows of every adapter
-    assert L.aipu_lora_workspace(65, 8) >= 4 * 65 + 16 * (8 + 9)
-    assert L.aipu_q4k_gemm_lora_workspace(0, 32, 256, 3, 2) >= 4 * 3 * 32
-    assert L.aipu_q4k_gemm_lora_workspace(0, 32, 100, 3, 2) == 0
+    assert L.aipu_lora_workspace(64, 8, 16) == 0
+    for bad in ((-1, 8, 16), (65, 0, 16), (65, 32769, 16), (65, 8, 0), (65, 8, 129)):
+        assert L.aipu_lora_workspace(*bad) == 0
+    # an int per row, tiles of every adapter, and the fp32 sums of 16 ranks at least
+    assert L.aipu_lora_workspace(65, 8, 3) >= 4 * 65 + 16 * 9 + 4 * 65 * 16
+    assert L.aipu_q4k_gemm_lora_workspace(0, 32, 256, 3, 2, 8) >= 4 * 3 * 32
+    assert L.aipu_q4k_gemm_lora_workspace(0, 32, 100, 3, 2, 8) == 0
 
 
 def _process(**kw):
