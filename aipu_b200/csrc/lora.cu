@@ -169,6 +169,11 @@ __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, cons
 }
 
 // ------------------------------------------------------------------ second product and the result rows
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // rounded to the nearest, ties to even
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // acc[q][j]: MMA q's rows g and g + 8 are columns n0 + 8 g + 2 q and + 2 q + 1 of y, its columns 2 t and
 // 2 t + 1 the rows 8 (nt0 + j) + 2 t (+ 1) of the tile. Rows of y, 8 columns a lane, loaded ahead:
 template <int NT, bool Y32>
@@ -227,7 +232,7 @@ __device__ __forceinline__ void store_rows(const LoraParams& p, const int* tok, 
           uint32_t o[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            o[i] = bf16_rne_bits(d[2 * i]) | (static_cast<uint32_t>(bf16_rne_bits(d[2 * i + 1])) << 16);
+            o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
           *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + n) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       } else {
@@ -249,7 +254,7 @@ __device__ __forceinline__ void pieces(float2 v, int ns, uint32_t (&w)[3]) {
   float r0, r1, q0, q1;
   w[0] = piece(v.x, r0) | (piece(v.y, r1) << 16);
   if (ns == 2) {
-    w[1] = bf16_rne_bits(r0) | (static_cast<uint32_t>(bf16_rne_bits(r1)) << 16);
+    w[1] = pack_bf16(r0, r1);
   } else {
     w[1] = piece(r0, q0) | (piece(r1, q1) << 16);
     w[2] = (__float_as_uint(q0) >> 16) | (__float_as_uint(q1) & 0xFFFF0000u);
@@ -287,24 +292,29 @@ template <int NTG, int AT>
 __device__ __forceinline__ void expand_step(float (&acc)[4][NTG][4], const uint4 (&vb)[8], const uint16_t* hf, int hpitch,
                                             int hsplit, int ns, int nt0, int rows, int rc, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  uint4 bh[8], bl[8];
+  // (fp16 adapters: a pair of B rows at a time is split into its two pieces, and h read again for it)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (AT == AD_F16) split4_f16(vb[i], bh[i], bl[i]);
-    else bh[i] = vb[i];
-  }
+  for (int q0 = 0; q0 < 4; q0 += AT == AD_F16 ? 1 : 4) {
+    uint4 h0, l0, h1, l1;
+    if (AT == AD_F16) {
+      split4_f16(vb[2 * q0], h0, l0);
+      split4_f16(vb[2 * q0 + 1], h1, l1);
+    }
 #pragma unroll
-  for (int j = 0; j < NTG; ++j) {
-    if (8 * (nt0 + j) >= rows) continue;  // warp-uniform
-    const uint16_t* hrow = hf + (8 * (nt0 + j) + g) * hpitch + 32 * rc + 8 * t;
+    for (int j = 0; j < NTG; ++j) {
+      if (8 * (nt0 + j) >= rows) continue;  // warp-uniform
+      const uint16_t* hrow = hf + (8 * (nt0 + j) + g) * hpitch + 32 * rc + 8 * t;
 #pragma unroll
-    for (int s = 0; s < 3; ++s) {
-      if (s >= ns) break;  // uniform
-      const uint4 h = *reinterpret_cast<const uint4*>(hrow + s * hsplit);
+      for (int s = 0; s < 3; ++s) {
+        if (s >= ns) break;  // uniform
+        const uint4 h = *reinterpret_cast<const uint4*>(hrow + s * hsplit);
+        if (AT == AD_F16) {
+          mma_pair(acc[q0][j], h0, h1, h);
+          mma_pair(acc[q0][j], l0, l1, h);
+        } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mma_pair(acc[q][j], bh[2 * q], bh[2 * q + 1], h);
-        if (AT == AD_F16) mma_pair(acc[q][j], bl[2 * q], bl[2 * q + 1], h);
+          for (int q = 0; q < 4; ++q) mma_pair(acc[q][j], vb[2 * q], vb[2 * q + 1], h);
+        }
       }
     }
   }
@@ -331,33 +341,44 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t crank = cluster_rank(), csize = cluster_size();
-  const int lead = blockIdx.x / csize;  // the row that this cluster's tile would begin with
   const int ns = p.out_f32 ? 3 : 2;
   constexpr int HS = C::TM * C::HPITCH;  // elements of one piece
   // x (and the ids) may come from the kernel before the one that writes y, so they wait too unless the
   // launch says that only y does
   if (!p.wait_y) pdl_wait();
 
-  // row `lead` leads a tile if the number of earlier rows with its id is a multiple of the tile's rows; the
-  // tile is that row and the following ones of the id
-  const int n0 = lane < p.M ? p.ids[lane] : -2, n1 = lane + 32 < p.M ? p.ids[lane + 32] : -2;
-  int id = p.ids[lead];
-  if (id < 0 || id >= p.L) {
-    if (id >= p.L && crank == 0 && tid == 0 && p.status) atomicOr(p.status, ST_BAD_ARGS);
-    id = -1;
+  // a row leads a tile if the number of earlier rows with its id is a multiple of a tile's rows; the tile is
+  // that row and the following ones of the id, and this cluster's is the one of the cluster's number
+  __shared__ int key[kDirectRows];
+  for (int i = tid; i < p.M; i += kLoraThreads) {
+    const int v = p.ids[i];
+    if (v >= p.L && blockIdx.x == 0 && p.status) atomicOr(p.status, ST_BAD_ARGS);
+    key[i] = (v < 0 || v >= p.L) ? -1 : v;
   }
-  const LoraTile own = lora_tile(p, id, 0);
-  auto same = [&](int v, int row) { return row < p.M && (id < 0 ? (v < 0 || v >= p.L) : v == id); };
-  const uint32_t b0 = __ballot_sync(0xffffffffu, same(n0, lane));
-  const uint32_t b1 = __ballot_sync(0xffffffffu, same(n1, lane + 32));
-  const uint64_t all = static_cast<uint64_t>(b1) << 32 | b0;
-  const uint64_t below = (1ull << lead) - 1;
-  // (the same for every thread of the cluster)
-  if (__popcll(all & below) % C::TM != 0 || (id < 0 && p.skip_plain)) {
+  __syncthreads();
+  const int k0 = lane < p.M ? key[lane] : -2, k1 = lane + 32 < p.M ? key[lane + 32] : -2;
+  // earlier rows with the ids of rows `lane` and `lane + 32`
+  const uint32_t lower = (1u << lane) - 1;
+  const int same0 = __popc(__match_any_sync(0xffffffffu, k0) & lower);
+  int same1 = __popc(__match_any_sync(0xffffffffu, k1) & lower);
+  if (p.M > 32)
+    for (int i = 0; i < 32; ++i) same1 += __shfl_sync(0xffffffffu, k0, i) == k1;
+  const bool any0 = k0 >= 0 || (k0 == -1 && !p.skip_plain), any1 = k1 >= 0 || (k1 == -1 && !p.skip_plain);
+  const uint32_t l0 = __ballot_sync(0xffffffffu, any0 && same0 % C::TM == 0);
+  const uint32_t l1 = __ballot_sync(0xffffffffu, any1 && same1 % C::TM == 0);
+  uint64_t leaders = static_cast<uint64_t>(l1) << 32 | l0;
+  for (int i = blockIdx.x / csize; i > 0 && leaders; --i) leaders &= leaders - 1;
+  if (!leaders) {  // (the same for every thread of the cluster)
     pdl_launch_dependents();
     if (p.wait_y) pdl_wait();  // a cluster without a tile may not end before what it depends on
     return;
   }
+  const int lead = __ffsll(static_cast<long long>(leaders)) - 1;
+  const int id = key[lead];
+  const LoraTile own = lora_tile(p, id, 0);
+  const uint32_t b0 = __ballot_sync(0xffffffffu, k0 == id), b1 = __ballot_sync(0xffffffffu, k1 == id);
+  const uint64_t all = static_cast<uint64_t>(b1) << 32 | b0;
+  const uint64_t below = (1ull << lead) - 1;
   const uint64_t rest = all & ~below;
   LoraTile tl = own;
   tl.rows = min(C::TM, __popcll(rest));
@@ -457,7 +478,9 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_co
 
 // ------------------------------------------------------------------ many rows: first product
 constexpr int kTile = 64;    // rows of a tile
-constexpr int kStages = 4;   // ring of 64-wide k chunks
+// ring of 64-wide k chunks: two CTAs' rings fill an SM's shared memory (80 KB on their way an SM where rank <= 32)
+template <int MT>
+constexpr int kStages = MT == 1 ? 8 : MT == 2 ? 7 : MT == 4 ? 6 : 4;
 constexpr int kMaxSplit = 8; // shares of K
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -494,19 +517,19 @@ __device__ __forceinline__ void stage8(uint32_t dst, const uint16_t* src, int va
   }
 }
 
-// CTA (tile, share of K): sums[share][position][rank], positions in the plan's order. Warp w takes 16 rows
+// CTA (tile, share of K): scaled sums[share][position][rank], positions in the plan's order. Warp w takes 16 rows
 // and half the rank; operands by ldmatrix from rows of 128 bytes whose 16-byte chunks are XORed with the row.
 template <int MT, int AT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int RP = 16 * MT, STAGE = (kTile + RP) * 128;
+  constexpr int RP = 16 * MT, STAGE = (kTile + RP) * 128, S = kStages<MT>;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait();
+  pdl_launch_dependents();  // (the second product reads the plan, which is complete, before it waits for this)
   const int ti = blockIdx.x / p.ksplit, ks = blockIdx.x - ti * p.ksplit;
-  if (ti >= *p.n_tiles) return;
-  const int4 tile = p.tiles[ti];
-  if (tile.x < 0) return;
-  const LoraTile tl = lora_tile(p, tile.x, tile.z);
-  if (tl.rank == 0) return;
+  const int4 tile = p.tiles[ti];  // (only tiles below n_tiles are written, but there is room for every ti)
+  if (ti >= *p.n_tiles || tile.x < 0) return;
+  const LoraTile tl = {tile.x, tile.z, tile.w, 1.f};
+  const float scale = p.scale ? p.scale[tile.x] : 1.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int chunks = (p.K + 63) / 64;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * ks / p.ksplit);
@@ -522,53 +545,73 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
     xs[i] = p.x + static_cast<int64_t>(xok[i] ? p.perm[tile.y + m] : 0) * p.ldx + 8 * cc;
   }
   const uint16_t* as = static_cast<const uint16_t*>(p.a) + (static_cast<int64_t>(tl.id) * p.R + cr) * p.K + 8 * cc;
-  const uint32_t base = smem_u32(smem);
+  constexpr int AI = (RP + 31) / 32;
+  const bool arow = RP % 32 == 0 || cr < RP;
+  const uint32_t base = smem_u32(smem), at = cr * 128 + ((cc ^ (cr & 7)) << 4);  // (32 rows on: the same chunk)
+  int slot = 0;
   auto issue = [&](int c) {
     if (c < c1) {
-      const uint32_t st = base + (c - c0) % kStages * STAGE;
-      const int k = 64 * c, valid = p.K - k - 8 * cc;
+      const uint32_t st = base + slot * STAGE + at;
+      const int k = 64 * c;
+      if (VEC && k + 64 <= p.K) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int m = cr + 32 * i;
-        const bool in = xok[i] && valid > 0;
-        stage8<VEC>(st + m * 128 + ((cc ^ (m & 7)) << 4), in ? xs[i] + k : p.x, in ? valid : 0, p.wx);
-      }
+        for (int i = 0; i < 2; ++i) cp_async16(st + 4096 * i, xs[i] + k, xok[i] ? 16 : 0);
 #pragma unroll
-      for (int i = 0; i < (RP + 31) / 32; ++i) {
-        const int r = cr + 32 * i;
-        const bool in = r < tl.rank && valid > 0;
-        if (RP % 32 == 0 || r < RP)
-          stage8<VEC>(st + (kTile + r) * 128 + ((cc ^ (r & 7)) << 4),
-                      in ? as + static_cast<int64_t>(32 * i) * p.K + k : static_cast<const uint16_t*>(p.a), in ? valid : 0, p.wa);
+        for (int i = 0; i < AI; ++i) {
+          const bool in = cr + 32 * i < tl.rank;
+          if (arow) cp_async16(st + kTile * 128 + 4096 * i, in ? as + static_cast<int64_t>(32 * i) * p.K + k : as, in ? 16 : 0);
+        }
+      } else {
+        const int valid = p.K - k - 8 * cc;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool in = xok[i] && valid > 0;
+          stage8<VEC>(st + 4096 * i, in ? xs[i] + k : p.x, in ? valid : 0, p.wx);
+        }
+#pragma unroll
+        for (int i = 0; i < AI; ++i) {
+          const bool in = cr + 32 * i < tl.rank && valid > 0;
+          if (arow)
+            stage8<VEC>(st + kTile * 128 + 4096 * i,
+                        in ? as + static_cast<int64_t>(32 * i) * p.K + k : static_cast<const uint16_t*>(p.a), in ? valid : 0, p.wa);
+        }
       }
     }
+    if (++slot == S) slot = 0;
     cp_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(c0 + i);
+  for (int i = 0; i < S - 1; ++i) issue(c0 + i);
   float acc[MT][4];  // 8-rank groups of this warp's half
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int q = 0; q < 4; ++q) acc[i][q] = 0.f;
   const int tg = 16 * (warp & 3), r0 = 8 * MT * (warp >> 2);
-  const int xr = tg + (lane & 15), xh = lane >> 4;             // x rows and k halves that this lane addresses
-  const int ar = (lane & 7) + ((lane >> 4) << 3), ah = (lane >> 3) & 1;  // A: two groups of 8 ranks, k halves
+  const int xr = tg + (lane & 15), xh = lane >> 4;  // x row and k half that this lane addresses
+  // A: two groups of 8 ranks and their k halves (one group only: its lines are addressed twice)
+  const int ar = r0 + (MT == 1 ? (lane & 7) : (lane & 7) + ((lane >> 4) << 3)), ah = (lane >> 3) & 1;
+  uint32_t xo[4], ao[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    xo[k] = base + xr * 128 + (((2 * k + xh) ^ (xr & 7)) << 4);
+    ao[k] = base + (kTile + ar) * 128 + (((2 * k + ah) ^ (ar & 7)) << 4);
+  }
+  int use = 0;
   for (int c = c0; c < c1; ++c) {
-    cp_wait<kStages - 2>();
+    cp_wait<S - 2>();
     __syncthreads();
-    issue(c + kStages - 1);
-    const uint32_t st = base + (c - c0) % kStages * STAGE;
+    issue(c + S - 1);
+    const uint32_t st = use * STAGE;
+    if (++use == S) use = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint32_t x[4];
-      ldsm4(st + xr * 128 + (((2 * k + xh) ^ (xr & 7)) << 4), x);
+      ldsm4(st + xo[k], x);
 #pragma unroll
       for (int i = 0; i < MT; i += 2) {
-        // (one group of 8 only: its lines are addressed twice)
-        const int r = r0 + 8 * i + (MT == 1 ? (lane & 7) : ar);
         uint32_t w[4];
-        ldsm4(st + (kTile + r) * 128 + (((2 * k + ah) ^ (r & 7)) << 4), w);
+        ldsm4(st + ao[k] + 1024 * i, w);
 #pragma unroll
         for (int h = 0; h < (MT == 1 ? 1 : 2); ++h) {
           if (AT == AD_F16) {
@@ -594,31 +637,63 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
       const int m = tg + g + 8 * h;
       if (m < tl.rows)
         *reinterpret_cast<float2*>(dst + static_cast<int64_t>(m) * RP + r0 + 8 * i + 2 * t) =
-            make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+            make_float2(__fmul_rn(acc[i][2 * h], scale), __fmul_rn(acc[i][2 * h + 1], scale));
     }
-  pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ many rows: second product
-// CTA (tile, share of N): the shares of K are summed in order, then warps take 64 columns x NT * 8 rows.
+// CTA (tile, 512 columns of N, 256 where y is fp32): a warp takes 64 columns, and goes through the tile's rows (or
+// half of them) 8 * NT at a time. The tile's part of y, its rows and its B rows do not depend on the first
+// product: they are on their way (y by asynchronous copies) while that runs, so what follows it is the sums of
+// the shares of K in order, the MMAs and the stores.
+template <bool Y32>
+struct ExpandCfg {
+  static constexpr int BLOCKS = Y32 ? 4 : 8;            // 64-column blocks of a CTA
+  static constexpr int COLS = 64 * BLOCKS;
+  static constexpr int YPITCH = COLS * (Y32 ? 4 : 2) + 16;  // bytes; rows 2t of a quarter warp on distinct banks
+  static constexpr int YBYTES = kTile * YPITCH;
+};
+
 template <int AT, bool VEC, bool Y32>
 __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int NT = 2;
+  using C = ExpandCfg<Y32>;
+  constexpr int NT = Y32 ? 1 : 2, HALVES = kLoraWarps / C::BLOCKS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[kTile];
-  uint16_t* hf = reinterpret_cast<uint16_t*>(smem);
+  uint16_t* hf = reinterpret_cast<uint16_t*>(smem + C::YBYTES);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  pdl_wait();
   const int ti = blockIdx.x / p.nsplit, np = blockIdx.x - ti * p.nsplit;
-  if (ti >= *p.n_tiles) return;
-  const int4 tile = p.tiles[ti];
-  if (tile.x < 0 && p.skip_plain) return;
-  const LoraTile tl = lora_tile(p, tile.x, tile.z);
+  const int4 tile = p.tiles[ti];  // (only tiles below n_tiles are written, but there is room for every ti)
+  if (ti >= *p.n_tiles || (tile.x < 0 && p.skip_plain)) {
+    pdl_wait();
+    return;
+  }
+  const LoraTile tl = {tile.x, tile.z, tile.w, 1.f};
+  if (tid < kTile) tok[tid] = tid < tl.rows ? p.perm[tile.y + tid] : 0;
+  __syncthreads();
   const int ns = p.out_f32 ? 3 : 2;
   const int rchunks = (tl.rank + 31) / 32;
   const int hpitch = 32 * ((p.rp + 31) / 32) + 8, hs = kTile * hpitch;
-  if (tid < kTile) tok[tid] = tid < tl.rows ? p.perm[tile.y + tid] : 0;
+  const int col0 = np * C::COLS, n0 = col0 + 64 * (warp % C::BLOCKS);
+  const bool busy = n0 < p.N;
+  auto load_y = [&]() {
+    if (p.vy) {  // 16 bytes a copy, whole rows of the tile
+      constexpr int per = C::COLS * (Y32 ? 4 : 2) / 16, each = Y32 ? 4 : 8;
+      for (int i = tid; i < tl.rows * per; i += kLoraThreads) {
+        const int m = i / per, n = col0 + (i % per) * each;
+        if (n + each <= p.N)
+          cp_async16(smem_u32(smem) + m * C::YPITCH + (i % per) * 16,
+                     static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2), 16);
+      }
+    }
+    cp_commit();
+  };
+  if (!p.wait_y) load_y();
+  uint4 vb[8];
+  if (busy && rchunks > 0) load_b<VEC>(p, tl, n0, 8 * t, g, vb);
+  pdl_wait();
+  if (p.wait_y) load_y();
   for (int e = tid; e < tl.rows * rchunks * 16; e += kLoraThreads) {
     const int m = e / (rchunks * 16), r = 2 * (e - m * rchunks * 16);
     float2 v = make_float2(0.f, 0.f);
@@ -631,21 +706,21 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
         v.y = __fadd_rn(v.y, o.y);
       }
     }
-    v.x = r < tl.rank ? __fmul_rn(v.x, tl.scale) : 0.f;
-    v.y = r + 1 < tl.rank ? __fmul_rn(v.y, tl.scale) : 0.f;
+    // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
+    if (r >= tl.rank) v.x = 0.f;
+    if (r + 1 >= tl.rank) v.y = 0.f;
     uint32_t w[3];
     pieces(v, ns, w);
     for (int s = 0; s < ns; ++s) reinterpret_cast<uint32_t*>(hf)[(s * hs + m * hpitch + r) >> 1] = w[s];
   }
+  cp_wait<0>();
   __syncthreads();
-  const int nblk = (p.N + 63) / 64;
-  const int nb0 = static_cast<int>(static_cast<int64_t>(nblk) * np / p.nsplit);
-  const int nb1 = static_cast<int>(static_cast<int64_t>(nblk) * (np + 1) / p.nsplit);
+  pdl_launch_dependents();
+  if (!busy) return;
+  const uint8_t* ys = smem + (n0 - col0 + 8 * g) * (Y32 ? 4 : 2);
   const int groups = (tl.rows + 8 * NT - 1) / (8 * NT);
-  for (int it = warp; it < (nb1 - nb0) * groups; it += kLoraWarps) {
-    const int nb = nb0 + it / groups, nt0 = (it % groups) * NT;
-    YTile<NT, Y32> yt;
-    yt.load(p, tok, tl.rows, nb * 64, lane, nt0);
+  for (int gr = warp / C::BLOCKS; gr < groups; gr += HALVES) {
+    const int nt0 = gr * NT;
     float acc[4][NT][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -654,20 +729,27 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[q][j][i] = -0.f;  // y + -0 is y, also for y = -0
     for (int rc = 0; rc < rchunks; ++rc) {
-      uint4 vb[8];
-      load_b<VEC>(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
+      if (rchunks > 1 && (gr >= HALVES || rc)) load_b<VEC>(p, tl, n0, 32 * rc + 8 * t, g, vb);
       expand_step<NT, AT>(acc, vb, hf, hpitch, hs, ns, nt0, tl.rows, rc, lane);
     }
-    store_rows<NT, Y32>(p, tok, tl.rows, nb * 64, lane, acc, yt, nt0);
+    YTile<NT, Y32> yt;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < (Y32 ? 2 : 1); ++i)
+          yt.v[j][e][i] = reinterpret_cast<const uint4*>(ys + (8 * (nt0 + j) + 2 * t + e) * C::YPITCH)[i];
+    store_rows<NT, Y32>(p, tok, tl.rows, n0, lane, acc, yt, nt0);
   }
-  pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ plan: rows ordered by adapter
 // Counting sort of the rows by id in one CTA: perm (rows of an adapter together), and tiles of at most
-// kTile of them. Rows of a warp that share an id take one atomic (the rows of a prompt all do). The order
+// kTile of them (with the adapter's rank). Rows of a warp that share an id take one atomic (the rows of a prompt all do). The order
 // inside an adapter follows the atomics; a row's result does not depend on its place in a tile.
-__global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __restrict__ ids, int M, int L,
+__global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __restrict__ ids,
+                                                              const int32_t* __restrict__ ranks, int M, int L, int R,
                                                               int32_t* __restrict__ perm, int4* __restrict__ tiles,
                                                               int32_t* __restrict__ n_tiles, int* status) {
   extern __shared__ int cnt[];  // [L + 1]; L = rows without an adapter
@@ -745,7 +827,8 @@ __global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __r
   for (int k = k0; k < k1; ++k) {
     const int n = cnt[k];
     cnt[k] = r0;
-    for (int i = 0; i < n; i += kTile) tiles[t0++] = make_int4(k == L ? -1 : k, r0 + i, min(kTile, n - i), 0);
+    const int rank = (k == L || n == 0) ? 0 : ranks ? min(max(ranks[k], 0), R) : R;
+    for (int i = 0; i < n; i += kTile) tiles[t0++] = make_int4(k == L ? -1 : k, r0 + i, min(kTile, n - i), rank);
     r0 += n;
   }
   __syncthreads();
@@ -813,8 +896,9 @@ static int direct_launch(LoraParams& p, cudaStream_t s, bool pdl) {
   const int rc = set_smem_attr_once(kern, LoraCfg<MT>::TOTAL, attr, "cudaFuncSetAttribute(lora)");
   if (rc) return rc;
   void* args[1] = {&p};
-  // a cluster for every row that may lead a tile
-  return launch(kern, p.M * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, kDirectCtas, s, pdl, args, "aipu_lora_kernel");
+  // a cluster for every tile that there may be
+  const int tiles = std::min(p.M, p.M / kDirectTile + std::min(p.L + 1, p.M));
+  return launch(kern, tiles * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, kDirectCtas, s, pdl, args, "aipu_lora_kernel");
 }
 template <int MT>
 static int direct_launch_t(LoraParams& p, bool vec, cudaStream_t s, bool pdl) {
@@ -828,7 +912,7 @@ static int direct_launch_t(LoraParams& p, bool vec, cudaStream_t s, bool pdl) {
 
 template <int MT, int AT, bool VEC>
 static int shrink_launch(LoraParams& p, cudaStream_t s) {
-  constexpr int smem = kStages * (kTile + 16 * MT) * 128;
+  constexpr int smem = kStages<MT> * (kTile + 16 * MT) * 128;
   const void* kern = reinterpret_cast<const void*>(aipu_lora_shrink_kernel<MT, AT, VEC>);
   static bool attr[64] = {false};
   const int rc = set_smem_attr_once(kern, smem, attr, "cudaFuncSetAttribute(lora shrink)");
@@ -845,10 +929,10 @@ static int shrink_launch_t(LoraParams& p, bool vec, cudaStream_t s) {
 
 template <int AT, bool VEC, bool Y32>
 static int expand_launch(LoraParams& p, cudaStream_t s, bool pdl) {
-  const int smem = 3 * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
+  const int smem = ExpandCfg<Y32>::YBYTES + (p.out_f32 ? 3 : 2) * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
   const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, VEC, Y32>);
   static bool attr[64] = {false};
-  const int rc = set_smem_attr_once(kern, 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
+  const int rc = set_smem_attr_once(kern, ExpandCfg<Y32>::YBYTES + 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
   if (rc) return rc;
   void* args[1] = {&p};
   return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, 1, s, pdl, args,
@@ -886,14 +970,12 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   p.tiles = reinterpret_cast<int4*>(b);
   p.sums = reinterpret_cast<float*>(b + al256l(16 * max_tiles(p.M, p.L)));
   p.ksplit = k_split(p.M, p.L);
-  // shares of N: about three CTAs an SM, of eight 64-column blocks at least
-  const int64_t likely = std::max<int64_t>(1, p.M / kTile + std::min(p.L, p.M) / 2);
-  p.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((p.N + 255) / 256, 444 / likely)));
+  p.nsplit = p.y_f32 ? (p.N + ExpandCfg<true>::COLS - 1) / ExpandCfg<true>::COLS : (p.N + ExpandCfg<false>::COLS - 1) / ExpandCfg<false>::COLS;
   const void* kern = reinterpret_cast<const void*>(aipu_lora_plan_kernel);
   static bool attr[64] = {false};
   int rc = set_smem_attr_once(kern, (kMaxAdapters + 1) * 4, attr, "cudaFuncSetAttribute(lora plan)");
   if (rc) return rc;
-  void* args[7] = {&p.ids, &p.M, &p.L, &p.perm, &p.tiles, &p.n_tiles, &p.status};
+  void* args[9] = {&p.ids, &p.ranks, &p.M, &p.L, &p.R, &p.perm, &p.tiles, &p.n_tiles, &p.status};
   if ((rc = launch(kern, 1, 1024, static_cast<size_t>(p.L + 1) * 4, 1, s, pdl, args, "aipu_lora_plan_kernel"))) return rc;
   const bool vec = p.wa == 8 && p.wx == 8;
   switch (p.rp) {
