@@ -331,7 +331,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int id, int r
 }
 
 template <int MT, int AT, bool VEC, bool Y32>
-__global__ void __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
   using C = LoraCfg<MT>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[C::TM];
@@ -864,28 +864,19 @@ size_t lora_plan_bytes(int64_t M, int64_t L, int64_t R) {
          al256l(static_cast<size_t>(4) * M * padded_rank(R) * k_split(M, L));
 }
 
-static int launch(const void* kern, int grid, int block, size_t smem, int cluster, cudaStream_t s, bool pdl, void** args,
+static int launch(const void* kern, int grid, int block, size_t smem, cudaStream_t s, bool pdl, void** args,
                   const char* what) {
+  if (!pdl) return set_cuda_error(cudaLaunchKernel(kern, dim3(grid), dim3(block), args, smem, s), what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  int n = 0;
-  if (cluster > 1) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = cluster;
-    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (pdl) {
-    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = n;
+  cfg.numAttrs = 1;
   return set_cuda_error(cudaLaunchKernelExC(&cfg, kern, args), what);
 }
 
@@ -898,7 +889,7 @@ static int direct_launch(LoraParams& p, cudaStream_t s, bool pdl) {
   void* args[1] = {&p};
   // a cluster for every tile that there may be
   const int tiles = std::min(p.M, p.M / kDirectTile + std::min(p.L + 1, p.M));
-  return launch(kern, tiles * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, kDirectCtas, s, pdl, args, "aipu_lora_kernel");
+  return launch(kern, tiles * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, s, pdl, args, "aipu_lora_kernel");
 }
 template <int MT>
 static int direct_launch_t(LoraParams& p, bool vec, cudaStream_t s, bool pdl) {
@@ -918,7 +909,7 @@ static int shrink_launch(LoraParams& p, cudaStream_t s) {
   const int rc = set_smem_attr_once(kern, smem, attr, "cudaFuncSetAttribute(lora shrink)");
   if (rc) return rc;
   void* args[1] = {&p};
-  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.ksplit, kLoraThreads, smem, 1, s, true, args,
+  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.ksplit, kLoraThreads, smem, s, true, args,
                 "aipu_lora_shrink_kernel");
 }
 template <int MT>
@@ -935,7 +926,7 @@ static int expand_launch(LoraParams& p, cudaStream_t s, bool pdl) {
   const int rc = set_smem_attr_once(kern, ExpandCfg<Y32>::YBYTES + 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
   if (rc) return rc;
   void* args[1] = {&p};
-  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, 1, s, pdl, args,
+  return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, s, pdl, args,
                 "aipu_lora_expand_kernel");
 }
 template <int AT, bool VEC>
@@ -976,7 +967,7 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   int rc = set_smem_attr_once(kern, (kMaxAdapters + 1) * 4, attr, "cudaFuncSetAttribute(lora plan)");
   if (rc) return rc;
   void* args[9] = {&p.ids, &p.ranks, &p.M, &p.L, &p.R, &p.perm, &p.tiles, &p.n_tiles, &p.status};
-  if ((rc = launch(kern, 1, 1024, static_cast<size_t>(p.L + 1) * 4, 1, s, pdl, args, "aipu_lora_plan_kernel"))) return rc;
+  if ((rc = launch(kern, 1, 1024, static_cast<size_t>(p.L + 1) * 4, s, pdl, args, "aipu_lora_plan_kernel"))) return rc;
   const bool vec = p.wa == 8 && p.wx == 8;
   switch (p.rp) {
     case 16: return shrink_launch_t<1>(p, vec, s);

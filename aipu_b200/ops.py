@@ -44,12 +44,6 @@ def _on(ctx: Optional["Context"], *ts) -> tuple:
     return ctx, index
 
 
-def _contiguous(**ts):
-    for name, t in ts.items():
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-
-
 def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
@@ -357,13 +351,14 @@ def moe_combine(sel: torch.Tensor, sel_w: torch.Tensor, experts_per_piece: int, 
 # ------------------------------------------------------------------------------------ per-request adapters
 def _row_stride(t: torch.Tensor, name: str, rows: int, width: int) -> int:
     """Elements between the rows of a [rows, width] tensor whose rows are contiguous (columns of a wider tensor too)."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != rows or shape[1] != width:
+    if t.shape != (rows, width):
         raise ValueError(f"{name} must be [{rows}, {width}]")
+    if t.is_contiguous():
+        return width
     ld, step = t.stride()
-    if rows <= 1:
+    if rows == 1:
         ld = max(ld, width)
-    if rows and ((width > 1 and step != 1) or ld < width):
+    if (width > 1 and step != 1) or ld < width:
         raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
     return ld
 
@@ -381,31 +376,41 @@ class LoraAdapters:
 
     def cstruct(self) -> L.Lora:
         a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
-        sa, sb = a.shape, b.shape
-        if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2]:
+        if a.dim() != 3 or b.dim() != 3:
+            raise ValueError("adapters must be a [L, R, K] and b [L, N, R]")
+        n, R, K = a.shape
+        nb, N, Rb = b.shape
+        if n != nb or R != Rb:
             raise ValueError("adapters must be a [L, R, K] and b [L, N, R]")
         dtype = a.dtype
-        if b.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
+        code = _ADAPTER_DTYPE.get(dtype)
+        if code is None or b.dtype != dtype:
             raise ValueError("adapters must be bf16 or fp16, both the same")
-        if scale is not None and (scale.dtype != torch.float32 or scale.shape != sa[:1]):
-            raise ValueError("scale must be fp32 [L]")
-        if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != sa[:1]):
-            raise ValueError("ranks must be int32 [L]")
         if not (a.is_contiguous() and b.is_contiguous()):
             raise ValueError("a and b must be contiguous")
-        _contiguous(scale=scale, ranks=ranks)
-        return L.Lora(L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F16, sa[0], sa[1], sa[2], sb[1], a.data_ptr(),
-                      b.data_ptr(), scale.data_ptr() if scale is not None else None,
-                      ranks.data_ptr() if ranks is not None else None)
+        ps = pr = None
+        if scale is not None:
+            if scale.dtype != torch.float32 or scale.shape != (n,) or not scale.is_contiguous():
+                raise ValueError("scale must be fp32 [L], contiguous")
+            ps = scale.data_ptr()
+        if ranks is not None:
+            if ranks.dtype != torch.int32 or ranks.shape != (n,) or not ranks.is_contiguous():
+                raise ValueError("ranks must be int32 [L], contiguous")
+            pr = ranks.data_ptr()
+        return L.Lora(code, n, R, K, N, a.data_ptr(), b.data_ptr(), ps, pr)
 
 
-def _lora_inputs(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor) -> int:
+_ADAPTER_DTYPE = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
+
+
+def _lora_inputs(ids: torch.Tensor, x: torch.Tensor) -> int:
     """Rows of x; checks x and the rows' adapters."""
     if x.dtype != torch.bfloat16 or x.dim() != 2:
         raise ValueError("adapter activations must be bf16 [M, K]")
-    if ids.dtype != torch.int32 or ids.dim() != 1 or len(ids) != len(x) or not ids.is_contiguous():
+    M = x.shape[0]
+    if ids.dtype != torch.int32 or ids.shape != (M,) or not ids.is_contiguous():
         raise ValueError("ids must be int32 [M], contiguous, one for each row of x")
-    return len(x)
+    return M
 
 
 def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -414,22 +419,27 @@ def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tens
     projection that gave y (bf16 or fp32 [M, N]). x bf16 [M, K]; a negative id leaves the row as it is (an id >= L too,
     with bit 4 of the context's status set). Sums in fp32, one rounding. out: bf16 or y's type (default: like y); out=y
     adds in place, otherwise out must not overlap the inputs. x, y and out may be columns of wider tensors."""
-    M = _lora_inputs(ad, ids, x)
+    M = _lora_inputs(ids, x)
     cs = ad.cstruct()
     N = cs.out_features
     ldx, ldy = _row_stride(x, "x", M, cs.in_features), _row_stride(y, "y", M, N)
-    ydt = y.dtype
+    odt = ydt = y.dtype
     if out is None:
-        out = torch.empty_like(y, memory_format=torch.contiguous_format)
-    ldo = _row_stride(out, "out", M, N)
-    odt = out.dtype
+        out = torch.empty_like(y) if ldy == N else torch.empty_like(y, memory_format=torch.contiguous_format)
+        ldo = N
+    else:
+        ldo = _row_stride(out, "out", M, N)
+        odt = out.dtype
     if ydt not in _DTYPE or odt not in (torch.bfloat16, ydt):
         raise ValueError("y must be bf16 or fp32, out bf16 or y's type")
     ctx, index = _on(ctx, x, ids, y, out, ad.a, ad.b, ad.scale, ad.ranks)
-    n = lib().aipu_lora_workspace(M, cs.n_adapters, cs.rank)
+    so = lib()
+    n = so.aipu_lora_workspace(M, cs.n_adapters, cs.rank)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    check(lib().aipu_lora_add(ctx.handle, cs, ids.data_ptr(), x.data_ptr(), ldx, M, y.data_ptr(), _DTYPE[ydt], ldy,
-                              out.data_ptr(), _DTYPE[odt], ldo, ws.data_ptr() if n else None, n, _raw_stream(index)))
+    rc = so.aipu_lora_add(ctx.handle, cs, ids.data_ptr(), x.data_ptr(), ldx, M, y.data_ptr(), _DTYPE[ydt], ldy,
+                          out.data_ptr(), _DTYPE[odt], ldo, ws.data_ptr() if n else None, n, _raw_stream(index))
+    if rc:
+        check(rc)
     return out
 
 
@@ -438,11 +448,12 @@ def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: 
     """y[m] bf16 = x[m] W^T + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m]: a shared quantised projection (W = N GGUF rows
     of K weights, as in gemm) and the adapters of its rows, rounded once. Few rows run on the decode GEMV, 64 and more of
     Q4_K or Q6_K on the tensor-core GEMM."""
-    M = _lora_inputs(ad, ids, x)
+    M = _lora_inputs(ids, x)
     cs = ad.cstruct()
     if x.shape[1] != K or cs.in_features != K or cs.out_features != N:
         raise ValueError("x must be [M, K], a [L, R, K] and b [L, N, R]")
-    _contiguous(w=w, x=x, out=out)
+    if not (w.is_contiguous() and x.is_contiguous() and (out is None or out.is_contiguous())):
+        raise ValueError("w, x and out must be contiguous")
     if w.numel() * w.element_size() < N * row_bytes(wtype, K):
         raise ValueError("weight buffer smaller than N * row_bytes")
     if out is None:
@@ -450,10 +461,13 @@ def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: 
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
         raise ValueError("out must be bf16 [M, N]")
     ctx, index = _on(ctx, x, w, ids, out, ad.a, ad.b, ad.scale, ad.ranks)
-    n = lib().aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters, cs.rank)
+    so = lib()
+    n = so.aipu_q4k_gemm_lora_workspace(wtype, N, K, M, cs.n_adapters, cs.rank)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    check(lib().aipu_q4k_gemm_lora(ctx.handle, wtype, w.data_ptr(), N, K, x.data_ptr(), M, cs, ids.data_ptr(),
-                                   out.data_ptr(), ws.data_ptr() if n else None, n, _raw_stream(index)))
+    rc = so.aipu_q4k_gemm_lora(ctx.handle, wtype, w.data_ptr(), N, K, x.data_ptr(), M, cs, ids.data_ptr(),
+                               out.data_ptr(), ws.data_ptr() if n else None, n, _raw_stream(index))
+    if rc:
+        check(rc)
     return out
 
 
@@ -490,22 +504,24 @@ class LogitControls:
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
             return t.data_ptr()
 
-        s = L.LogitCtl()
-        if self.spans is not None or self.penalties is not None or self.tokens is not None:
-            s.spans = need(self.spans, "spans", torch.int64, (M, 3))
-            s.penalties = need(self.penalties, "penalties", torch.float32, (M, 3))
-            n = self.tokens.numel() if self.tokens is not None else 0
-            s.tokens, s.n_tokens = need(self.tokens, "tokens", torch.int32, (n,)), n
-        if self.bias_begin is not None or self.bias_ids is not None or self.bias_vals is not None:
-            s.bias_begin = need(self.bias_begin, "bias_begin", torch.int64, (M + 1,))
-            n = self.bias_ids.numel() if self.bias_ids is not None else 0
-            s.bias_ids, s.n_bias = need(self.bias_ids, "bias_ids", torch.int32, (n,)), n
-            s.bias_vals = need(self.bias_vals, "bias_vals", torch.float32, (n,))
-        if self.mask is not None or self.mask_rows is not None:
-            n = self.mask.shape[0] if self.mask is not None else 0
-            s.mask, s.n_masks = need(self.mask, "mask", torch.int32, (n, (V + 31) // 32)), n
-            s.mask_rows = need(self.mask_rows, "mask_rows", torch.int32, (M,))
-        return s
+        tokens, spans, pen, begin, bid, val, mask, rows = self.tensors()
+        nt = nb = nm = 0
+        pt = ps = pp = p0 = p1 = p2 = pm = pw = None
+        if spans is not None or pen is not None or tokens is not None:
+            nt = tokens.numel() if tokens is not None else 0
+            pt = need(tokens, "tokens", torch.int32, (nt,))
+            ps = need(spans, "spans", torch.int64, (M, 3))
+            pp = need(pen, "penalties", torch.float32, (M, 3))
+        if begin is not None or bid is not None or val is not None:
+            nb = bid.numel() if bid is not None else 0
+            p0 = need(begin, "bias_begin", torch.int64, (M + 1,))
+            p1 = need(bid, "bias_ids", torch.int32, (nb,))
+            p2 = need(val, "bias_vals", torch.float32, (nb,))
+        if mask is not None or rows is not None:
+            nm = mask.shape[0] if mask is not None else 0
+            pm = need(mask, "mask", torch.int32, (nm, (V + 31) // 32))
+            pw = need(rows, "mask_rows", torch.int32, (M,))
+        return L.LogitCtl(pt, nt, ps, pp, p0, p1, p2, nb, pm, pw, nm)
 
 
 def _logits(logits, controls, ctx, out, want_out):
@@ -514,15 +530,20 @@ def _logits(logits, controls, ctx, out, want_out):
     M, V = logits.shape
     ld = _row_stride(logits, "logits", M, V)
     cs = controls.cstruct(M, V) if controls is not None else None
-    if out is None and want_out:
-        out = torch.empty((M, V), dtype=torch.float32, device=logits.device)
-    ldo = _row_stride(out, "out", M, V) if want_out else 0
-    if want_out and out.dtype != torch.float32:
-        raise ValueError("out must be fp32 [M, V]")
+    ldo = V
+    if out is None:
+        if want_out:
+            out = torch.empty((M, V), dtype=torch.float32, device=logits.device)
+    else:
+        ldo = _row_stride(out, "out", M, V)
+        if out.dtype != torch.float32:
+            raise ValueError("out must be fp32 [M, V]")
     token = torch.empty(M, dtype=torch.int32, device=logits.device)
     ctx, index = _on(ctx, logits, out, *(controls.tensors() if controls is not None else ()))
-    check(lib().aipu_logits_process(ctx.handle, logits.data_ptr(), _DTYPE[logits.dtype], ld, M, V, cs,
-                                    out.data_ptr() if want_out else None, ldo, token.data_ptr(), _raw_stream(index)))
+    rc = lib().aipu_logits_process(ctx.handle, logits.data_ptr(), _DTYPE[logits.dtype], ld, M, V, cs,
+                                   out.data_ptr() if want_out else None, ldo, token.data_ptr(), _raw_stream(index))
+    if rc:
+        check(rc)
     return out, token
 
 
