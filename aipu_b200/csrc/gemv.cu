@@ -825,15 +825,52 @@ __device__ __forceinline__ int prescale_shift(float mx) {
   return s < -100 ? -100 : (s > 100 ? 100 : s);
 }
 
-// Stage the activations of group `grp` into shared memory as fp16 columns (see gemv.cuh). Tokens
-// are handled two at a time: 16-byte vectors are loaded once into registers (up to 4 per thread per
-// token), reduced for the per-token power-of-two prescale, converted and stored; for Q4_K the
-// 32-weight sub-block sums are reduced across the 4 (bf16) or 8 (fp32) lanes holding a sub-block.
+// One 16-byte vector of a token (vector v; lanes past the row have in = false) to its fp16 columns, and
+// for Q4_K the 32-weight sub-block sums, reduced across the 4 (bf16) or 8 (fp32) lanes holding a
+// sub-block. Every lane of the warp takes part.
+template <int WT, int XT>
+__device__ __forceinline__ void stage_token_vec(const uint4 q, bool in, float sc, uint8_t* colhi, uint8_t* collo,
+                                                uint8_t* sxs, int chi, int nsb, int v) {
+  constexpr int LPS = 32 / ((XT == XT_F32) ? 4 : 8);  // lanes holding one 32-weight sub-block
+  float shi = 0.f, slo = 0.f;
+  if (in) stage_vec<XT, WT != WT_F16>(q, sc, colhi, collo, v, shi, slo);
+  if (WT == WT_Q4K) {
+#pragma unroll
+    for (int o = 1; o < LPS; o <<= 1) {
+      shi = __fadd_rn(shi, __shfl_xor_sync(0xffffffffu, shi, o));
+      if (XT == XT_F32) slo = __fadd_rn(slo, __shfl_xor_sync(0xffffffffu, slo, o));
+    }
+    if (in && (v % LPS) == 0) {
+      const int sub = v / LPS;
+      // the fp32 sum as three fp16 parts (33 significant bits)
+      const __half hh = __float2half_rn(shi);
+      const float r1 = __fsub_rn(shi, __half2float(hh));
+      const __half hl = __float2half_rn(r1);
+      const __half hl2 = __float2half_rn(__fsub_rn(r1, __half2float(hl)));
+      __half* dst = reinterpret_cast<__half*>(sxs + (chi * nsb + sub / 8) * 64);
+      dst[sub & 7] = hh;
+      dst[8 + (sub & 7)] = hl;
+      dst[16 + (sub & 7)] = hl2;
+      if (XT == XT_F32) {
+        const __half lh = __float2half_rn(slo);
+        const float q1 = __fsub_rn(slo, __half2float(lh));
+        const __half ll = __float2half_rn(q1);
+        const __half ll2 = __float2half_rn(__fsub_rn(q1, __half2float(ll)));
+        __half* d2 = reinterpret_cast<__half*>(sxs + ((chi + 1) * nsb + sub / 8) * 64);
+        d2[sub & 7] = lh;
+        d2[8 + (sub & 7)] = ll;
+        d2[16 + (sub & 7)] = ll2;
+      }
+    }
+  }
+}
+
 // Stage the activations of group `grp` into group slot `xs_slot` as fp16 columns (all threads of
-// the CTA). Tokens two at a time: 16-byte vectors are loaded once into registers (up to 4 per
-// thread per token), reduced for the per-token power-of-two prescale, converted and stored; for
-// Q4_K the 32-weight sub-block sums are reduced across the 4 (bf16) or 8 (fp32) lanes holding a
-// sub-block. Leaves with a __syncthreads.
+// the CTA; see gemv.cuh): 16-byte vectors are reduced for the per-token power-of-two prescale,
+// converted and stored. One or two tokens: all threads on both, the vectors kept in registers (up to 4
+// per thread per token) between the two steps. More: a warp per token, so that all tokens' loads are in
+// flight at once and no barrier stands between the steps (the second step's loads come from L1). The
+// values are the same either way. Leaves with a __syncthreads.
 template <int WT, int XT, int EPI>
 __device__ void gemv_stage_x(const GemvParams& p, uint8_t* smem, const GemvLayout& L, int grp, int xs_slot,
                              int ncols, float* red) {
@@ -841,23 +878,60 @@ __device__ void gemv_stage_x(const GemvParams& p, uint8_t* smem, const GemvLayou
   const int NT = blockDim.x, NW = NT >> 5;
   constexpr int VEC = (XT == XT_F32) ? 4 : 8;
   constexpr int VPT = 4;
-  constexpr bool SWZ = (WT != WT_F16);
-  constexpr int LPS = 32 / VEC;  // lanes holding one 32-weight sub-block
   int* misc = reinterpret_cast<int*>(smem + L.off_misc) + xs_slot * 8;
   uint8_t* xs = smem + L.off_xs + xs_slot * ncols * p.xpitch;
   const int K = p.K, M = p.M, nv = K / VEC, nsb = K / 256;
   uint8_t* sxs = smem + L.off_sxs + xs_slot * ncols * nsb * 64;
   const uint4* xv = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.x) +
                                                    static_cast<int64_t>(grp) * p.x_group_stride * (XT == XT_F32 ? 4 : 2));
+  if (M > 2) {
+    const int lane = tid & 31;
+    for (int m = tid >> 5; m < M; m += NW) {
+      const uint4* row = xv + static_cast<int64_t>(m) * nv;
+      float mx = 0.f;
+      for (int v0 = lane; v0 < nv; v0 += 32 * 8) {  // nv is a multiple of 32
+        uint4 q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (v0 + 32 * j < nv) q[j] = __ldg(row + v0 + 32 * j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (v0 + 32 * j < nv) mx = vec_absmax(q[j], XT == XT_F32, mx);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const int sh = prescale_shift(mx);
+      const float sc = exp2i(-sh);
+      const int chi = (XT == XT_F32) ? 2 * m : m;
+      if (lane == 0) {
+        misc[chi] = sh;
+        if (XT == XT_F32) misc[chi + 1] = sh;
+      }
+      uint8_t* colhi = xs + chi * p.xpitch;
+      uint8_t* collo = (XT == XT_F32) ? xs + (chi + 1) * p.xpitch : colhi;
+      for (int v0 = lane; v0 < nv; v0 += 32 * 4) {
+        uint4 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v0 + 32 * j < nv) q[j] = __ldg(row + v0 + 32 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v0 - lane + 32 * j < nv)  // (warp-uniform: whole warps of vectors)
+            stage_token_vec<WT, XT>(q[j], true, sc, colhi, collo, sxs, chi, nsb, v0 + 32 * j);
+      }
+    }
+    __syncthreads();
+    return;
+  }
   const bool one_pass = nv <= VPT * NT;
-  for (int m0 = 0; m0 < M; m0 += 2) {
-    const int mt = min(2, M - m0);
+  {
+    const int mt = M;
     uint4 q[2][VPT];
     float mx[2] = {0.f, 0.f};
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
       if (t2 < mt) {
-        const uint4* row = xv + static_cast<int64_t>(m0 + t2) * nv;
+        const uint4* row = xv + static_cast<int64_t>(t2) * nv;
         if (one_pass) {
 #pragma unroll
           for (int j = 0; j < VPT; ++j) {
@@ -884,59 +958,28 @@ __device__ void gemv_stage_x(const GemvParams& p, uint8_t* smem, const GemvLayou
     if (tid == 0) {
       for (int t2 = 0; t2 < mt; ++t2) {
         if (XT == XT_F32) {
-          misc[2 * (m0 + t2)] = sh[t2];
-          misc[2 * (m0 + t2) + 1] = sh[t2];
+          misc[2 * t2] = sh[t2];
+          misc[2 * t2 + 1] = sh[t2];
         } else {
-          misc[m0 + t2] = sh[t2];
+          misc[t2] = sh[t2];
         }
       }
     }
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
       if (t2 >= mt) continue;
-      const int m = m0 + t2;
       const float sc = exp2i(-sh[t2]);
-      const int chi = (XT == XT_F32) ? 2 * m : m;
+      const int chi = (XT == XT_F32) ? 2 * t2 : t2;
       uint8_t* colhi = xs + chi * p.xpitch;
       uint8_t* collo = (XT == XT_F32) ? xs + (chi + 1) * p.xpitch : colhi;
-      const uint4* row = xv + static_cast<int64_t>(m) * nv;
+      const uint4* row = xv + static_cast<int64_t>(t2) * nv;
       const int nrounds = one_pass ? 1 : (nv + VPT * NT - 1) / (VPT * NT);
       for (int rd = 0; rd < nrounds; ++rd) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
           const int v = tid + (rd * VPT + j) * NT;
           if (!one_pass && v < nv) q[t2][j] = __ldg(row + v);
-          float shi = 0.f, slo = 0.f;
-          if (v < nv) stage_vec<XT, SWZ>(q[t2][j], sc, colhi, collo, v, shi, slo);
-          if (WT == WT_Q4K) {
-#pragma unroll
-            for (int o = 1; o < LPS; o <<= 1) {
-              shi = __fadd_rn(shi, __shfl_xor_sync(0xffffffffu, shi, o));
-              if (XT == XT_F32) slo = __fadd_rn(slo, __shfl_xor_sync(0xffffffffu, slo, o));
-            }
-            if (v < nv && (v % LPS) == 0) {
-              const int sub = v / LPS;
-              // the fp32 sum as three fp16 parts (33 significant bits)
-              const __half hh = __float2half_rn(shi);
-              const float r1 = __fsub_rn(shi, __half2float(hh));
-              const __half hl = __float2half_rn(r1);
-              const __half hl2 = __float2half_rn(__fsub_rn(r1, __half2float(hl)));
-              __half* dst = reinterpret_cast<__half*>(sxs + (chi * nsb + sub / 8) * 64);
-              dst[sub & 7] = hh;
-              dst[8 + (sub & 7)] = hl;
-              dst[16 + (sub & 7)] = hl2;
-              if (XT == XT_F32) {
-                const __half lh = __float2half_rn(slo);
-                const float q1 = __fsub_rn(slo, __half2float(lh));
-                const __half ll = __float2half_rn(q1);
-                const __half ll2 = __float2half_rn(__fsub_rn(q1, __half2float(ll)));
-                __half* d2 = reinterpret_cast<__half*>(sxs + ((chi + 1) * nsb + sub / 8) * 64);
-                d2[sub & 7] = lh;
-                d2[8 + (sub & 7)] = ll;
-                d2[16 + (sub & 7)] = ll2;
-              }
-            }
-          }
+          stage_token_vec<WT, XT>(q[t2][j], v < nv, sc, colhi, collo, sxs, chi, nsb, v);
         }
       }
     }
