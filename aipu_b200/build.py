@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaipu_q4k.so")
 DUMP = os.path.join(HERE, "aipu_dequant_dump")  # CLI over the C ABI (csrc/dequant_dump.cpp)
 
-SOURCES = ["capi.cu", "chain.cu", "ep.cu", "gemv.cu", "kernels.cu", "lmhead.cu", "logits.cu", "lora.cu", "tc_gemm.cu"]
+SOURCES = ["capi.cu", "chain.cu", "dense.cu", "ep.cu", "gemv.cu", "kernels.cu", "lmhead.cu", "logits.cu", "lora.cu", "tc_gemm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # No --use_fast_math and no -ftz: the exact kernels depend on IEEE fp32 with subnormals.
 # Per-file flags. chain.cu: its packed fp32 products and sums must round separately (the reference's

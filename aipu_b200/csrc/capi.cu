@@ -11,6 +11,7 @@
 #include "../../include/aipu_q4k.h"
 #include "common.cuh"
 #include "deq.cuh"
+#include "dense.cuh"
 #include "gemv.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -50,7 +51,7 @@ int launch_kernel(const void* kern, dim3 grid, dim3 block, int smem, cudaStream_
 }
 
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base, const cuuint64_t* dims,
-                 const cuuint64_t* strides, const cuuint32_t* box) {
+                 const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
   if (!encode) {
     cudaDriverEntryPointQueryResult qr;
@@ -61,7 +62,7 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const vo
   }
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = encode(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(ECUDA_, "tensor map encoding failed");
   return OK;
@@ -1377,15 +1378,16 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
   return lora_finish(p, s, pdl || p.tiles);
 }
 
-// rows from which the projection runs on the tcgen05 GEMM
-static bool gemm_lora_tc(int wtype, int64_t M) { return (wtype == AIPU_Q4_K || wtype == AIPU_Q6_K) && M >= 64; }
+// rows from which the projection dequantises its weights once and runs as an fp16 GEMM: above the rows of one
+// decode GEMV launch
+static bool gemm_lora_dense(int64_t M) { return M > 8; }
 
 extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank) {
   if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
       n_adapters > 32768 || rank < 1 || rank > 128)
     return 0;
   size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * static_cast<size_t>(M) * N);
-  if (gemm_lora_tc(wtype, M)) b += al256x(xt_bytes(M, K)) + al256x(4 * M);
+  if (gemm_lora_dense(M)) b += dense_bytes(wtype, N, K, M);
   return static_cast<int64_t>(b);
 }
 
@@ -1420,24 +1422,8 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   p.y_f32 = 1;
   p.status = c->status;
   if ((rc = lora_begin(p, plan, s, false))) return rc;
-  if (gemm_lora_tc(wtype, M)) {
-    uint8_t* xt = b;
-    int* shift = reinterpret_cast<int*>(xt + al256x(xt_bytes(M, K)));
-    rc = prescale_tiled_launch(p.x, p.M, p.K, nullptr, 0, static_cast<int>((M + 7) & ~7LL), nullptr, xt, shift, s, false);
-    if (rc) return rc;
-    TcParams t = {};
-    t.wt = wtype;
-    t.shared_id = -1;
-    t.w[0] = static_cast<const uint8_t*>(w);
-    t.row_bytes = row_bytes_of(wtype, K);
-    t.N = p.N;
-    t.K = p.K;
-    t.M = p.M;
-    t.xt = xt;
-    t.xshift = shift;
-    t.y32 = y32;
-    t.status = c->status;
-    rc = tc_gemm_launch(t, 128, 1, static_cast<int>((M + 127) / 128), c->num_sms, s, true);
+  if (gemm_lora_dense(M)) {
+    rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, b, c->status, s);
   } else {
     for (int64_t m0 = 0; m0 < M && !rc; m0 += 8) {
       GemvParams g = {};

@@ -1,0 +1,356 @@
+// Projection of many token rows on the 5th-generation tensor cores, for every weight type, sm_100a.
+//
+//   y32[m, n] = sum_k x[m, k] * w[n, k],  x bf16, w = GGUF rows (Q4_K, Q6_K, Q8_0, F16), fp32 out
+//
+// Three kernels: the weights as fp16 rows, the tokens as fp16 rows, and a GEMM of the two (TMA tiles with
+// 128-byte swizzle, tcgen05.mma kind::f16, fp32 accumulators in TMEM). Dequantising once per call and not
+// once per token tile is what makes this faster than a GEMM that dequantises its own tiles as soon as there
+// are a few dozen rows: the fp16 rows (2 bytes a weight) stay in L2 between the kernels.
+//
+// Rounding: a token row is scaled by a power of two and is then exact in fp16 (bf16 has 8 bits; values below
+// 2^-24 of the row's largest lose bits). A weight is dequantised in fp32 as ggml defines it, scaled by a
+// power of two per row, and rounded to fp16: 2^-11 of the weight at most, independent from weight to weight,
+// so that a result differs by about 2^-12 of its typical size, a tenth of its own rounding to bf16. F16
+// weights are used as they are stored. Products are exact, sums fp32.
+#include <algorithm>
+
+#include "deq.cuh"
+#include "dense.cuh"
+#include "kernels.h"
+#include "launch.h"
+#include "tc.cuh"
+
+namespace aipu {
+
+// ------------------------------------------------------------------ operands
+// power of two that brings a magnitude of at most `bound` into [2^13, 2^14) (0 and not finite: some scale)
+__device__ __forceinline__ int scale_shift(float bound, int top) {
+  const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 0xFFu);
+  const int s = bound == 0.f ? 0 : e - 127 - top;
+  return min(max(s, -100), 100);
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 8 bytes from a 2-byte aligned address
+__device__ __forceinline__ uint2 ld8_a2(const uint8_t* p) {
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+  return make_uint2(__ldg(q) | (static_cast<uint32_t>(__ldg(q + 1)) << 16), __ldg(q + 2) | (static_cast<uint32_t>(__ldg(q + 3)) << 16));
+}
+
+// largest magnitude that the header of unit u (256 weights) of a row allows, from its scales
+template <int WT>
+__device__ __forceinline__ float unit_bound(const uint8_t* row, int u) {
+  if (WT == WT_Q4K) {
+    const uint32_t h = __ldg(reinterpret_cast<const uint32_t*>(row + 144 * u));
+    return fabsf(f16_bits_to_f32(h)) * 945.f + fabsf(f16_bits_to_f32(h >> 16)) * 63.f;
+  }
+  if (WT == WT_Q6K) return fabsf(f16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(row + 210 * u + 208)))) * 4096.f;
+  float m = 0.f;
+  for (int b = 0; b < 8; ++b)
+    m = fmaxf(m, fabsf(f16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(row + 272 * u + 34 * b)))) * 128.f);
+  return m;
+}
+
+// weights 8 l .. 8 l + 7 of unit u, with the roundings of ggml's dequantisation
+template <int WT>
+__device__ __forceinline__ void unit_weights(const uint8_t* row, int u, int l, float (&w)[8]) {
+  if (WT == WT_Q4K) {
+    const uint8_t* b = row + 144 * u;
+    const uint4 h = __ldg(reinterpret_cast<const uint4*>(b));  // d, dmin, 12 bytes of scales
+    const int j = l >> 2, i = j & 3;
+    const uint32_t near = h.y >> (8 * i), far = h.z >> (8 * i), both = h.w >> (8 * i);
+    const uint32_t sc = j < 4 ? near & 63u : (both & 15u) | ((near >> 6 & 3u) << 4);
+    const uint32_t mn = j < 4 ? far & 63u : (both >> 4 & 15u) | ((far >> 6 & 3u) << 4);
+    const float d = __fmul_rn(f16_bits_to_f32(h.x), static_cast<float>(sc));
+    const float m = __fmul_rn(f16_bits_to_f32(h.x >> 16), static_cast<float>(mn));
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(b + 16 + 32 * (j >> 1) + 8 * (l & 3)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t code = (k < 4 ? q.x : q.y) >> (8 * (k & 3) + 4 * (j & 1)) & 15u;
+      w[k] = __fsub_rn(__fmul_rn(d, static_cast<float>(code)), m);
+    }
+  } else if (WT == WT_Q6K) {
+    const uint8_t* b = row + 210 * u;
+    const int half = l >> 4, run = (l >> 2) & 3, n = 8 * (l & 3);
+    const uint2 lo = ld8_a2(b + 64 * half + 32 * (run & 1) + n), hi = ld8_a2(b + 128 + 32 * half + n);
+    const int sc = static_cast<int8_t>(__ldg(b + 192 + (l >> 1)));
+    const float d = __fmul_rn(f16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(b + 208))), static_cast<float>(sc));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t nib = (k < 4 ? lo.x : lo.y) >> (8 * (k & 3) + 4 * (run >> 1)) & 15u;
+      const uint32_t top = (k < 4 ? hi.x : hi.y) >> (8 * (k & 3) + 2 * run) & 3u;
+      w[k] = __fmul_rn(d, static_cast<float>(static_cast<int>(nib | (top << 4)) - 32));
+    }
+  } else {
+    const uint8_t* b = row + 272 * u + 34 * (l >> 2);
+    const float d = f16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(b)));
+    const uint2 q = ld8_a2(b + 2 + 8 * (l & 3));
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      w[k] = __fmul_rn(d, static_cast<float>(static_cast<int8_t>((k < 4 ? q.x : q.y) >> (8 * (k & 3)) & 255u)));
+  }
+}
+
+// A warp per weight row: its scale from the blocks' headers, then 256 weights a step, 16 bytes a lane.
+template <int WT>
+__global__ void __launch_bounds__(256) aipu_dense_weights_kernel(const uint8_t* __restrict__ w, int N, int K, int64_t row_bytes,
+                                                                 uint16_t* __restrict__ out, int* __restrict__ shift) {
+  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (n >= N) return;
+  const uint8_t* row = w + n * row_bytes;
+  const int units = K / 256;
+  float bound = 0.f;
+  for (int u = lane; u < units; u += 32) bound = fmaxf(bound, unit_bound<WT>(row, u));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+  const int s = scale_shift(bound, 13);
+  const float f = exp2i(-s);
+  if (lane == 0) shift[n] = s;
+  uint4* dst = reinterpret_cast<uint4*>(out + static_cast<int64_t>(n) * K) + lane;
+#pragma unroll 2
+  for (int u = 0; u < units; ++u) {
+    float v[8];
+    unit_weights<WT>(row, u, lane, v);
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = half2_bits(__fmul_rn(v[2 * k], f), __fmul_rn(v[2 * k + 1], f));
+    dst[32 * u] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// A CTA per token row: its scale from the largest magnitude (into [2^9, 2^10)), then fp16.
+__global__ void __launch_bounds__(128) aipu_dense_tokens_kernel(const uint16_t* __restrict__ x, int K, uint16_t* __restrict__ out,
+                                                                int* __restrict__ shift) {
+  __shared__ float red[4];
+  const int m = blockIdx.x, tid = threadIdx.x;
+  const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(m) * K);
+  const int nv = K / 8;
+  float mx = 0.f;
+  for (int v = tid; v < nv; v += 128) {
+    const uint4 q = __ldg(src + v);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if ((tid & 31) == 0) red[tid >> 5] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int s = scale_shift(mx, 9);
+  const float f = exp2i(-s);
+  if (tid == 0) shift[m] = s;
+  uint4* dst = reinterpret_cast<uint4*>(out + static_cast<int64_t>(m) * K);
+  for (int v = tid; v < nv; v += 128) {
+    const uint4 q = __ldg(src + v);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = half2_bits(__fmul_rn(__uint_as_float(w[i] << 16), f), __fmul_rn(__uint_as_float(w[i] & 0xFFFF0000u), f));
+    dst[v] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ------------------------------------------------------------------ GEMM
+struct DenseParams {
+  alignas(64) CUtensorMap wmap;  // [N][K] fp16, box 128 rows x 64 k, 128-byte swizzle
+  alignas(64) CUtensorMap xmap;  // [M][K] fp16, box NT rows x 64 k
+  const int* wshift;             // [N] or nullptr (0)
+  const int* xshift;             // [M]
+  float* y;
+  int N, K, M;
+  int* status;
+};
+
+constexpr int kDenseThreads = 320;  // 8 epilogue warps, the copy warp, the MMA warp
+
+template <int NT>
+struct DenseCfg {
+  static constexpr int A = 128 * 128, B = NT * 128;  // bytes of a stage: 64 k of 128 weight rows and NT token rows
+  static constexpr int STAGE = A + B;
+  static constexpr int S = 196608 / STAGE;           // stages in 192 KB: 4, 6 or 8
+  static constexpr int TOTAL = S * STAGE + 1024;     // (tiles start on 1024 bytes)
+};
+
+struct DenseBars {
+  uint64_t full[8], empty[8], done;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// One 128 x NT tile of (weight rows, token rows) a CTA. Copy warp: a stage is one TMA box of each operand.
+// MMA warp: four K = 16 steps a stage, one thread; a commit releases the stage. Epilogue: TMEM lane =
+// weight row, so a warp's store is 32 neighbouring results of a token. Every wait is bounded: on expiry the
+// status word is set, the roles leave, copies and MMAs in flight are waited for (bounded), TMEM is freed.
+template <int NT>
+__global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const __grid_constant__ DenseParams p) {
+  using C = DenseCfg<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ DenseBars bars;
+  __shared__ int xs[NT];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int n0 = blockIdx.x * 128, m0 = blockIdx.y * NT;
+  if (tid == 0) {
+    for (int i = 0; i < C::S; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    mbar_init(&bars.done, 1);
+    bars.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(&bars.tmem, NT);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  pdl_wait();
+  const int steps = p.K / 64;
+  volatile int* abort = &bars.abort;
+  if (warp == 8) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < steps && !*abort; ++i, ++issued) {
+        const int s = i % C::S;
+        if (i >= C::S && !mbar_wait_bounded(&bars.empty[s], (i / C::S + 1) & 1, p.status, ST_TIMEOUT_EMPTY)) {
+          *abort = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&bars.full[s], C::STAGE);
+        tma_load_2d(base + s * C::STAGE, &p.wmap, 64 * i, n0, &bars.full[s]);
+        tma_load_2d(base + s * C::STAGE + C::A, &p.xmap, 64 * i, m0, &bars.full[s]);
+      }
+      if (*abort)  // no copy may land after the CTA has ended
+        for (int i = max(0, issued - C::S); i < issued; ++i)
+          mbar_wait_bounded(&bars.full[i % C::S], (i / C::S) & 1, p.status, ST_TIMEOUT_FULL, 200000000LL);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_f16(128, NT);
+      for (int i = 0; i < steps; ++i) {
+        const int s = i % C::S;
+        if (*abort || !mbar_wait_bounded(&bars.full[s], (i / C::S) & 1, p.status, ST_TIMEOUT_FULL)) {
+          *abort = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = base + s * C::STAGE, b = a + C::A;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16(tmem, umma_desc_sw128(a + 32 * k, 1024), umma_desc_sw128(b + 32 * k, 1024), idesc, (i | k) ? 1u : 0u);
+        umma_commit(&bars.empty[s]);
+      }
+      umma_commit(&bars.done);
+    }
+  } else {
+    for (int i = tid; i < NT; i += 256) xs[i] = m0 + i < p.M ? p.xshift[m0 + i] : 0;
+    named_bar_sync(1, 256);
+    const int q = warp & 3, n = n0 + 32 * q + lane;
+    const int ws = (p.wshift && n < p.N) ? p.wshift[n] : 0;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL)) && !*abort;
+    if (ok) {
+      tc_fence_after();
+      const int cols = min(NT, p.M - m0);
+#pragma unroll 1
+      for (int c0 = (warp >> 2) * 16; c0 < cols; c0 += 32) {
+        float v[16];
+        tmem_ld16(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0, v);
+        if (n < p.N) {
+          float* dst = p.y + static_cast<int64_t>(m0 + c0) * p.N + n;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < cols) dst[static_cast<int64_t>(j) * p.N] = __fmul_rn(__fmul_rn(v[j], exp2i(xs[c0 + j])), exp2i(ws));
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  if (warp == 9) {
+    mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL, 200000000LL);  // the MMAs in flight (after an abort too)
+    tc_fence_after();
+    tmem_dealloc(tmem, NT);
+    tmem_relinquish();
+  }
+}
+
+// ------------------------------------------------------------------ host
+static size_t al1k(size_t v) { return (v + 1023) & ~static_cast<size_t>(1023); }
+
+size_t dense_bytes(int wt, int64_t N, int64_t K, int64_t M) {
+  const size_t w = wt == WT_F16 ? 0 : al1k(static_cast<size_t>(2) * N * K) + al1k(4 * N);
+  return w + al1k(static_cast<size_t>(2) * M * K) + al1k(4 * M);
+}
+
+static int rows_map(CUtensorMap* map, const void* base, int rows, int K, int box) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
+  const cuuint32_t bx[2] = {64, static_cast<cuuint32_t>(box)};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, bx, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int NT>
+static int dense_launch(DenseParams& p, cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(aipu_dense_gemm_kernel<NT>);
+  static bool attr[64] = {false};
+  const int rc = set_smem_attr_once(kern, DenseCfg<NT>::TOTAL, attr, "cudaFuncSetAttribute(dense)");
+  if (rc) return rc;
+  return launch_kernel(kern, dim3((p.N + 127) / 128, (p.M + NT - 1) / NT), dim3(kDenseThreads), DenseCfg<NT>::TOTAL, s, true, &p);
+}
+
+int dense_gemm(int wt, const uint8_t* w, int N, int K, const uint16_t* x, int M, float* y32, void* scratch, int* status,
+               cudaStream_t s) {
+  if (K % 256 || K <= 0 || N <= 0 || M <= 0) return set_error(EINVAL_, "dense: K must be a multiple of 256");
+  uint8_t* b = static_cast<uint8_t*>(scratch);
+  DenseParams p = {};
+  const void* w16 = w;
+  if (wt != WT_F16) {
+    uint16_t* out = reinterpret_cast<uint16_t*>(b);
+    b += al1k(static_cast<size_t>(2) * N * K);
+    int* shift = reinterpret_cast<int*>(b);
+    b += al1k(4 * static_cast<size_t>(N));
+    const int64_t rb = row_bytes_of(wt, K);
+    const int grid = (N + 7) / 8;
+    if (wt == WT_Q4K) aipu_dense_weights_kernel<WT_Q4K><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
+    else if (wt == WT_Q6K) aipu_dense_weights_kernel<WT_Q6K><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
+    else aipu_dense_weights_kernel<WT_Q80><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return set_cuda_error(e, "aipu_dense_weights_kernel");
+    w16 = out;
+    p.wshift = shift;
+  }
+  uint16_t* x16 = reinterpret_cast<uint16_t*>(b);
+  b += al1k(static_cast<size_t>(2) * M * K);
+  int* xshift = reinterpret_cast<int*>(b);
+  aipu_dense_tokens_kernel<<<M, 128, 0, s>>>(x, K, x16, xshift);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e, "aipu_dense_tokens_kernel");
+  const int nt = M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  int rc = rows_map(&p.wmap, w16, N, K, 128);
+  if (!rc) rc = rows_map(&p.xmap, x16, M, K, nt);
+  if (rc) return rc;
+  p.xshift = xshift;
+  p.y = y32;
+  p.N = N;
+  p.K = K;
+  p.M = M;
+  p.status = status;
+  return nt == 64 ? dense_launch<64>(p, s) : nt == 128 ? dense_launch<128>(p, s) : dense_launch<256>(p, s);
+}
+
+}  // namespace aipu

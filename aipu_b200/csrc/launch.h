@@ -26,10 +26,11 @@ int num_sms_of_current_device();
 // table of 64 device flags.
 int set_smem_attr_once(const void* kern, int bytes, bool* done, const char* what);
 
-// Encode a tiled TMA tensor map (no swizzle, no interleave, OOB reads return 0). The driver entry
+// Encode a tiled TMA tensor map (no interleave, OOB reads return 0). The driver entry
 // point is looked up through the runtime, so the library does not link libcuda.
 // dims/box in elements (innermost first); strides in bytes for dims 1..rank-1.
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base, const cuuint64_t* dims,
-                 const cuuint64_t* strides, const cuuint32_t* box);
+                 const cuuint64_t* strides, const cuuint32_t* box,
+                 CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
 }  // namespace aipu

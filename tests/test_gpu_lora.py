@@ -8,8 +8,10 @@ the value, eps(t) / 2: bf16 has 8 significant bits, so 2^-8; fp32 2^-24. Error s
     2^-24: the MMA's sums may truncate). Sums run through blocks, so K / 16 + 64 bounds the length;
   * h as bf16 pieces: the first is h truncated to 8 bits, its rest is below 2^-7 |h|; two pieces (bf16
     result) round that rest by 2^-8 of itself, 2^-15 |h|; three (fp32 result) hold all 24 bits;
-  * for gemm, the projection's own sum of K products, 4 * K * 2^-24 relative to its magnitudes.
+  * for gemm, the projection's own sum of K products, 4 * K * 2^-24 relative to its magnitudes, and its
+    operands' rounding (see there).
 With S = sum_r |scale| (sum_k |x a|) |b| every term is at most a fixed multiple of S."""
+import numpy as np
 import pytest
 import torch
 
@@ -206,28 +208,61 @@ def test_gemm_lora_matches_the_definition(wt, M, K, N, R):
     A.b.mul_(float(wd.square().mean().sqrt()) * K ** 0.5)  # a share of the result that 16 bits show
     d, s = _delta(A, ids, x)
     o = ops.gemm_lora(wt, w, N, K, x, A, ids)
-    # the projection: fp32 sums of its products; Q4_K's d * sum - dmin * sum and Q6_K's rounded operand
-    # (2^-12 of a weight, tcgen05 path) are relative to the same magnitudes
+    # the projection's fp32 sums: relative to the magnitudes of its products
     mag = x64.abs() @ wd.abs().t()
-    if wt == F.Q4_K:  # |d sc q| + |dmin m| of every weight: at most |w| + 2 |dmin m|
-        b = w.view(-1, 144).cpu().numpy()
-        import numpy as np
-        dm = np.ascontiguousarray(b[:, 2:4]).view(np.float16).astype(np.float64).reshape(N, K // 256)
-        mag = mag + 2 * 63 * (x64.abs().view(M, -1, 256).sum(2) @ torch.from_numpy(dm).t())
-    few = M < 64 or wt not in (F.Q4_K, F.Q6_K)
-    # one token: the integer engine rounds x once to 2^-21 of the row's maximum, relative to sums of |w|
-    x_round = 2.0 ** -21 * x64.abs().amax(1, keepdim=True) * wd.abs().sum(1) if few and M == 1 else 0.0
-    extra = mag * (4 * K * 2.0 ** -24 + (0.0 if few or wt != F.Q6_K else 2.0 ** -12)) + x_round
+    if M > 8 and wt != F.F16:
+        # fp16 GEMM: a weight is rounded by 2^-11 of itself at most (half a step), and the tokens, scaled to 2^9 .. 2^10,
+        # by half the smallest fp16 step, 2^-25, where they are small: 2^-34 of the row's largest
+        extra = mag * (4 * K * 2.0 ** -24 + 2.0 ** -11)
+    else:
+        if wt == F.Q4_K and M <= 8:  # d * sum - dmin * sum: |d sc q| + |dmin m| of a weight is at most |w| + 2 |dmin m|
+            dm = np.ascontiguousarray(w.view(-1, 144).cpu().numpy()[:, 2:4]).view(np.float16).astype(np.float64).reshape(N, K // 256)
+            mag = mag + 2 * 63 * (x64.abs().view(M, -1, 256).sum(2) @ torch.from_numpy(dm).t())
+        extra = mag * (4 * K * 2.0 ** -24)
+    if M == 1:  # the integer engine rounds x once to 2^-21 of the row's maximum, relative to sums of |w|
+        extra = extra + 2.0 ** -21 * x64.abs().amax(1, keepdim=True) * wd.abs().sum(1)
+    if M > 8:
+        extra = extra + 2.0 ** -34 * x64.abs().amax(1, keepdim=True) * wd.abs().sum(1)
     _check(o, x64 @ wd.t(), d, s, K, extra)
 
 
 def test_gemm_lora_without_adapters_is_the_projection():
-    """Rows without an adapter: the bits of gemm (few rows) and of gemm_tc (many)."""
-    for M, ref in ((1, ops.gemm), (5, ops.gemm), (100, ops.gemm_tc)):
+    """Rows without an adapter: up to 8 rows give the bits of gemm; more rows do not depend on the adapters at all."""
+    for M in (1, 5, 8, 100):
         A, _, x = _case(M, 512, 200, 8, 2)
         ids = torch.full((M,), -1, dtype=torch.int32, device=x.device)
         w = torch.from_numpy(F.random_rows_np(F.Q4_K, 200, 512, seed=3)).to(x.device)
-        assert torch.equal(ops.gemm_lora(F.Q4_K, w, 200, 512, x, A, ids), ref(F.Q4_K, w, 200, 512, x))
+        o = ops.gemm_lora(F.Q4_K, w, 200, 512, x, A, ids)
+        if M <= 8:
+            assert torch.equal(o, ops.gemm(F.Q4_K, w, 200, 512, x))
+        A.a.fill_(float("nan"))
+        assert torch.equal(ops.gemm_lora(F.Q4_K, w, 200, 512, x, A, ids), o)
+
+
+@pytest.mark.parametrize("wt", [F.Q4_K, F.Q6_K, F.Q8_0, F.F16])
+@pytest.mark.parametrize("M,K,N", [(9, 256, 1), (64, 2048, 128), (65, 256, 129), (128, 512, 127), (129, 768, 300), (256, 512, 256),
+                                   (257, 256, 640), (700, 2304, 520)])
+def test_gemm_lora_many_rows_at_tile_borders(wt, M, K, N):
+    """Weights of the extremes too: scales of zero, of fp16's smallest and of its largest numbers, in some rows."""
+    A, ids, x = _case(M, K, N, 8, 2)
+    w_np = F.random_rows_np(wt, N, K, seed=N + 1)
+    if wt != F.F16:
+        bb, at = F.BLOCK_BYTES[wt], {F.Q4_K: 0, F.Q6_K: 208, F.Q8_0: 0}[wt]
+        blocks = w_np.reshape(N, -1, bb)
+        for row, scale in ((0, 0.0), (N // 2, 2.0 ** -24), (N - 1, 300.0)):
+            blocks[row, :, at:at + 2] = np.frombuffer(np.float16(scale).tobytes(), np.uint8)
+            if wt == F.Q4_K:
+                blocks[row, :, 2:4] = 0
+    w = torch.from_numpy(w_np).to(x.device)
+    x[0] = 0
+    x[M - 1] *= 2.0 ** 60
+    wd = ops.dequant(wt, w, N, K).double().cpu()
+    x64 = x.double().cpu()
+    ids.fill_(-1)
+    o = ops.gemm_lora(wt, w, N, K, x, A, ids)
+    mag, big = x64.abs() @ wd.abs().t(), x64.abs().amax(1, keepdim=True) * wd.abs().sum(1)
+    extra = mag * (4 * K * 2.0 ** -24 + (0.0 if wt == F.F16 else 2.0 ** -11)) + 2.0 ** -34 * big
+    _check(o, x64 @ wd.t(), torch.zeros_like(mag), torch.zeros_like(mag), K, extra)
 
 
 @pytest.mark.parametrize("M", [3, 90])
