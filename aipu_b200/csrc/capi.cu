@@ -1381,12 +1381,15 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
 // rows from which the projection dequantises its weights once and runs as an fp16 GEMM: above the rows of one
 // decode GEMV launch
 static bool gemm_lora_dense(int64_t M) { return M > 8; }
+// row stride of its fp32 sums: rows start on 32 bytes
+static int64_t gemm_lora_ld(int64_t N) { return (N + 7) & ~static_cast<int64_t>(7); }
 
 extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank) {
   if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
       n_adapters > 32768 || rank < 1 || rank > 128)
     return 0;
-  size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * static_cast<size_t>(M) * N);
+  const size_t parts = gemm_lora_dense(M) ? dense_parts(N, K, M) : 1;
+  size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * parts * M * gemm_lora_ld(N));
   if (gemm_lora_dense(M)) b += dense_bytes(wtype, N, K, M);
   return static_cast<int64_t>(b);
 }
@@ -1413,35 +1416,37 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   void* plan = b;
   b += al256x(lora_plan_bytes(M, p.L, p.R));
   float* y32 = reinterpret_cast<float*>(b);
-  b += al256x(4 * static_cast<size_t>(M) * N);
+  if (gemm_lora_dense(M)) p.yparts = dense_parts(N, K, M);
+  b += al256x(4 * static_cast<size_t>(std::max(p.yparts, 1)) * M * gemm_lora_ld(N));
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = K;
   p.y = y32;
-  p.ldy = p.ldo = N;
+  p.ldy = gemm_lora_ld(N);
+  p.ldo = N;
   p.out = y;
   p.y_f32 = 1;
   p.status = c->status;
   if ((rc = lora_begin(p, plan, s, false))) return rc;
   if (gemm_lora_dense(M)) {
-    rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, b, c->status, s);
+    // (beside the first product of the adapters, which was launched just before where there are many rows)
+    rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, p.ldy, b, c->status, s, p.tiles != nullptr);
   } else {
-    for (int64_t m0 = 0; m0 < M && !rc; m0 += 8) {
-      GemvParams g = {};
-      g.w0 = static_cast<const uint8_t*>(w);
-      g.row_bytes = row_bytes_of(wtype, K);
-      g.n_groups = 1;
-      g.N = p.N;
-      g.K = p.K;
-      g.x = p.x + m0 * K;
-      g.M = static_cast<int>(std::min<int64_t>(8, M - m0));
-      g.y32 = y32 + m0 * N;
-      g.partials = c->ws[0].partials;
-      g.counters = c->ws[0].counters;
-      g.status = c->status;
-      // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
-      // kernel behind it may read x, the ids and the adapters without waiting for it
-      rc = gemv_launch(wtype, XT_BF16, EPI_STORE, g, c->num_sms, s, false);
-    }
+    GemvParams g = {};
+    g.w0 = static_cast<const uint8_t*>(w);
+    g.row_bytes = row_bytes_of(wtype, K);
+    g.n_groups = 1;
+    g.N = p.N;
+    g.K = p.K;
+    g.x = p.x;
+    g.M = p.M;
+    g.y32 = y32;
+    g.y32_ld = p.ldy;
+    g.partials = c->ws[0].partials;
+    g.counters = c->ws[0].counters;
+    g.status = c->status;
+    // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
+    // kernel behind it may read x, the ids and the adapters without waiting for it
+    rc = gemv_launch(wtype, XT_BF16, EPI_STORE, g, c->num_sms, s, false);
   }
   if (rc) return rc;
   p.wait_y = 1;

@@ -2,10 +2,11 @@
 //
 //   y32[m, n] = sum_k x[m, k] * w[n, k],  x bf16, w = GGUF rows (Q4_K, Q6_K, Q8_0, F16), fp32 out
 //
-// Three kernels: the weights as fp16 rows, the tokens as fp16 rows, and a GEMM of the two (TMA tiles with
-// 128-byte swizzle, tcgen05.mma kind::f16, fp32 accumulators in TMEM). Dequantising once per call and not
-// once per token tile is what makes this faster than a GEMM that dequantises its own tiles as soon as there
-// are a few dozen rows: the fp16 rows (2 bytes a weight) stay in L2 between the kernels.
+// Two kernels: the weights and tokens as fp16 rows, and a GEMM of the two (TMA tiles with 128-byte swizzle,
+// tcgen05.mma kind::f16, fp32 accumulators in TMEM). Dequantising once per call and not once per token tile
+// is what makes this faster than a GEMM that dequantises its own tiles (2048 rows of 6144 x 2048: 60 us
+// against 145): the fp16 rows (2 bytes a weight) stay in L2 between the kernels. What bounds the GEMM is the
+// L2 traffic of its tiles (128 x 256: 590 MB for that case, 12.8 TB/s).
 //
 // Rounding: a token row is scaled by a power of two and is then exact in fp16 (bf16 has 8 bits; values below
 // 2^-24 of the row's largest lose bits). A weight is dequantised in fp32 as ggml defines it, scaled by a
@@ -95,66 +96,78 @@ __device__ __forceinline__ void unit_weights(const uint8_t* row, int u, int l, f
   }
 }
 
-// A warp per weight row: its scale from the blocks' headers, then 256 weights a step, 16 bytes a lane.
+// Both operands in one launch; four warps a row, two rows a CTA. The first CTAs take weight rows (their scale
+// from the blocks' headers, then 256 weights a warp and step, 16 bytes a lane), the others token rows (their
+// scale from the largest magnitude, into [2^9, 2^10)). It depends on nothing that the kernel before it
+// writes and only ends after it, so both run at the same time.
 template <int WT>
-__global__ void __launch_bounds__(256) aipu_dense_weights_kernel(const uint8_t* __restrict__ w, int N, int K, int64_t row_bytes,
-                                                                 uint16_t* __restrict__ out, int* __restrict__ shift) {
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (n >= N) return;
-  const uint8_t* row = w + n * row_bytes;
-  const int units = K / 256;
-  float bound = 0.f;
-  for (int u = lane; u < units; u += 32) bound = fmaxf(bound, unit_bound<WT>(row, u));
+__global__ void __launch_bounds__(256) aipu_dense_operands_kernel(const uint8_t* __restrict__ w, int N, int K, int64_t row_bytes,
+                                                                  uint16_t* __restrict__ w16, int* __restrict__ wshift,
+                                                                  const uint16_t* __restrict__ x, int M,
+                                                                  uint16_t* __restrict__ x16, int* __restrict__ xshift) {
+  __shared__ float red[2][4];
+  const int half = threadIdx.x >> 7, t = threadIdx.x & 127, warp = t >> 5, lane = t & 31;
+  const int wblocks = WT == WT_F16 ? 0 : (N + 1) / 2;
+  pdl_launch_dependents();  // (the GEMM waits for this grid before it reads)
+  if (WT != WT_F16 && blockIdx.x < wblocks) {
+    const int n = 2 * blockIdx.x + half;
+    if (n < N) {
+      const uint8_t* row = w + n * row_bytes;
+      const int units = K / 256;
+      float bound = 0.f;
+      for (int u = lane; u < units; u += 32) bound = fmaxf(bound, unit_bound<WT>(row, u));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
-  const int s = scale_shift(bound, 13);
-  const float f = exp2i(-s);
-  if (lane == 0) shift[n] = s;
-  uint4* dst = reinterpret_cast<uint4*>(out + static_cast<int64_t>(n) * K) + lane;
+      for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+      const int s = scale_shift(bound, 13);
+      const float f = exp2i(-s);
+      if (t == 0) wshift[n] = s;
+      uint4* dst = reinterpret_cast<uint4*>(w16 + static_cast<int64_t>(n) * K) + lane;
 #pragma unroll 2
-  for (int u = 0; u < units; ++u) {
-    float v[8];
-    unit_weights<WT>(row, u, lane, v);
-    uint32_t o[4];
+      for (int u = warp; u < units; u += 4) {
+        float v[8];
+        unit_weights<WT>(row, u, lane, v);
+        uint32_t o[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = half2_bits(__fmul_rn(v[2 * k], f), __fmul_rn(v[2 * k + 1], f));
-    dst[32 * u] = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 4; ++k) o[k] = half2_bits(__fmul_rn(v[2 * k], f), __fmul_rn(v[2 * k + 1], f));
+        dst[32 * u] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  } else {
+    const int m = 2 * (blockIdx.x - wblocks) + half;
+    if (m < M) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(m) * K);
+      const int nv = K / 8;
+      float mx = 0.f;
+#pragma unroll 4
+      for (int v = t; v < nv; v += 128) {
+        const uint4 q = __ldg(src + v);
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(u[i] << 16)), fabsf(__uint_as_float(u[i] & 0xFFFF0000u))));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (lane == 0) red[half][warp] = mx;
+      named_bar_sync(1 + half, 128);
+      mx = fmaxf(fmaxf(red[half][0], red[half][1]), fmaxf(red[half][2], red[half][3]));
+      const int s = scale_shift(mx, 9);
+      const float f = exp2i(-s);
+      if (t == 0) xshift[m] = s;
+      uint4* dst = reinterpret_cast<uint4*>(x16 + static_cast<int64_t>(m) * K);
+#pragma unroll 4
+      for (int v = t; v < nv; v += 128) {
+        const uint4 q = __ldg(src + v);
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[i] = half2_bits(__fmul_rn(__uint_as_float(u[i] << 16), f), __fmul_rn(__uint_as_float(u[i] & 0xFFFF0000u), f));
+        dst[v] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
   }
-}
-
-// A CTA per token row: its scale from the largest magnitude (into [2^9, 2^10)), then fp16.
-__global__ void __launch_bounds__(128) aipu_dense_tokens_kernel(const uint16_t* __restrict__ x, int K, uint16_t* __restrict__ out,
-                                                                int* __restrict__ shift) {
-  __shared__ float red[4];
-  const int m = blockIdx.x, tid = threadIdx.x;
-  const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(m) * K);
-  const int nv = K / 8;
-  float mx = 0.f;
-  for (int v = tid; v < nv; v += 128) {
-    const uint4 q = __ldg(src + v);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if ((tid & 31) == 0) red[tid >> 5] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int s = scale_shift(mx, 9);
-  const float f = exp2i(-s);
-  if (tid == 0) shift[m] = s;
-  uint4* dst = reinterpret_cast<uint4*>(out + static_cast<int64_t>(m) * K);
-  for (int v = tid; v < nv; v += 128) {
-    const uint4 q = __ldg(src + v);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o[i] = half2_bits(__fmul_rn(__uint_as_float(w[i] << 16), f), __fmul_rn(__uint_as_float(w[i] & 0xFFFF0000u), f));
-    dst[v] = make_uint4(o[0], o[1], o[2], o[3]);
-  }
+  pdl_wait();
 }
 
 // ------------------------------------------------------------------ GEMM
@@ -163,7 +176,8 @@ struct DenseParams {
   alignas(64) CUtensorMap xmap;  // [M][K] fp16, box NT rows x 64 k
   const int* wshift;             // [N] or nullptr (0)
   const int* xshift;             // [M]
-  float* y;
+  float* y;                      // share of K z at y + z * M * ldy
+  int64_t ldy;
   int N, K, M;
   int* status;
 };
@@ -191,7 +205,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, int x
       : "memory");
 }
 
-// One 128 x NT tile of (weight rows, token rows) a CTA. Copy warp: a stage is one TMA box of each operand.
+// One 128 x NT tile of (weight rows, token rows) and share of K a CTA. Copy warp: a stage is one TMA box of each operand.
 // MMA warp: four K = 16 steps a stage, one thread; a commit releases the stage. Epilogue: TMEM lane =
 // weight row, so a warp's store is 32 neighbouring results of a token. Every wait is bounded: on expiry the
 // status word is set, the roles leave, copies and MMAs in flight are waited for (bounded), TMEM is freed.
@@ -219,7 +233,10 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   pdl_wait();
-  const int steps = p.K / 64;
+  pdl_launch_dependents();
+  const int all = p.K / 64;
+  const int k0 = static_cast<int>(static_cast<int64_t>(all) * blockIdx.z / gridDim.z);
+  const int steps = static_cast<int>(static_cast<int64_t>(all) * (blockIdx.z + 1) / gridDim.z) - k0;
   volatile int* abort = &bars.abort;
   if (warp == 8) {
     if (lane == 0) {
@@ -231,8 +248,8 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           break;
         }
         mbar_arrive_expect_tx(&bars.full[s], C::STAGE);
-        tma_load_2d(base + s * C::STAGE, &p.wmap, 64 * i, n0, &bars.full[s]);
-        tma_load_2d(base + s * C::STAGE + C::A, &p.xmap, 64 * i, m0, &bars.full[s]);
+        tma_load_2d(base + s * C::STAGE, &p.wmap, 64 * (k0 + i), n0, &bars.full[s]);
+        tma_load_2d(base + s * C::STAGE + C::A, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
       }
       if (*abort)  // no copy may land after the CTA has ended
         for (int i = max(0, issued - C::S); i < issued; ++i)
@@ -270,17 +287,16 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
         float v[16];
         tmem_ld16(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0, v);
         if (n < p.N) {
-          float* dst = p.y + static_cast<int64_t>(m0 + c0) * p.N + n;
+          float* dst = p.y + (static_cast<int64_t>(blockIdx.z) * p.M + m0 + c0) * p.ldy + n;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c0 + j < cols) dst[static_cast<int64_t>(j) * p.N] = __fmul_rn(__fmul_rn(v[j], exp2i(xs[c0 + j])), exp2i(ws));
+            if (c0 + j < cols) dst[j * p.ldy] = __fmul_rn(__fmul_rn(v[j], exp2i(xs[c0 + j])), exp2i(ws));
         }
       }
     }
     tc_fence_before();
   }
   __syncthreads();
-  pdl_launch_dependents();
   if (warp == 9) {
     mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL, 200000000LL);  // the MMAs in flight (after an abort too)
     tc_fence_after();
@@ -305,52 +321,76 @@ static int rows_map(CUtensorMap* map, const void* base, int rows, int K, int box
 }
 
 template <int NT>
-static int dense_launch(DenseParams& p, cudaStream_t s) {
+static int dense_launch(DenseParams& p, int parts, cudaStream_t s) {
   const void* kern = reinterpret_cast<const void*>(aipu_dense_gemm_kernel<NT>);
   static bool attr[64] = {false};
   const int rc = set_smem_attr_once(kern, DenseCfg<NT>::TOTAL, attr, "cudaFuncSetAttribute(dense)");
   if (rc) return rc;
-  return launch_kernel(kern, dim3((p.N + 127) / 128, (p.M + NT - 1) / NT), dim3(kDenseThreads), DenseCfg<NT>::TOTAL, s, true, &p);
+  return launch_kernel(kern, dim3((p.N + 127) / 128, (p.M + NT - 1) / NT, parts), dim3(kDenseThreads), DenseCfg<NT>::TOTAL, s, true, &p);
 }
 
-int dense_gemm(int wt, const uint8_t* w, int N, int K, const uint16_t* x, int M, float* y32, void* scratch, int* status,
-               cudaStream_t s) {
+static int token_tile(int64_t M) { return M <= 64 ? 64 : M <= 128 ? 128 : 256; }
+
+int dense_parts(int64_t N, int64_t K, int64_t M) {
+  // as many shares of K (of four steps at least) as still leave a CTA an SM (148)
+  const int64_t tiles = ((N + 127) / 128) * ((M + token_tile(M) - 1) / token_tile(M));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / 256), 148 / tiles)));
+}
+
+template <int WT>
+static int operands_launch(const uint8_t* w, int N, int K, uint16_t* w16, int* wshift, const uint16_t* x, int M, uint16_t* x16,
+                           int* xshift, cudaStream_t s, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((WT == WT_F16 ? 0 : (N + 1) / 2) + (M + 1) / 2);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return set_cuda_error(cudaLaunchKernelEx(&cfg, aipu_dense_operands_kernel<WT>, w, N, K, row_bytes_of(WT, K), w16, wshift, x, M,
+                                           x16, xshift),
+                        "aipu_dense_operands_kernel");
+}
+
+int dense_gemm(int wt, const uint8_t* w, int N, int K, const uint16_t* x, int M, float* y32, int64_t ldy, void* scratch,
+               int* status, cudaStream_t s, bool pdl) {
   if (K % 256 || K <= 0 || N <= 0 || M <= 0) return set_error(EINVAL_, "dense: K must be a multiple of 256");
   uint8_t* b = static_cast<uint8_t*>(scratch);
-  DenseParams p = {};
-  const void* w16 = w;
+  uint16_t* w16 = nullptr;
+  int* wshift = nullptr;
   if (wt != WT_F16) {
-    uint16_t* out = reinterpret_cast<uint16_t*>(b);
+    w16 = reinterpret_cast<uint16_t*>(b);
     b += al1k(static_cast<size_t>(2) * N * K);
-    int* shift = reinterpret_cast<int*>(b);
+    wshift = reinterpret_cast<int*>(b);
     b += al1k(4 * static_cast<size_t>(N));
-    const int64_t rb = row_bytes_of(wt, K);
-    const int grid = (N + 7) / 8;
-    if (wt == WT_Q4K) aipu_dense_weights_kernel<WT_Q4K><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
-    else if (wt == WT_Q6K) aipu_dense_weights_kernel<WT_Q6K><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
-    else aipu_dense_weights_kernel<WT_Q80><<<grid, 256, 0, s>>>(w, N, K, rb, out, shift);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return set_cuda_error(e, "aipu_dense_weights_kernel");
-    w16 = out;
-    p.wshift = shift;
   }
   uint16_t* x16 = reinterpret_cast<uint16_t*>(b);
   b += al1k(static_cast<size_t>(2) * M * K);
   int* xshift = reinterpret_cast<int*>(b);
-  aipu_dense_tokens_kernel<<<M, 128, 0, s>>>(x, K, x16, xshift);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error(e, "aipu_dense_tokens_kernel");
-  const int nt = M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  int rc = rows_map(&p.wmap, w16, N, K, 128);
+  int rc;
+  switch (wt) {
+    case WT_Q4K: rc = operands_launch<WT_Q4K>(w, N, K, w16, wshift, x, M, x16, xshift, s, pdl); break;
+    case WT_Q6K: rc = operands_launch<WT_Q6K>(w, N, K, w16, wshift, x, M, x16, xshift, s, pdl); break;
+    case WT_Q80: rc = operands_launch<WT_Q80>(w, N, K, w16, wshift, x, M, x16, xshift, s, pdl); break;
+    default: rc = operands_launch<WT_F16>(w, N, K, w16, wshift, x, M, x16, xshift, s, pdl);
+  }
+  if (rc) return rc;
+  const int nt = token_tile(M), parts = dense_parts(N, K, M);
+  DenseParams p = {};
+  rc = rows_map(&p.wmap, wt == WT_F16 ? static_cast<const void*>(w) : w16, N, K, 128);
   if (!rc) rc = rows_map(&p.xmap, x16, M, K, nt);
   if (rc) return rc;
+  p.wshift = wshift;
   p.xshift = xshift;
   p.y = y32;
+  p.ldy = ldy;
   p.N = N;
   p.K = K;
   p.M = M;
   p.status = status;
-  return nt == 64 ? dense_launch<64>(p, s) : nt == 128 ? dense_launch<128>(p, s) : dense_launch<256>(p, s);
+  return nt == 64 ? dense_launch<64>(p, parts, s) : nt == 128 ? dense_launch<128>(p, parts, s) : dense_launch<256>(p, parts, s);
 }
 
 }  // namespace aipu

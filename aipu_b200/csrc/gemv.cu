@@ -719,14 +719,13 @@ __device__ void gemv_epilogue(const GemvParams& p, const int* misc, int grp, int
   if (EPI == EPI_STORE) {
     const int n0 = lt * 16 + g, n1 = n0 + 8;
     if (XT == XT_BF16 && p.y32) {
-      float* y32 = p.y32 + static_cast<int64_t>(grp) * p.y_group_stride;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = 2 * t + h;
         if (c < p.M) {
           const float s = exp2i(misc[c]);
-          if (n0 < p.N) y32[static_cast<int64_t>(c) * p.N + n0] = __fmul_rn(v[h], s);
-          if (n1 < p.N) y32[static_cast<int64_t>(c) * p.N + n1] = __fmul_rn(v[2 + h], s);
+          if (n0 < p.N) p.y32[c * p.y32_ld + n0] = __fmul_rn(v[h], s);
+          if (n1 < p.N) p.y32[c * p.y32_ld + n1] = __fmul_rn(v[2 + h], s);
         }
       }
     } else if (XT == XT_BF16) {

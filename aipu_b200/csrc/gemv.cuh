@@ -55,7 +55,8 @@ struct GemvParams {
   int64_t x_group_stride;    // elements
   int M;                     // tokens (<= 8 bf16, <= 4 fp32)
   uint16_t* y;               // bf16 out [M, N] per group (EPI_SWIGLU: h [M, N])
-  float* y32;                // EPI_STORE, bf16 x: fp32 out instead of y (nullable)
+  float* y32;                // EPI_STORE, bf16 x: fp32 out instead of y (nullable), one group
+  int64_t y32_ld;            // elements between its rows
   int64_t y_group_stride;    // elements
   float* partials;           // stream-K workspace [grid][2][32][4]
   int* counters;             // stream-K arrival counters, one per tile, zero between launches

@@ -123,7 +123,6 @@ struct TcParams {
   const int4* tiles;       // per tile (segment, first position, tokens, 0) (nullable: dense tiles over M)
   const int* tile_count;   // device number of tiles
   uint16_t* y;             // bf16 [positions, N]
-  float* y32;              // fp32 out instead of y (nullable; not with swiglu)
   int* status;
   alignas(64) CUtensorMap wmap[2];
   alignas(64) CUtensorMap smap[2];

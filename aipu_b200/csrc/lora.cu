@@ -192,6 +192,16 @@ struct YTile {
                                                           (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2));
 #pragma unroll
         for (int i = 0; i < (Y32 ? 2 : 1); ++i) v[j][e][i] = src[i];
+        if (Y32)
+          for (int s = 1; s < p.yparts; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float4 o = reinterpret_cast<const float4*>(static_cast<const float*>(p.y) +
+                                                               (static_cast<int64_t>(s) * p.M + tok[m]) * p.ldy + n)[i];
+              float4 a = *reinterpret_cast<float4*>(&v[j][e][i]);
+              a = make_float4(__fadd_rn(a.x, o.x), __fadd_rn(a.y, o.y), __fadd_rn(a.z, o.z), __fadd_rn(a.w, o.w));
+              v[j][e][i] = *reinterpret_cast<uint4*>(&a);
+            }
       }
   }
 };
@@ -224,26 +234,39 @@ __device__ __forceinline__ void store_rows(const LoraParams& p, const int* tok, 
                               : __uint_as_float((i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
           d[i] = __fadd_rn(y, d[i]);
         }
-        if (Y32 && p.out_f32) {
-          float4* op = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + n);
-          op[0] = make_float4(d[0], d[1], d[2], d[3]);
-          op[1] = make_float4(d[4], d[5], d[6], d[7]);
-        } else {
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + n) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (i >= cols) break;
-          const float y = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
-                              : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
-          const float v = __fadd_rn(y, d[i]);
-          if (Y32 && p.out_f32) static_cast<float*>(p.out)[row * p.ldo + n + i] = v;
-          else static_cast<uint16_t*>(p.out)[row * p.ldo + n + i] = bf16_rne_bits(v);
+          float y = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
+                        : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
+          if (Y32)
+            for (int s = 1; s < p.yparts; ++s)
+              y = __fadd_rn(y, static_cast<const float*>(p.y)[(static_cast<int64_t>(s) * p.M + row) * p.ldy + n + i]);
+          d[i] = __fadd_rn(y, d[i]);
+        }
+      }
+      if (Y32 && p.out_f32) {
+        float* op = static_cast<float*>(p.out) + row * p.ldo + n;
+        if (p.vo && cols == 8) {
+          reinterpret_cast<float4*>(op)[0] = make_float4(d[0], d[1], d[2], d[3]);
+          reinterpret_cast<float4*>(op)[1] = make_float4(d[4], d[5], d[6], d[7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < cols) op[i] = d[i];
+        }
+      } else {
+        uint16_t* op = static_cast<uint16_t*>(p.out) + row * p.ldo + n;
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
+        if (p.vo && cols == 8) {
+          *reinterpret_cast<uint4*>(op) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < cols) op[i] = static_cast<uint16_t>(o[i >> 1] >> (16 * (i & 1)));
         }
       }
     }
@@ -682,9 +705,20 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
       constexpr int per = C::COLS * (Y32 ? 4 : 2) / 16, each = Y32 ? 4 : 8;
       for (int i = tid; i < tl.rows * per; i += kLoraThreads) {
         const int m = i / per, n = col0 + (i % per) * each;
-        if (n + each <= p.N)
-          cp_async16(smem_u32(smem) + m * C::YPITCH + (i % per) * 16,
-                     static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2), 16);
+        if (n + each > p.N) continue;
+        uint8_t* dst = smem + m * C::YPITCH + (i % per) * 16;
+        const uint8_t* src = static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2);
+        if (Y32 && p.yparts > 1) {
+          float4 v = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+          for (int s = 1; s < p.yparts; ++s) {
+            const float4 o = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * p.M * p.ldy * 4);
+            v = make_float4(__fadd_rn(v.x, o.x), __fadd_rn(v.y, o.y), __fadd_rn(v.z, o.z), __fadd_rn(v.w, o.w));
+          }
+          *reinterpret_cast<float4*>(dst) = v;
+        } else {
+          cp_async16(smem_u32(dst), src, 16);
+        }
       }
     }
     cp_commit();
@@ -951,7 +985,8 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   auto rows16 = [](const void* q, int64_t ld, int esz) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * esz % 16 == 0;
   };
-  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2) && rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
+  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2);
+  p.vo = rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
   p.tiles = nullptr;
   if (p.M <= kDirectRows) return OK;
   uint8_t* b = static_cast<uint8_t*>(plan);

@@ -22,6 +22,7 @@ struct LoraParams {
   void* out;             // bf16, or fp32 when y is
   int64_t ldo;
   int y_f32, out_f32;
+  int yparts;            // shares of fp32 y to be summed, M * ldy elements apart (0: one)
   int* status;           // device status word (nullable)
   int wait_y;            // 1: y comes from the kernel launched just before lora_finish's (programmatic launch)
   // set by lora_begin
@@ -33,7 +34,7 @@ struct LoraParams {
   int rp;                // padded rank: 16, 32, 64 or 128
   int skip_plain;        // 1: in-place, rows without an adapter are not touched
   int wa, wx, wb;        // widest aligned load of A rows, x rows, B rows (elements: 8, 2 or 1)
-  int vy;                // 1: 16-byte loads and stores of y and out
+  int vy, vo;            // 1: 16-byte loads of y, stores of out
 };
 
 // bytes of the scratch of M rows (0 when the one launch takes them)

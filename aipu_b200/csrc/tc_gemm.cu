@@ -765,11 +765,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) aipu_tc_gemm_kernel(const __gri
           if (col >= it.tn) break;  // warp-uniform
           const int shn = __shfl_sync(0xffffffffu, n < 32 ? shl0 : shl1, n & 31);
           const int pos = it.t0 + col;
-          const float v = __fmul_rn(acc[n], exp2i(shn));
-          if (nrow < p.N) {
-            if (p.y32) p.y32[static_cast<int64_t>(pos) * p.N + nrow] = v;
-            else p.y[static_cast<int64_t>(pos) * p.N + nrow] = bf16_rne_bits(v);
-          }
+          if (nrow < p.N) p.y[static_cast<int64_t>(pos) * p.N + nrow] = bf16_rne_bits(__fmul_rn(acc[n], exp2i(shn)));
         }
       }
       tw[1] += clock64() - t_out;
@@ -816,7 +812,7 @@ static int tc_encode(CUtensorMap* map, int wt, const uint8_t* base, int64_t row_
 int tc_gemm_launch(TcParams& p, int nt, int n_experts, int max_tiles, int num_sms, cudaStream_t s, bool pdl) {
   if (nt != 64 && nt != 128) return set_error(EINVAL_, "tc_gemm: tile width must be 64 or 128");
   if (p.K % 256 || p.K <= 0 || p.N <= 0 || (p.wt != WT_Q4K && p.wt != WT_Q6K) || (p.swiglu && p.wt != WT_Q4K) ||
-      !p.w[0] || (p.swiglu && !p.w[1]) || !p.xt || !p.xshift || (!p.y && (p.swiglu || !p.y32)))
+      !p.w[0] || (p.swiglu && !p.w[1]) || !p.xt || !p.xshift || !p.y)
     return set_error(EINVAL_, "tc_gemm: needs Q4_K or Q6_K weights, K % 256 == 0 (SwiGLU: Q4_K)");
   if (max_tiles <= 0) return OK;
   const bool has_shared = p.shared_id >= 0;
