@@ -8,8 +8,8 @@
 // before the tensor pipe; mma.sync, whose fragments come straight from global memory, feeds it without
 // a trip through shared memory or TMEM.
 //
-// Up to kDirectRows rows: ONE launch. A cluster of CTAs takes a tile of up to 8 rows that share an adapter
-// (found by two ballots over the ids).
+// Few rows (lora_direct): ONE launch. A cluster of CTAs takes a tile of up to 8 rows that share an adapter
+// (found by comparing the ids).
 //   1. CTA c and its 8 warps each take a share of K. Rank rows are the 16 MMA rows, token rows the 8
 //      MMA columns; a lane loads 8 consecutive k of its rows (16 bytes) and uses them as two MMA steps
 //      whose k order is permuted the same way on both sides.
@@ -18,6 +18,7 @@
 //   3. CTA c and its warps each take 64-column blocks of N. The MMA's rows are columns of y, ordered so
 //      that a lane ends with 8 consecutive columns of a row: y is read and written 16 bytes at a time.
 //   h never leaves the chip, and the reads of B and y do not wait for the sums of A.
+//   (4096 x 4096, device time in a graph: 1 row of rank 16 7.6 us, 128 rows on eight adapters 9.1 us.)
 // More rows: a plan (rows ordered by adapter, tiles of up to 64 of them), the first product (a tile and a
 // share of K a CTA: x and A stream through a ring of asynchronous copies in shared memory, partial sums to
 // global memory), the second product (a tile and a share of N a CTA: step 3 above). As one cluster kernel
@@ -38,7 +39,7 @@ namespace aipu {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kDirectRows = 64;      // rows of the one-launch kernel
+constexpr int kDirectRows = 256;     // rows of the one-launch kernel (a thread each) at most
 constexpr int kDirectCtas = 8;       // CTAs of its clusters
 constexpr int kMaxAdapters = 32768;  // counters of the plan kernel in shared memory
 
@@ -109,6 +110,7 @@ __device__ __forceinline__ void split4_f16(const uint4& v, uint4& hi, uint4& lo)
 }
 
 constexpr int kDirectTile = 8;  // rows of a tile of the one-launch kernel
+static_assert(kDirectRows <= kLoraThreads, "a thread a row");
 template <int MT>
 struct LoraCfg {
   static constexpr int TM = kDirectTile;
@@ -370,56 +372,61 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
   // launch says that only y does
   if (!p.wait_y) pdl_wait();
 
-  // a row leads a tile if the number of earlier rows with its id is a multiple of a tile's rows; the tile is
-  // that row and the following ones of the id, and this cluster's is the one of the cluster's number
+  // A row leads a tile if the number of earlier rows with its id is a multiple of a tile's rows; the tile is
+  // that row and the following ones of the id, and this cluster's is the one of the cluster's number.
   __shared__ int key[kDirectRows];
-  for (int i = tid; i < p.M; i += kLoraThreads) {
-    const int v = p.ids[i];
+  __shared__ uint32_t lead_bits[kDirectRows / 32];
+  int mine = -2, prior = 0;  // this thread's row: its id and the earlier rows with it
+  if (tid < p.M) {
+    const int v = p.ids[tid];
     if (v >= p.L && blockIdx.x == 0 && p.status) atomicOr(p.status, ST_BAD_ARGS);
-    key[i] = (v < 0 || v >= p.L) ? -1 : v;
+    mine = (v < 0 || v >= p.L) ? -1 : v;
   }
+  key[tid] = mine;
   __syncthreads();
-  const int k0 = lane < p.M ? key[lane] : -2, k1 = lane + 32 < p.M ? key[lane + 32] : -2;
-  // earlier rows with the ids of rows `lane` and `lane + 32`
-  const uint32_t lower = (1u << lane) - 1;
-  const int same0 = __popc(__match_any_sync(0xffffffffu, k0) & lower);
-  int same1 = __popc(__match_any_sync(0xffffffffu, k1) & lower);
-  if (p.M > 32)
-    for (int i = 0; i < 32; ++i) same1 += __shfl_sync(0xffffffffu, k0, i) == k1;
-  const bool any0 = k0 >= 0 || (k0 == -1 && !p.skip_plain), any1 = k1 >= 0 || (k1 == -1 && !p.skip_plain);
-  const uint32_t l0 = __ballot_sync(0xffffffffu, any0 && same0 % C::TM == 0);
-  const uint32_t l1 = __ballot_sync(0xffffffffu, any1 && same1 % C::TM == 0);
-  uint64_t leaders = static_cast<uint64_t>(l1) << 32 | l0;
-  for (int i = blockIdx.x / csize; i > 0 && leaders; --i) leaders &= leaders - 1;
-  if (!leaders) {  // (the same for every thread of the cluster)
+  if (32 * warp < p.M) {
+    prior = __popc(__match_any_sync(0xffffffffu, mine) & ((1u << lane) - 1));
+    for (int i = 0; i < 32 * warp; i += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(key + i);
+      prior += (k.x == mine) + (k.y == mine) + (k.z == mine) + (k.w == mine);
+    }
+  }
+  const uint32_t bits = __ballot_sync(0xffffffffu, (mine >= 0 || (mine == -1 && !p.skip_plain)) && prior % C::TM == 0);
+  if (lane == 0) lead_bits[warp] = bits;
+  __syncthreads();
+  int lead = -1;
+  for (int i = 0, skip = blockIdx.x / csize; i < kDirectRows / 32 && lead < 0; ++i) {
+    uint32_t word = lead_bits[i];
+    const int n = __popc(word);
+    if (skip >= n) {
+      skip -= n;
+      continue;
+    }
+    for (; skip > 0; --skip) word &= word - 1;
+    lead = 32 * i + __ffs(word) - 1;
+  }
+  if (lead < 0) {  // (the same for every thread of the cluster)
     pdl_launch_dependents();
     if (p.wait_y) pdl_wait();  // a cluster without a tile may not end before what it depends on
     return;
   }
-  const int lead = __ffsll(static_cast<long long>(leaders)) - 1;
   const int id = key[lead];
-  const LoraTile own = lora_tile(p, id, 0);
-  const uint32_t b0 = __ballot_sync(0xffffffffu, k0 == id), b1 = __ballot_sync(0xffffffffu, k1 == id);
-  const uint64_t all = static_cast<uint64_t>(b1) << 32 | b0;
-  const uint64_t below = (1ull << lead) - 1;
-  const uint64_t rest = all & ~below;
-  LoraTile tl = own;
-  tl.rows = min(C::TM, __popcll(rest));
-  if (warp == 0) {
-    if (lane < C::TM) tok[lane] = 0;
-    __syncwarp();
-    for (int h = 0; h < 2; ++h) {
-      const int row = lane + 32 * h;
-      if ((rest >> row) & 1) {
-        const int at = __popcll(rest & ((1ull << row) - 1));
-        if (at < C::TM) tok[at] = row;
-      }
-    }
+  LoraTile tl = lora_tile(p, id, 0);
+  __shared__ int lead_prior, count;
+  if (tid < C::TM) tok[tid] = 0;
+  if (tid == lead) lead_prior = prior;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  const int place = prior - lead_prior;
+  if (mine == id && place >= 0 && place < C::TM) {
+    tok[place] = tid;
+    atomicAdd(&count, 1);
   }
   if (C::RF > C::RP)  // rank columns that the second product reads and the first does not give
     for (int i = tid; i < 3 * C::TM * (C::HPITCH - C::RP); i += kLoraThreads)
       hf[(i / (C::HPITCH - C::RP)) * C::HPITCH + C::RP + i % (C::HPITCH - C::RP)] = 0;
   __syncthreads();
+  tl.rows = count;
 
   const int nblk = (p.N + 63) / 64;
   const int gw = crank * kLoraWarps + warp, nw = csize * kLoraWarps;
@@ -892,8 +899,17 @@ static int k_split(int64_t M, int64_t L) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 296 / tiles)));
 }
 
+// The one launch: up to 256 rows, whose adapters it reads once for every 8 rows. 4096 x 4096, rank 16 / 64, eight
+// adapters: 128 rows 9.1 / 12.6 us against 10.4 / 14.2 us with the plan, one adapter 9.0 / 12.4 against 17.1 / 35.1
+// (the tiles are few), 256 rows on 64 adapters 23 / 30 against 24 / 30. Ranks above 64 leave one CTA an SM: as long as
+// all tiles fit at once (64 rows on eight adapters of rank 128 17 us; 96 rows 32 against 21.5 with the plan, 64 rows on
+// 64 adapters 113 against 58). 16 rows or fewer always go this way.
+static bool lora_direct(int64_t M, int64_t L, int64_t R) {
+  return M <= kDirectRows && (R <= 64 || M / kDirectTile + std::min<int64_t>(L + 1, M) <= 148 / kDirectCtas);
+}
+
 size_t lora_plan_bytes(int64_t M, int64_t L, int64_t R) {
-  if (M <= kDirectRows) return 0;
+  if (lora_direct(M, L, R)) return 0;
   return 256 + al256l(4 * M) + al256l(16 * max_tiles(M, L)) +
          al256l(static_cast<size_t>(4) * M * padded_rank(R) * k_split(M, L));
 }
@@ -988,7 +1004,7 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2);
   p.vo = rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
   p.tiles = nullptr;
-  if (p.M <= kDirectRows) return OK;
+  if (lora_direct(p.M, p.L, p.R)) return OK;
   uint8_t* b = static_cast<uint8_t*>(plan);
   p.n_tiles = reinterpret_cast<int32_t*>(b);
   p.perm = reinterpret_cast<int32_t*>(b + 256);

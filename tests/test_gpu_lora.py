@@ -71,8 +71,9 @@ def _check(out, y64, d, s, K, extra=0.0):
 
 @pytest.mark.parametrize("M,K,N,R,L", [
     (1, 4096, 4096, 16, 4), (1, 8, 8, 1, 1), (3, 256, 64, 8, 2), (8, 512, 520, 32, 1), (9, 1024, 192, 64, 1),
-    (64, 640, 256, 16, 64), (64, 2048, 512, 128, 3), (65, 512, 256, 16, 2), (200, 768, 320, 64, 3),
-    (300, 512, 192, 128, 2), (1000, 256, 1024, 32, 5), (700, 256, 128, 16, 200), (130, 384, 264, 24, 1)])
+    (64, 640, 256, 16, 64), (64, 2048, 512, 128, 3), (65, 512, 256, 16, 2), (200, 768, 320, 64, 3), (256, 256, 96, 16, 9),
+    (257, 256, 96, 16, 9), (257, 4160, 576, 32, 1), (300, 512, 192, 128, 2), (40, 512, 192, 128, 40), (1000, 256, 1024, 32, 5),
+    (700, 256, 128, 16, 200), (130, 384, 264, 24, 1), (640, 192, 72, 64, 3)])
 @pytest.mark.parametrize("ad", [BF, HF])
 def test_add_matches_the_definition(M, K, N, R, L, ad):
     A, ids, x = _case(M, K, N, R, L, ad, ranks=R > 8)
@@ -87,7 +88,7 @@ def test_add_matches_the_definition(M, K, N, R, L, ad):
 
 
 @pytest.mark.parametrize("M,K,N,R", [(1, 1, 1, 1), (5, 13, 7, 3), (77, 1001, 2051, 13), (12, 100, 33, 5), (90, 34, 70, 127),
-                                     (66, 999, 9, 128)])
+                                     (66, 999, 9, 128), (300, 34, 70, 127), (301, 999, 9, 128), (277, 1001, 515, 13), (400, 1, 1, 1)])
 @pytest.mark.parametrize("ad", [BF, HF])
 def test_odd_sizes(M, K, N, R, ad):
     A, ids, x = _case(M, K, N, R, 3, ad, ranks=True)
@@ -97,7 +98,7 @@ def test_odd_sizes(M, K, N, R, ad):
     _check(ops.lora_add(A, ids, x, y.to(BF)), y.to(BF).double().cpu(), d, s, K)
 
 
-@pytest.mark.parametrize("M", [6, 150])
+@pytest.mark.parametrize("M", [6, 150, 300])
 def test_columns_of_wider_tensors_and_in_place(M):
     """Queries and values of a fused projection: columns of one tensor, added to in place; what lies beside stays."""
     A, ids, x = _case(M, 256, 72, 16, 3)
@@ -115,7 +116,7 @@ def test_columns_of_wider_tensors_and_in_place(M):
     assert torch.equal(wide[:, 144 + 29:], before[:, 144 + 29:])
 
 
-@pytest.mark.parametrize("M", [1, 40, 64, 65, 500])
+@pytest.mark.parametrize("M", [1, 40, 64, 65, 256, 500])
 def test_rows_without_an_adapter(M):
     """Left as they are to the bit, signs of zero and NaN among them; all rows, or all but one."""
     A, _, x = _case(M, 128, 96, 8, 2)
@@ -133,7 +134,7 @@ def test_rows_without_an_adapter(M):
 
 
 def test_an_id_out_of_range_is_no_adapter_and_sets_the_status():
-    for M in (5, 80):
+    for M in (5, 80, 300):
         A, _, x = _case(M, 128, 64, 8, 2)
         ctx = ops.Context(x.device)
         y = torch.randn((M, 64), device=x.device).to(BF)
@@ -148,7 +149,7 @@ def test_an_id_out_of_range_is_no_adapter_and_sets_the_status():
         ctx.close()
 
 
-@pytest.mark.parametrize("M", [4, 100])
+@pytest.mark.parametrize("M", [4, 100, 300])
 def test_nothing_is_read_past_a_rank(M):
     """NaN in the rows of a and columns of b past an adapter's rank, rank 0, and ranks outside 0..R."""
     A, ids, x = _case(M, 96, 80, 24, 5, ids=[m % 5 for m in range(M)])
@@ -165,7 +166,7 @@ def test_nothing_is_read_past_a_rank(M):
 
 
 def test_infinities_and_nan_stay_in_their_row():
-    for M in (6, 70):
+    for M in (6, 70, 270):
         A, ids, x = _case(M, 128, 64, 16, 1, ids=[0] * M)
         y = torch.zeros((M, 64), device=x.device)
         clean = ops.lora_add(A, ids, x, y)
@@ -186,6 +187,15 @@ def test_equal_calls_give_equal_bits_whatever_shares_the_batch():
     o = ops.lora_add(A, ids, x, y)
     for _ in range(5):
         assert torch.equal(ops.lora_add(A, ids, x, y), o)
+
+
+def test_up_to_16_rows_do_not_depend_on_what_shares_the_call():
+    for R in (16, 100):
+        A, ids, x = _case(16, 512, 300, R, 9)
+        y = torch.randn((16, 300), device=x.device)
+        o = ops.lora_add(A, ids, x, y)
+        for m in range(16):
+            assert torch.equal(ops.lora_add(A, ids[m:m + 1], x[m:m + 1], y[m:m + 1]), o[m:m + 1])
 
 
 def test_no_rows():
@@ -265,7 +275,7 @@ def test_gemm_lora_many_rows_at_tile_borders(wt, M, K, N):
     _check(o, x64 @ wd.t(), torch.zeros_like(mag), torch.zeros_like(mag), K, extra)
 
 
-@pytest.mark.parametrize("M", [3, 90])
+@pytest.mark.parametrize("M", [3, 90, 290])
 def test_captured_and_replayed_with_new_inputs(M):
     A, ids, x = _case(M, 512, 96, 16, 3)
     w = torch.from_numpy(F.random_rows_np(F.Q4_K, 96, 512, seed=1)).to(x.device)

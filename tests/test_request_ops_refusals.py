@@ -100,7 +100,7 @@ def test_c_entry_refuses_adapters(kw, M):
     assert b"bad adapters" in L.aipu_last_error()
 
 
-def _add(M=100, x=16, ldx=256, y=16, ydt=1, ldy=32, out=32, odt=1, ldo=32, ws=16, n=1 << 30):
+def _add(M=300, x=16, ldx=256, y=16, ydt=1, ldy=32, out=32, odt=1, ldo=32, ws=16, n=1 << 30):
     return _lib.lib().aipu_lora_add(None, _lora(), 16, x, ldx, M, y, ydt, ldy, out, odt, ldo, ws, n, None)
 
 
@@ -130,11 +130,11 @@ def test_c_entry_refuses_a_projection(kw, text):
 
 def test_workspace_sizes():
     L = _lib.lib()
-    assert L.aipu_lora_workspace(64, 8, 16) == 0
-    for bad in ((-1, 8, 16), (65, 0, 16), (65, 32769, 16), (65, 8, 0), (65, 8, 129)):
+    assert L.aipu_lora_workspace(256, 8, 64) == 0 and L.aipu_lora_workspace(16, 32768, 128) == 0
+    for bad in ((-1, 8, 16), (257, 0, 16), (257, 32769, 16), (257, 8, 0), (257, 8, 129)):
         assert L.aipu_lora_workspace(*bad) == 0
     # an int per row, tiles of every adapter, and the fp32 sums of 16 ranks at least
-    assert L.aipu_lora_workspace(65, 8, 3) >= 4 * 65 + 16 * 9 + 4 * 65 * 16
+    assert L.aipu_lora_workspace(257, 8, 3) >= 4 * 257 + 16 * 9 + 4 * 257 * 16
     assert L.aipu_q4k_gemm_lora_workspace(0, 32, 256, 3, 2, 8) >= 4 * 3 * 32
     assert L.aipu_q4k_gemm_lora_workspace(0, 32, 100, 3, 2, 8) == 0
 
