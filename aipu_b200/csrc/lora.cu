@@ -52,28 +52,35 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint3
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 8 consecutive 16-bit values at p (only `valid` of them are read, the others are 0), as four packed
-// words. w: widest load that the row's alignment allows (8, 2 or 1 elements).
+// 8 consecutive 16-bit values at p, of which `valid` (from the first) are wanted and the others come as 0. VEC: p is
+// 16-byte aligned and valid is 0 or 8. Else from the one or two aligned 16-byte pieces that hold wanted values
+// (the tensors are readable to such boundaries), moved into place by selects and a funnel shift: an eighth of
+// the loads that one value at a time would take (rank 71, 2555 rows: MEASURED1).
 template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int valid, int w) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (VEC) {
-    if (valid >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
-  }
-  if (valid <= 0) return v;
-  uint32_t h[4] = {0, 0, 0, 0};
-  if (w >= 2) {
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int valid) {
+  if (valid <= 0) return make_uint4(0, 0, 0, 0);
+  if (VEC) return __ldg(reinterpret_cast<const uint4*>(p));
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const uint4* base = reinterpret_cast<const uint4*>(a & ~static_cast<uintptr_t>(15));
+  const int off = static_cast<int>(a & 15u);  // even
+  const uint4 u = __ldg(base);
+  const uint4 v = off + 2 * min(valid, 8) > 16 ? __ldg(base + 1) : make_uint4(0, 0, 0, 0);
+  const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  uint32_t s8[6], s4[5], o[4];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) s8[i] = (off & 8) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) s4[i] = (off & 4) ? s8[i + 1] : s8[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = (off & 2) ? __funnelshift_r(s4[i], s4[i + 1], 16) : s4[i];
+  if (valid < 8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (2 * i + 1 < valid) h[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-      else if (2 * i < valid) h[i] = __ldg(p + 2 * i);
+      if (2 * i >= valid) o[i] = 0;
+      else if (2 * i + 1 >= valid) o[i] &= 0xFFFFu;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < valid) h[i >> 1] |= static_cast<uint32_t>(__ldg(p + i)) << (16 * (i & 1));
   }
-  return make_uint4(h[0], h[1], h[2], h[3]);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // Two floats as packed bf16 pieces: hi truncated (never overflows), lo = the exact rest rounded or
@@ -91,10 +98,13 @@ __device__ __forceinline__ uint32_t piece(float v, float& rest) {
 }
 // packed pair of fp16 -> packed bf16 hi and lo (exact: 11 bits)
 __device__ __forceinline__ void split_f16(uint32_t w, uint32_t& hi, uint32_t& lo) {
-  float r0, r1;
-  const uint32_t h0 = piece(f16_bits_to_f32(w), r0), h1 = piece(f16_bits_to_f32(w >> 16), r1);
-  hi = h0 | (h1 << 16);
-  lo = (__float_as_uint(r0) >> 16) | (__float_as_uint(r1) & 0xFFFF0000u);
+  const float a = f16_bits_to_f32(w), b = f16_bits_to_f32(w >> 16);
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  hi = prmt(ua, ub, 0x7632u);
+  float ra = __fsub_rn(a, __uint_as_float(ua & 0xFFFF0000u)), rb = __fsub_rn(b, __uint_as_float(ub & 0xFFFF0000u));
+  if (not_finite(a)) ra = 0.f;
+  if (not_finite(b)) rb = 0.f;
+  lo = prmt(__float_as_uint(ra), __float_as_uint(rb), 0x7632u);
 }
 
 // acc += (16 rank or output rows: va rows g, vb rows g + 8) x (8 columns: x), two MMA steps of 16
@@ -148,9 +158,9 @@ __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, cons
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 16 * i + 8 * h + g;
-          va[u][i][h] = load8<VEC>(abase + static_cast<int64_t>(r) * p.K + k, r < tl.rank ? valid : 0, p.wa);
+          va[u][i][h] = load8<VEC>(abase + static_cast<int64_t>(r) * p.K + k, r < tl.rank ? valid : 0);
         }
-      vx[u] = load8<VEC>(xrow + k, g < tl.rows ? valid : 0, p.wx);
+      vx[u] = load8<VEC>(xrow + k, g < tl.rows ? valid : 0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -287,29 +297,27 @@ __device__ __forceinline__ void pieces(float2 v, int ns, uint32_t (&w)[3]) {
 }
 
 // B rows n0 + 8 g + 2 j (+ 1) for j = 0..3, rank columns r .. r + 7 (past the rank: 0, whatever is stored)
-template <bool VEC>
 __device__ __forceinline__ void load_b(const LoraParams& p, const LoraTile& tl, int n0, int r, int g, uint4 (&vb)[8]) {
-  const uint16_t* bbase = static_cast<const uint16_t*>(p.b) + static_cast<int64_t>(tl.id) * p.N * p.R;
-  const int valid = tl.rank - r;
+  const uint16_t* row = static_cast<const uint16_t*>(p.b) + (static_cast<int64_t>(tl.id) * p.N + n0 + 8 * g) * p.R + r;
+  const int valid = tl.rank - r, rows = p.N - n0 - 8 * g;
+  if (p.wb == 8) {  // R is a multiple of 8: whole vectors are in the row, the columns past the rank are cleared
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = n0 + 8 * g + i;
-    const uint16_t* row = bbase + static_cast<int64_t>(n) * p.R + r;
-    if (VEC) {  // R is a multiple of 8: whole vectors are in the row, the columns past the rank are cleared
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (n < p.N && valid > 0) v = __ldg(reinterpret_cast<const uint4*>(row));
-      if (valid < 8) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+    for (int i = 0; i < 8; ++i)
+      vb[i] = (i < rows && valid > 0) ? __ldg(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i) * p.R)) : make_uint4(0, 0, 0, 0);
+    if (valid < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&vb[i]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (2 * q >= valid) w[q] = 0;
           else if (2 * q + 1 >= valid) w[q] &= 0xFFFFu;
         }
       }
-      vb[i] = v;
-    } else {
-      vb[i] = load8<false>(row, n < p.N ? valid : 0, p.wb);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vb[i] = load8<false>(row + static_cast<int64_t>(i) * p.R, i < rows ? valid : 0);
   }
 }
 
@@ -446,7 +454,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
     const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (gw + 1) / nw);
     shrink<MT, AT, VEC>(p, tok, tl, c0, c1, lane, acc);
     // the first block's B rows are on the way while the sums are joined
-    if (gw < nblk) load_b<VEC>(p, tl, gw * 64, 8 * t, g, vb);
+    if (gw < nblk) load_b(p, tl, gw * 64, 8 * t, g, vb);
     // ---- sums over the warps of the CTA, in warp order
     float* mine = red + warp * C::TM * C::PITCH;
 #pragma unroll
@@ -497,7 +505,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
       for (int i = 0; i < 4; ++i) acc[q][0][i] = -0.f;  // y + -0 is y, also for y = -0
     if (nb != gw) yt.load(p, tok, tl.rows, nb * 64, lane, 0);
     for (int rc = 0; rc < rchunks; ++rc) {
-      if (nb != gw || rc != 0) load_b<VEC>(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
+      if (nb != gw || rc != 0) load_b(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
       expand_step<1, AT>(acc, vb, hf, C::HPITCH, HS, ns, 0, tl.rows, rc, lane);
     }
     store_rows<1, Y32>(p, tok, tl.rows, nb * 64, lane, acc, yt, 0);
@@ -542,7 +550,7 @@ __device__ __forceinline__ void stage8(uint32_t dst, const uint16_t* src, int va
       cp_async4(dst + 4 * i, n > 0 ? src + 2 * i : src, n > 0 ? 4 : 0);
     }
   } else {
-    const uint4 v = load8<false>(src, valid, 1);
+    const uint4 v = load8<false>(src, valid);
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
   }
 }
@@ -684,10 +692,10 @@ struct ExpandCfg {
   static constexpr int YBYTES = kTile * YPITCH;
 };
 
-template <int AT, bool VEC, bool Y32>
+template <int AT, bool Y32>
 __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const __grid_constant__ LoraParams p) {
   using C = ExpandCfg<Y32>;
-  constexpr int NT = Y32 ? 1 : 2, HALVES = kLoraWarps / C::BLOCKS;
+  constexpr int NT = 4, HALVES = kLoraWarps / C::BLOCKS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[kTile];
   uint16_t* hf = reinterpret_cast<uint16_t*>(smem + C::YBYTES);
@@ -732,7 +740,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   };
   if (!p.wait_y) load_y();
   uint4 vb[8];
-  if (busy && rchunks > 0) load_b<VEC>(p, tl, n0, 8 * t, g, vb);
+  if (busy && rchunks > 0) load_b(p, tl, n0, 8 * t, g, vb);
   pdl_wait();
   if (p.wait_y) load_y();
   for (int e = tid; e < tl.rows * rchunks * 16; e += kLoraThreads) {
@@ -770,18 +778,25 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[q][j][i] = -0.f;  // y + -0 is y, also for y = -0
     for (int rc = 0; rc < rchunks; ++rc) {
-      if (rchunks > 1 && (gr >= HALVES || rc)) load_b<VEC>(p, tl, n0, 32 * rc + 8 * t, g, vb);
+      if (rchunks > 1 && (gr >= HALVES || rc)) load_b(p, tl, n0, 32 * rc + 8 * t, g, vb);
       expand_step<NT, AT>(acc, vb, hf, hpitch, hs, ns, nt0, tl.rows, rc, lane);
     }
-    YTile<NT, Y32> yt;
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) {
+      if (8 * (nt0 + j) >= tl.rows) break;
+      YTile<1, Y32> yt;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int i = 0; i < (Y32 ? 2 : 1); ++i)
-          yt.v[j][e][i] = reinterpret_cast<const uint4*>(ys + (8 * (nt0 + j) + 2 * t + e) * C::YPITCH)[i];
-    store_rows<NT, Y32>(p, tok, tl.rows, n0, lane, acc, yt, nt0);
+          yt.v[0][e][i] = reinterpret_cast<const uint4*>(ys + (8 * (nt0 + j) + 2 * t + e) * C::YPITCH)[i];
+      float d[4][1][4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[q][0][i] = acc[q][j][i];
+      store_rows<1, Y32>(p, tok, tl.rows, n0, lane, d, yt, nt0 + j);
+    }
   }
 }
 
@@ -968,20 +983,16 @@ static int shrink_launch_t(LoraParams& p, bool vec, cudaStream_t s) {
   return vec ? shrink_launch<MT, AD_BF16, true>(p, s) : shrink_launch<MT, AD_BF16, false>(p, s);
 }
 
-template <int AT, bool VEC, bool Y32>
+template <int AT, bool Y32>
 static int expand_launch(LoraParams& p, cudaStream_t s, bool pdl) {
   const int smem = ExpandCfg<Y32>::YBYTES + (p.out_f32 ? 3 : 2) * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
-  const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, VEC, Y32>);
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, Y32>);
   static bool attr[64] = {false};
   const int rc = set_smem_attr_once(kern, ExpandCfg<Y32>::YBYTES + 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
   if (rc) return rc;
   void* args[1] = {&p};
   return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, s, pdl, args,
                 "aipu_lora_expand_kernel");
-}
-template <int AT, bool VEC>
-static int expand_launch_t(LoraParams& p, cudaStream_t s, bool pdl) {
-  return p.y_f32 ? expand_launch<AT, VEC, true>(p, s, pdl) : expand_launch<AT, VEC, false>(p, s, pdl);
 }
 
 // widest load (elements of 16 bits) of rows `ld` elements apart from `ptr`
@@ -1030,7 +1041,7 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
 
 int lora_finish(LoraParams& p, cudaStream_t s, bool pdl) {
   if (!p.tiles) {
-    const bool vec = p.wa == 8 && p.wx == 8 && p.wb == 8;
+    const bool vec = p.wa == 8 && p.wx == 8;
     switch (p.rp) {
       case 16: return direct_launch_t<1>(p, vec, s, pdl);
       case 32: return direct_launch_t<2>(p, vec, s, pdl);
@@ -1038,9 +1049,8 @@ int lora_finish(LoraParams& p, cudaStream_t s, bool pdl) {
       default: return direct_launch_t<8>(p, vec, s, pdl);
     }
   }
-  const bool vec = p.wb == 8;
-  if (p.adtype == AD_F16) return vec ? expand_launch_t<AD_F16, true>(p, s, pdl) : expand_launch_t<AD_F16, false>(p, s, pdl);
-  return vec ? expand_launch_t<AD_BF16, true>(p, s, pdl) : expand_launch_t<AD_BF16, false>(p, s, pdl);
+  if (p.adtype == AD_F16) return p.y_f32 ? expand_launch<AD_F16, true>(p, s, pdl) : expand_launch<AD_F16, false>(p, s, pdl);
+  return p.y_f32 ? expand_launch<AD_BF16, true>(p, s, pdl) : expand_launch<AD_BF16, false>(p, s, pdl);
 }
 
 }  // namespace aipu

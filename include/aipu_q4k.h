@@ -257,7 +257,8 @@ int aipu_ep_destroy(aipu_ep* ep);
 
 /* Low-rank adapters of one projection of K inputs and N outputs: adapter l has a[l] (R rows of K),
  * b[l] (N rows of R), a factor and a rank <= R (rows of a[l] and columns of b[l] from the rank on are
- * not used, whatever they hold). All device pointers; a, b 2-byte aligned (16-byte rows are fastest). */
+ * not used, whatever they hold). All device pointers, 2-byte aligned; a, b and the x rows used with them must be
+ * readable to the 16-byte boundaries around them (rows that start on such boundaries are fastest). */
 typedef struct aipu_lora {
   int32_t dtype;        /* of a and b: AIPU_DT_BF16 or AIPU_DT_F16 */
   int32_t n_adapters;   /* 1 .. 32768 */
