@@ -186,102 +186,111 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // rounded 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// acc[q][j]: MMA q's rows g and g + 8 are columns n0 + 8 g + 2 q and + 2 q + 1 of y, its columns 2 t and
-// 2 t + 1 the rows 8 (nt0 + j) + 2 t (+ 1) of the tile. Rows of y, 8 columns a lane, loaded ahead:
-template <int NT, bool Y32>
-struct YTile {
-  uint4 v[NT][2][Y32 ? 2 : 1];
-  __device__ __forceinline__ void load(const LoraParams& p, const int* tok, int rows, int n0, int lane, int nt0) {
-    const int g = lane >> 2, t = lane & 3, n = n0 + 8 * g;
-    if (!p.vy || n + 8 > p.N) return;
+// A warp's block of y is 16 Q columns: MMA q's rows g and g + 8 are its columns 2 Q g + 2 q and + 2 q + 1, so a
+// lane holds 2 Q neighbouring columns of rows 2 t and 2 t + 1 of the 8 token columns of an MMA. Those values of y:
+template <int Q, bool Y32>
+struct YRows {
+  static constexpr int W = Q * (Y32 ? 2 : 1);  // 32-bit words a row
+  uint32_t w[2][W];
+  __device__ __forceinline__ void put(int e, const void* src) {
+    if constexpr (W == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(src);
+      w[e][0] = v.x;
+      w[e][1] = v.y;
+    } else {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int m = 8 * (nt0 + j) + 2 * t + e;
-        if (m >= rows) continue;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.y) +
-                                                          (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2));
-#pragma unroll
-        for (int i = 0; i < (Y32 ? 2 : 1); ++i) v[j][e][i] = src[i];
-        if (Y32)
-          for (int s = 1; s < p.yparts; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float4 o = reinterpret_cast<const float4*>(static_cast<const float*>(p.y) +
-                                                               (static_cast<int64_t>(s) * p.M + tok[m]) * p.ldy + n)[i];
-              float4 a = *reinterpret_cast<float4*>(&v[j][e][i]);
-              a = make_float4(__fadd_rn(a.x, o.x), __fadd_rn(a.y, o.y), __fadd_rn(a.z, o.z), __fadd_rn(a.w, o.w));
-              v[j][e][i] = *reinterpret_cast<uint4*>(&a);
-            }
+      for (int i = 0; i < W; i += 4) {
+        const uint4 v = reinterpret_cast<const uint4*>(src)[i / 4];
+        w[e][i] = v.x;
+        w[e][i + 1] = v.y;
+        w[e][i + 2] = v.z;
+        w[e][i + 3] = v.w;
       }
+    }
+  }
+  // rows 8 j + 2 t (+ 1) of the tile from global memory, columns n on (where whole 16-byte pieces may be read)
+  __device__ __forceinline__ void load(const LoraParams& p, const int* tok, int rows, int n, int j, int t) {
+    if (!p.vy || n + 2 * Q > p.N) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int m = 8 * j + 2 * t + e;
+      if (m >= rows) continue;
+      put(e, static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2));
+      if (Y32)
+        for (int s = 1; s < p.yparts; ++s) {
+          const float* o = static_cast<const float*>(p.y) + (static_cast<int64_t>(s) * p.M + tok[m]) * p.ldy + n;
+#pragma unroll
+          for (int i = 0; i < W; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(o + i);
+            w[e][i] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i]), v.x));
+            w[e][i + 1] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 1]), v.y));
+            w[e][i + 2] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 2]), v.z));
+            w[e][i + 3] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 3]), v.w));
+          }
+        }
+    }
+  }
+  __device__ __forceinline__ float get(int e, int i) const {
+    if (Y32) return __uint_as_float(w[e][Y32 ? i : 0]);
+    return __uint_as_float((i & 1) ? w[e][i >> 1] & 0xFFFF0000u : w[e][i >> 1] << 16);
   }
 };
 
-template <int NT, bool Y32>
-__device__ __forceinline__ void store_rows(const LoraParams& p, const int* tok, int rows, int n0, int lane,
-                                           const float (&acc)[4][NT][4], const YTile<NT, Y32>& yt, int nt0) {
-  const int g = lane >> 2, t = lane & 3;
-  const int n = n0 + 8 * g;
-  if (n >= p.N) return;
-  const int cols = min(8, p.N - n);
+// out rows 8 j + 2 t (+ 1) of the tile, columns n on: y + acc, rounded once
+template <int Q, bool Y32>
+__device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok, int rows, int n, int j, int t,
+                                            const float (&acc)[Q][4], const YRows<Q, Y32>& y) {
+  constexpr int C = 2 * Q;
+  const int cols = p.N - n;
+  if (cols <= 0) return;
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int e = 0; e < 2; ++e) {
+    const int m = 8 * j + 2 * t + e;
+    if (m >= rows) continue;
+    const int64_t row = tok[m];
+    float d[C];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int m = 8 * (nt0 + j) + 2 * t + e;
-      if (m >= rows) continue;
-      const int64_t row = tok[m];
-      float d[8];
+    for (int i = 0; i < C; ++i) d[i] = acc[i >> 1][e + 2 * (i & 1)];
+    if (p.vy && cols >= C) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        d[2 * q] = acc[q][j][e];
-        d[2 * q + 1] = acc[q][j][2 + e];
-      }
-      if (p.vy && cols == 8) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(yt.v[j][e]);
+      for (int i = 0; i < C; ++i) d[i] = __fadd_rn(y.get(e, i), d[i]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = Y32 ? __uint_as_float(w[Y32 ? i : 0])
-                              : __uint_as_float((i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
-          d[i] = __fadd_rn(y, d[i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i >= cols) break;
-          float y = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
-                        : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
-          if (Y32)
-            for (int s = 1; s < p.yparts; ++s)
-              y = __fadd_rn(y, static_cast<const float*>(p.y)[(static_cast<int64_t>(s) * p.M + row) * p.ldy + n + i]);
-          d[i] = __fadd_rn(y, d[i]);
-        }
-      }
-      if (Y32 && p.out_f32) {
-        float* op = static_cast<float*>(p.out) + row * p.ldo + n;
-        if (p.vo && cols == 8) {
-          reinterpret_cast<float4*>(op)[0] = make_float4(d[0], d[1], d[2], d[3]);
-          reinterpret_cast<float4*>(op)[1] = make_float4(d[4], d[5], d[6], d[7]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < cols) op[i] = d[i];
-        }
-      } else {
-        uint16_t* op = static_cast<uint16_t*>(p.out) + row * p.ldo + n;
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
-        if (p.vo && cols == 8) {
-          *reinterpret_cast<uint4*>(op) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < cols) op[i] = static_cast<uint16_t>(o[i >> 1] >> (16 * (i & 1)));
-        }
+      for (int i = 0; i < C; ++i) {
+        if (i >= cols) break;
+        float v = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
+                      : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
+        if (Y32)
+          for (int s = 1; s < p.yparts; ++s)
+            v = __fadd_rn(v, static_cast<const float*>(p.y)[(static_cast<int64_t>(s) * p.M + row) * p.ldy + n + i]);
+        d[i] = __fadd_rn(v, d[i]);
       }
     }
+    if (Y32 && p.out_f32) {
+      float* op = static_cast<float*>(p.out) + row * p.ldo + n;
+      if (p.vo && cols >= C) {
+#pragma unroll
+        for (int i = 0; i < C; i += 4) *reinterpret_cast<float4*>(op + i) = make_float4(d[i], d[i + 1], d[i + 2], d[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+          if (i < cols) op[i] = d[i];
+      }
+    } else {
+      uint16_t* op = static_cast<uint16_t*>(p.out) + row * p.ldo + n;
+      uint32_t o[Q];
+#pragma unroll
+      for (int i = 0; i < Q; ++i) o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
+      if (p.vo && cols >= C) {
+        if constexpr (Q == 2) *reinterpret_cast<uint2*>(op) = make_uint2(o[0], o[1]);
+        else *reinterpret_cast<uint4*>(op) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+          if (i < cols) op[i] = static_cast<uint16_t>(o[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
 }
 
 // scale * h of one token and two ranks as packed bf16 pieces
@@ -296,17 +305,18 @@ __device__ __forceinline__ void pieces(float2 v, int ns, uint32_t (&w)[3]) {
   }
 }
 
-// B rows n0 + 8 g + 2 j (+ 1) for j = 0..3, rank columns r .. r + 7 (past the rank: 0, whatever is stored)
-__device__ __forceinline__ void load_b(const LoraParams& p, const LoraTile& tl, int n0, int r, int g, uint4 (&vb)[8]) {
-  const uint16_t* row = static_cast<const uint16_t*>(p.b) + (static_cast<int64_t>(tl.id) * p.N + n0 + 8 * g) * p.R + r;
-  const int valid = tl.rank - r, rows = p.N - n0 - 8 * g;
+// B rows n .. n + 2 Q - 1 (a lane's columns), rank columns r .. r + 7 (past the rank: 0, whatever is stored)
+template <int Q>
+__device__ __forceinline__ void load_b(const LoraParams& p, const LoraTile& tl, int n, int r, uint4 (&vb)[2 * Q]) {
+  const uint16_t* row = static_cast<const uint16_t*>(p.b) + (static_cast<int64_t>(tl.id) * p.N + n) * p.R + r;
+  const int valid = tl.rank - r, rows = p.N - n;
   if (p.wb == 8) {  // R is a multiple of 8: whole vectors are in the row, the columns past the rank are cleared
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 2 * Q; ++i)
       vb[i] = (i < rows && valid > 0) ? __ldg(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i) * p.R)) : make_uint4(0, 0, 0, 0);
     if (valid < 8) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 2 * Q; ++i) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&vb[i]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -317,36 +327,37 @@ __device__ __forceinline__ void load_b(const LoraParams& p, const LoraTile& tl, 
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vb[i] = load8<false>(row + static_cast<int64_t>(i) * p.R, i < rows ? valid : 0);
+    for (int i = 0; i < 2 * Q; ++i) vb[i] = load8<false>(row + static_cast<int64_t>(i) * p.R, i < rows ? valid : 0);
   }
 }
 
-template <int NTG, int AT>
-__device__ __forceinline__ void expand_step(float (&acc)[4][NTG][4], const uint4 (&vb)[8], const uint16_t* hf, int hpitch,
-                                            int hsplit, int ns, int nt0, int rows, int rc, int lane) {
+// acc[q][j] += B rows x h of the tile's rows 8 (j0 + j) .. + 7, rank columns 32 rc .. 32 rc + 31
+template <int Q, int NT, int AT>
+__device__ __forceinline__ void expand_step(float (&acc)[NT][Q][4], const uint4 (&vb)[2 * Q], const uint16_t* hf, int hpitch,
+                                            int hsplit, int ns, int j0, int rows, int rc, int lane) {
   const int g = lane >> 2, t = lane & 3;
   // (fp16 adapters: a pair of B rows at a time is split into its two pieces, and h read again for it)
 #pragma unroll
-  for (int q0 = 0; q0 < 4; q0 += AT == AD_F16 ? 1 : 4) {
+  for (int q0 = 0; q0 < Q; q0 += AT == AD_F16 ? 1 : Q) {
     uint4 h0, l0, h1, l1;
     if (AT == AD_F16) {
       split4_f16(vb[2 * q0], h0, l0);
       split4_f16(vb[2 * q0 + 1], h1, l1);
     }
 #pragma unroll
-    for (int j = 0; j < NTG; ++j) {
-      if (8 * (nt0 + j) >= rows) continue;  // warp-uniform
-      const uint16_t* hrow = hf + (8 * (nt0 + j) + g) * hpitch + 32 * rc + 8 * t;
+    for (int j = 0; j < NT; ++j) {
+      if (8 * (j0 + j) >= rows) continue;  // warp-uniform
+      const uint16_t* hrow = hf + (8 * (j0 + j) + g) * hpitch + 32 * rc + 8 * t;
 #pragma unroll
       for (int s = 0; s < 3; ++s) {
         if (s >= ns) break;  // uniform
         const uint4 h = *reinterpret_cast<const uint4*>(hrow + s * hsplit);
         if (AT == AD_F16) {
-          mma_pair(acc[q0][j], h0, h1, h);
-          mma_pair(acc[q0][j], l0, l1, h);
+          mma_pair(acc[j][q0], h0, h1, h);
+          if (s < 2) mma_pair(acc[j][q0], l0, l1, h);  // (the third pieces' product is below 2^-24 of h b)
         } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mma_pair(acc[q][j], vb[2 * q], vb[2 * q + 1], h);
+          for (int q = 0; q < Q; ++q) mma_pair(acc[j][q], vb[2 * q], vb[2 * q + 1], h);
         }
       }
     }
@@ -438,9 +449,10 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
 
   const int nblk = (p.N + 63) / 64;
   const int gw = crank * kLoraWarps + warp, nw = csize * kLoraWarps;
+  const int c8 = 8 * g;  // this lane's columns of a block
   uint4 vb[8];
-  YTile<1, Y32> yt;
-  if (!p.wait_y && gw < nblk) yt.load(p, tok, tl.rows, gw * 64, lane, 0);
+  YRows<4, Y32> yt;
+  if (!p.wait_y && gw < nblk) yt.load(p, tok, tl.rows, gw * 64 + c8, 0, t);
   bool pending = false;
   if (tl.rank > 0) {
     // ---- first product: this warp's share of K
@@ -454,7 +466,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
     const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (gw + 1) / nw);
     shrink<MT, AT, VEC>(p, tok, tl, c0, c1, lane, acc);
     // the first block's B rows are on the way while the sums are joined
-    if (gw < nblk) load_b(p, tl, gw * 64, 8 * t, g, vb);
+    if (gw < nblk) load_b<4>(p, tl, gw * 64 + c8, 8 * t, vb);
     // ---- sums over the warps of the CTA, in warp order
     float* mine = red + warp * C::TM * C::PITCH;
 #pragma unroll
@@ -493,22 +505,22 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
   }
   if (p.wait_y) {
     pdl_wait();
-    if (gw < nblk) yt.load(p, tok, tl.rows, gw * 64, lane, 0);
+    if (gw < nblk) yt.load(p, tok, tl.rows, gw * 64 + c8, 0, t);
   }
   // ---- second product: 64-column blocks
   const int rchunks = (tl.rank + 31) / 32;
   for (int nb = gw; nb < nblk; nb += nw) {
-    float acc[4][1][4];
+    float acc[1][4][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[q][0][i] = -0.f;  // y + -0 is y, also for y = -0
-    if (nb != gw) yt.load(p, tok, tl.rows, nb * 64, lane, 0);
+      for (int i = 0; i < 4; ++i) acc[0][q][i] = -0.f;  // y + -0 is y, also for y = -0
+    if (nb != gw) yt.load(p, tok, tl.rows, nb * 64 + c8, 0, t);
     for (int rc = 0; rc < rchunks; ++rc) {
-      if (nb != gw || rc != 0) load_b(p, tl, nb * 64, 32 * rc + 8 * t, g, vb);
-      expand_step<1, AT>(acc, vb, hf, C::HPITCH, HS, ns, 0, tl.rows, rc, lane);
+      if (nb != gw || rc != 0) load_b<4>(p, tl, nb * 64 + c8, 32 * rc + 8 * t, vb);
+      expand_step<4, 1, AT>(acc, vb, hf, C::HPITCH, HS, ns, 0, tl.rows, rc, lane);
     }
-    store_rows<1, Y32>(p, tok, tl.rows, nb * 64, lane, acc, yt, 0);
+    finish_rows<4, Y32>(p, tok, tl.rows, nb * 64 + c8, 0, t, acc[0], yt);
   }
   pdl_launch_dependents();
   if (pending) cluster_wait();
@@ -680,14 +692,14 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
 }
 
 // ------------------------------------------------------------------ many rows: second product
-// CTA (tile, 512 columns of N, 256 where y is fp32): a warp takes 64 columns, and goes through the tile's rows (or
-// half of them) 8 * NT at a time. The tile's part of y, its rows and its B rows do not depend on the first
-// product: they are on their way (y by asynchronous copies) while that runs, so what follows it is the sums of
-// the shares of K in order, the MMAs and the stores.
+// CTA (tile, 512 columns of N, 256 where y is fp32): a warp takes 32 columns and all rows of the tile (half of them
+// where there are few columns), so every value of B is read and, where it has to be, split or moved into place once. The
+// tile's part of y, its rows and its B rows do not depend on the first product: they are on their way (y by
+// asynchronous copies) while that runs, so what follows it is the sums of the shares of K in order, the MMAs and
+// the stores.
 template <bool Y32>
 struct ExpandCfg {
-  static constexpr int BLOCKS = Y32 ? 4 : 8;            // 64-column blocks of a CTA
-  static constexpr int COLS = 64 * BLOCKS;
+  static constexpr int COLS = Y32 ? 256 : 512;
   static constexpr int YPITCH = COLS * (Y32 ? 4 : 2) + 16;  // bytes; rows 2t of a quarter warp on distinct banks
   static constexpr int YBYTES = kTile * YPITCH;
 };
@@ -695,7 +707,7 @@ struct ExpandCfg {
 template <int AT, bool Y32>
 __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const __grid_constant__ LoraParams p) {
   using C = ExpandCfg<Y32>;
-  constexpr int NT = 4, HALVES = kLoraWarps / C::BLOCKS;
+  constexpr int NT = kTile / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[kTile];
   uint16_t* hf = reinterpret_cast<uint16_t*>(smem + C::YBYTES);
@@ -713,8 +725,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   const int ns = p.out_f32 ? 3 : 2;
   const int rchunks = (tl.rank + 31) / 32;
   const int hpitch = 32 * ((p.rp + 31) / 32) + 8, hs = kTile * hpitch;
-  const int col0 = np * C::COLS, n0 = col0 + 64 * (warp % C::BLOCKS);
-  const bool busy = n0 < p.N;
+  const int col0 = np * C::COLS, blocks = (min(C::COLS, p.N - col0) + 31) / 32;
+  // this warp's first block and rows 8 j0 .. 8 j1 - 1 of the tile
+  const bool halves = blocks <= kLoraWarps / 2 && tl.rows > kTile / 2;
+  const int first = halves ? warp % (kLoraWarps / 2) : warp, step = halves ? kLoraWarps / 2 : kLoraWarps;
+  const int j0 = halves && warp >= kLoraWarps / 2 ? NT / 2 : 0;
+  const int rows = halves && warp < kLoraWarps / 2 ? kTile / 2 : tl.rows;
   auto load_y = [&]() {
     if (p.vy) {  // 16 bytes a copy, whole rows of the tile
       constexpr int per = C::COLS * (Y32 ? 4 : 2) / 16, each = Y32 ? 4 : 8;
@@ -739,8 +755,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
     cp_commit();
   };
   if (!p.wait_y) load_y();
-  uint4 vb[8];
-  if (busy && rchunks > 0) load_b(p, tl, n0, 8 * t, g, vb);
+  uint4 vb[4];
+  if (first < blocks && rchunks > 0) load_b<2>(p, tl, col0 + 32 * first + 4 * g, 8 * t, vb);
   pdl_wait();
   if (p.wait_y) load_y();
   for (int e = tid; e < tl.rows * rchunks * 16; e += kLoraThreads) {
@@ -765,37 +781,26 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   cp_wait<0>();
   __syncthreads();
   pdl_launch_dependents();
-  if (!busy) return;
-  const uint8_t* ys = smem + (n0 - col0 + 8 * g) * (Y32 ? 4 : 2);
-  const int groups = (tl.rows + 8 * NT - 1) / (8 * NT);
-  for (int gr = warp / C::BLOCKS; gr < groups; gr += HALVES) {
-    const int nt0 = gr * NT;
-    float acc[4][NT][4];
+  for (int bk = first; bk < blocks; bk += step) {
+    const int c = 32 * bk + 4 * g, n = col0 + c;
+    float acc[NT][2][4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[q][j][i] = -0.f;  // y + -0 is y, also for y = -0
+        for (int i = 0; i < 4; ++i) acc[j][q][i] = -0.f;  // y + -0 is y, also for y = -0
     for (int rc = 0; rc < rchunks; ++rc) {
-      if (rchunks > 1 && (gr >= HALVES || rc)) load_b(p, tl, n0, 32 * rc + 8 * t, g, vb);
-      expand_step<NT, AT>(acc, vb, hf, hpitch, hs, ns, nt0, tl.rows, rc, lane);
+      if (bk != first || rc) load_b<2>(p, tl, n, 32 * rc + 8 * t, vb);
+      expand_step<2, NT, AT>(acc, vb, hf, hpitch, hs, ns, j0, rows, rc, lane);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      if (8 * (nt0 + j) >= tl.rows) break;
-      YTile<1, Y32> yt;
+      if (8 * (j0 + j) >= rows) break;
+      YRows<2, Y32> y;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < (Y32 ? 2 : 1); ++i)
-          yt.v[0][e][i] = reinterpret_cast<const uint4*>(ys + (8 * (nt0 + j) + 2 * t + e) * C::YPITCH)[i];
-      float d[4][1][4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[q][0][i] = acc[q][j][i];
-      store_rows<1, Y32>(p, tok, tl.rows, n0, lane, d, yt, nt0 + j);
+      for (int e = 0; e < 2; ++e) y.put(e, smem + (8 * (j0 + j) + 2 * t + e) * C::YPITCH + c * (Y32 ? 4 : 2));
+      finish_rows<2, Y32>(p, tok, rows, n, j0 + j, t, acc[j], y);
     }
   }
 }
