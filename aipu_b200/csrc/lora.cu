@@ -759,24 +759,37 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   if (first < blocks && rchunks > 0) load_b<2>(p, tl, col0 + 32 * first + 4 * g, 8 * t, vb);
   pdl_wait();
   if (p.wait_y) load_y();
-  for (int e = tid; e < tl.rows * rchunks * 16; e += kLoraThreads) {
-    const int m = e / (rchunks * 16), r = 2 * (e - m * rchunks * 16);
-    float2 v = make_float2(0.f, 0.f);
-    if (r < p.rp) {
-      const float* src = p.sums + static_cast<int64_t>(tile.y + m) * p.rp + r;
-#pragma unroll 4
-      for (int s = 0; s < p.ksplit; ++s) {
-        const float2 o = *reinterpret_cast<const float2*>(src + static_cast<int64_t>(s) * p.M * p.rp);
-        v.x = __fadd_rn(v.x, o.x);
-        v.y = __fadd_rn(v.y, o.y);
-      }
+  // four ranks a thread and step, two steps at a time: their loads of all shares are in flight together
+  const int quads = 8 * rchunks, all = tl.rows * quads;
+  for (int e0 = tid; e0 < all; e0 += 2 * kLoraThreads) {
+    float4 v[2];
+    int m[2], r[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int e = e0 + u * kLoraThreads;
+      m[u] = e / quads;
+      r[u] = 4 * (e - m[u] * quads);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
-    if (r >= tl.rank) v.x = 0.f;
-    if (r + 1 >= tl.rank) v.y = 0.f;
-    uint32_t w[3];
-    pieces(v, ns, w);
-    for (int s = 0; s < ns; ++s) reinterpret_cast<uint32_t*>(hf)[(s * hs + m * hpitch + r) >> 1] = w[s];
+#pragma unroll 4
+    for (int s = 0; s < p.ksplit; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (e0 + u * kLoraThreads < all && r[u] < p.rp) {
+          const float4 o = *reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(s) * p.M + tile.y + m[u]) * p.rp + r[u]);
+          v[u] = make_float4(__fadd_rn(v[u].x, o.x), __fadd_rn(v[u].y, o.y), __fadd_rn(v[u].z, o.z), __fadd_rn(v[u].w, o.w));
+        }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (e0 + u * kLoraThreads >= all) break;
+      // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
+      const int left = tl.rank - r[u];
+      uint32_t w0[3], w1[3];
+      pieces(make_float2(left > 0 ? v[u].x : 0.f, left > 1 ? v[u].y : 0.f), ns, w0);
+      pieces(make_float2(left > 2 ? v[u].z : 0.f, left > 3 ? v[u].w : 0.f), ns, w1);
+      for (int s = 0; s < ns; ++s)
+        *reinterpret_cast<uint2*>(hf + s * hs + m[u] * hpitch + r[u]) = make_uint2(w0[s], w1[s]);
+    }
   }
   cp_wait<0>();
   __syncthreads();
@@ -1027,7 +1040,7 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   b += 256 + al256l(4 * static_cast<size_t>(p.M));
   p.tiles = reinterpret_cast<int4*>(b);
   p.sums = reinterpret_cast<float*>(b + al256l(16 * max_tiles(p.M, p.L)));
-  p.ksplit = k_split(p.M, p.L);
+  p.ksplit = std::min(k_split(p.M, p.L), std::max(1, p.K / 256));  // (of four chunks at least)
   p.nsplit = p.y_f32 ? (p.N + ExpandCfg<true>::COLS - 1) / ExpandCfg<true>::COLS : (p.N + ExpandCfg<false>::COLS - 1) / ExpandCfg<false>::COLS;
   const void* kern = reinterpret_cast<const void*>(aipu_lora_plan_kernel);
   static bool attr[64] = {false};
