@@ -251,7 +251,9 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
         tma_load_2d(base + s * C::STAGE, &p.wmap, 64 * (k0 + i), n0, &bars.full[s]);
         tma_load_2d(base + s * C::STAGE + C::A, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
       }
-      if (*abort)  // no copy may land after the CTA has ended
+      // no copy may land after the CTA has ended: the MMAs have read them all, or (abort) they are waited for
+      mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL);
+      if (*abort)
         for (int i = max(0, issued - C::S); i < issued; ++i)
           mbar_wait_bounded(&bars.full[i % C::S], (i / C::S) & 1, p.status, ST_TIMEOUT_FULL, 200000000LL);
     }

@@ -28,6 +28,7 @@
 // enters the second product as 2 (bf16 result) or 3 (fp32 result) bf16 pieces, 16 and 24 bits. fp16
 // adapters enter as two bf16 pieces (11 bits: exact).
 #include <algorithm>
+#include <cstdint>
 
 #include "cluster.cuh"
 #include "common.cuh"
@@ -54,8 +55,8 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint3
 
 // 8 consecutive 16-bit values at p, of which `valid` (from the first) are wanted and the others come as 0. VEC: p is
 // 16-byte aligned and valid is 0 or 8. Else from the one or two aligned 16-byte pieces that hold wanted values
-// (the tensors are readable to such boundaries), moved into place by selects and a funnel shift: an eighth of
-// the loads that one value at a time would take (rank 71, 2555 rows: MEASURED1).
+// (the tensors are readable to such boundaries), moved into place by selects and a funnel shift: a quarter of
+// the loads that one value at a time takes, and far less code (1 row of aligned 4096 x 4096 got 1.8 us faster too).
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int valid) {
   if (valid <= 0) return make_uint4(0, 0, 0, 0);
@@ -1021,6 +1022,8 @@ static int load_width(const void* ptr, int64_t ld) {
 
 int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   if (p.L > kMaxAdapters || p.R > 128) return set_error(EINVAL_, "lora: at most 32768 adapters of rank 128");
+  if (max_tiles(p.M, p.L) * std::max<int64_t>(kMaxSplit, (p.N + 255) / 256) > INT32_MAX)
+    return set_error(EINVAL_, "lora: too many rows and columns for one launch");
   p.skip_plain = (p.out == p.y && p.out_f32 == p.y_f32) ? 1 : 0;
   p.rp = padded_rank(p.R);
   // (an even row length is what the pairwise copies of the first product need of A and x)

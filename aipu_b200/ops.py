@@ -499,29 +499,30 @@ class LogitControls:
                 self.mask_rows)
 
     def cstruct(self, M: int, V: int) -> L.LogitCtl:
-        def need(t, name, dtype, shape):
-            if t is None or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
-            return t.data_ptr()
-
         tokens, spans, pen, begin, bid, val, mask, rows = self.tensors()
         nt = nb = nm = 0
         pt = ps = pp = p0 = p1 = p2 = pm = pw = None
         if spans is not None or pen is not None or tokens is not None:
             nt = tokens.numel() if tokens is not None else 0
-            pt = need(tokens, "tokens", torch.int32, (nt,))
-            ps = need(spans, "spans", torch.int64, (M, 3))
-            pp = need(pen, "penalties", torch.float32, (M, 3))
+            pt = _need(tokens, "tokens", torch.int32, (nt,))
+            ps = _need(spans, "spans", torch.int64, (M, 3))
+            pp = _need(pen, "penalties", torch.float32, (M, 3))
         if begin is not None or bid is not None or val is not None:
             nb = bid.numel() if bid is not None else 0
-            p0 = need(begin, "bias_begin", torch.int64, (M + 1,))
-            p1 = need(bid, "bias_ids", torch.int32, (nb,))
-            p2 = need(val, "bias_vals", torch.float32, (nb,))
+            p0 = _need(begin, "bias_begin", torch.int64, (M + 1,))
+            p1 = _need(bid, "bias_ids", torch.int32, (nb,))
+            p2 = _need(val, "bias_vals", torch.float32, (nb,))
         if mask is not None or rows is not None:
             nm = mask.shape[0] if mask is not None else 0
-            pm = need(mask, "mask", torch.int32, (nm, (V + 31) // 32))
-            pw = need(rows, "mask_rows", torch.int32, (M,))
+            pm = _need(mask, "mask", torch.int32, (nm, (V + 31) // 32))
+            pw = _need(rows, "mask_rows", torch.int32, (M,))
         return L.LogitCtl(pt, nt, ps, pp, p0, p1, p2, nb, pm, pw, nm)
+
+
+def _need(t, name, dtype, shape):
+    if t is None or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
+    return t.data_ptr()
 
 
 def _logits(logits, controls, ctx, out, want_out):
@@ -533,12 +534,12 @@ def _logits(logits, controls, ctx, out, want_out):
     ldo = V
     if out is None:
         if want_out:
-            out = torch.empty((M, V), dtype=torch.float32, device=logits.device)
+            out = logits.new_empty((M, V), dtype=torch.float32)
     else:
         ldo = _row_stride(out, "out", M, V)
         if out.dtype != torch.float32:
             raise ValueError("out must be fp32 [M, V]")
-    token = torch.empty(M, dtype=torch.int32, device=logits.device)
+    token = logits.new_empty((M,), dtype=torch.int32)
     ctx, index = _on(ctx, logits, out, *(controls.tensors() if controls is not None else ()))
     rc = lib().aipu_logits_process(ctx.handle, logits.data_ptr(), _DTYPE[logits.dtype], ld, M, V, cs,
                                    out.data_ptr() if want_out else None, ldo, token.data_ptr(), _raw_stream(index))

@@ -275,6 +275,56 @@ def test_gemm_lora_many_rows_at_tile_borders(wt, M, K, N):
     _check(o, x64 @ wd.t(), torch.zeros_like(mag), torch.zeros_like(mag), K, extra)
 
 
+@pytest.mark.parametrize("wt", [F.Q4_K, F.F16])
+@pytest.mark.parametrize("M", [4, 40, 200, 300])
+def test_gemm_lora_fp16_adapters_ranks_out_and_another_stream(wt, M):
+    K, N, R = 512, 333, 24
+    A, ids, x = _case(M, K, N, R, 4, HF, ranks=True)
+    w = torch.from_numpy(F.random_rows_np(wt, N, K, seed=M)).to(x.device)
+    wd = ops.dequant(wt, w, N, K).double().cpu()
+    A.b.mul_(float(wd.square().mean().sqrt()) * K ** 0.5)
+    d, s = _delta(A, ids, x)
+    ctx = ops.Context(x.device)
+    out = torch.full((M + 2, N), 7.0, dtype=BF, device=x.device)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        o = ops.gemm_lora(wt, w, N, K, x, A, ids, ctx=ctx, out=out[1:M + 1])
+    st.synchronize()
+    assert o.data_ptr() == out[1:].data_ptr() and (out[0] == 7).all() and (out[M + 1] == 7).all()
+    mag = x.double().cpu().abs() @ wd.abs().t()
+    if wt == F.Q4_K:
+        dm = np.ascontiguousarray(w.view(-1, 144).cpu().numpy()[:, 2:4]).view(np.float16).astype(np.float64).reshape(N, K // 256)
+        mag = mag + 2 * 63 * (x.double().cpu().abs().view(M, -1, 256).sum(2) @ torch.from_numpy(dm).t())
+    extra = mag * (4 * K * 2.0 ** -24 + (2.0 ** -11 if M > 8 and wt != F.F16 else 0.0))
+    extra = extra + 2.0 ** -34 * x.double().cpu().abs().amax(1, keepdim=True) * wd.abs().sum(1)
+    _check(o, x.double().cpu() @ wd.t(), d, s, K, extra)
+    assert ctx.status() == 0
+    bad = ids.clone()
+    bad[1] = 4
+    ids[1] = -1
+    assert torch.equal(ops.gemm_lora(wt, w, N, K, x, A, bad, ctx=ctx), ops.gemm_lora(wt, w, N, K, x, A, ids, ctx=ctx))
+    assert ctx.status() == 4
+    ctx.close()
+
+
+def test_two_devices():
+    """A context and tensors on another device than the current one; tensors on two devices are refused."""
+    if _dev() is None or torch.cuda.device_count() < 2:
+        pytest.skip("needs two CUDA devices")
+    A, ids, x = _case(70, 512, 96, 16, 3)
+    y = torch.randn((70, 96), device=x.device)
+    w = torch.from_numpy(F.random_rows_np(F.Q4_K, 96, 512, seed=1)).to(x.device)
+    far = torch.device("cuda", 1)
+    B = ops.LoraAdapters(A.a.to(far), A.b.to(far), A.scale.to(far))
+    assert torch.equal(ops.lora_add(B, ids.to(far), x.to(far), y.to(far)).cpu(), ops.lora_add(A, ids, x, y).cpu())
+    assert torch.equal(ops.gemm_lora(F.Q4_K, w.to(far), 96, 512, x.to(far), B, ids.to(far)).cpu(),
+                       ops.gemm_lora(F.Q4_K, w, 96, 512, x, A, ids).cpu())
+    assert torch.equal(ops.greedy_tokens(y.to(far)).cpu(), ops.greedy_tokens(y).cpu())
+    with pytest.raises(ValueError):
+        ops.lora_add(A, ids, x, y.to(far))
+
+
 @pytest.mark.parametrize("M", [3, 90, 290])
 def test_captured_and_replayed_with_new_inputs(M):
     A, ids, x = _case(M, 512, 96, 16, 3)
