@@ -1409,7 +1409,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
   if (!c) return set_error(EINVAL_, "gemm_lora: null context");
   if (M == 0) return OK;
-  if ((N + 15) / 16 > c->ws[0].max_tiles) return set_error(EINVAL_, "gemm_lora: N too large for the workspace");
+  if (!gemm_lora_dense(M) && (N + 15) / 16 > c->ws[0].max_tiles) return set_error(EINVAL_, "gemm_lora: N too large for the workspace");
   DeviceGuard dg(c->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* b = static_cast<uint8_t*>(ws);
@@ -1446,7 +1446,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     g.status = c->status;
     // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
     // kernel behind it may read x, the ids and the adapters without waiting for it
-    rc = gemv_launch(wtype, XT_BF16, EPI_STORE, g, c->num_sms, s, false);
+    rc = gemv_launch(wtype, XT_BF16, EPI_STORE32, g, c->num_sms, s, false);
   }
   if (rc) return rc;
   p.wait_y = 1;

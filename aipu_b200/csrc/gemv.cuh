@@ -39,7 +39,7 @@ constexpr int GEMV_MAXW = 16;   // warps per CTA (each an independent worker)
 constexpr int GEMV_MAXS = 4;    // ring slots per warp
 constexpr int GEMV_MAXXG = 4;   // activation groups staged per CTA
 
-enum Epi : int { EPI_STORE = 0, EPI_SWIGLU = 1 };
+enum Epi : int { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_STORE32 = 2 };  // (2: the fp32 sums, bf16 x, one group)
 
 struct GemvParams {
   const uint8_t* w0;         // rows of the matrix (or the gate rows for EPI_SWIGLU)
@@ -55,7 +55,7 @@ struct GemvParams {
   int64_t x_group_stride;    // elements
   int M;                     // tokens (<= 8 bf16, <= 4 fp32)
   uint16_t* y;               // bf16 out [M, N] per group (EPI_SWIGLU: h [M, N])
-  float* y32;                // EPI_STORE, bf16 x: fp32 out instead of y (nullable), one group
+  float* y32;                // EPI_STORE32: fp32 out [M, y32_ld]
   int64_t y32_ld;            // elements between its rows
   int64_t y_group_stride;    // elements
   float* partials;           // stream-K workspace [grid][2][32][4]
