@@ -238,7 +238,7 @@ struct YRows {
 };
 
 // out rows 8 j + 2 t (+ 1) of the tile, columns n on: y + acc, rounded once
-template <int Q, bool Y32>
+template <int Q, bool Y32, bool O32>
 __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok, int rows, int n, int j, int t,
                                             const float (&acc)[Q][4], const YRows<Q, Y32>& y) {
   constexpr int C = 2 * Q;
@@ -267,7 +267,7 @@ __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok,
         d[i] = __fadd_rn(v, d[i]);
       }
     }
-    if (Y32 && p.out_f32) {
+    if (O32) {
       float* op = static_cast<float*>(p.out) + row * p.ldo + n;
       if (p.vo && cols >= C) {
 #pragma unroll
@@ -295,10 +295,11 @@ __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok,
 }
 
 // scale * h of one token and two ranks as packed bf16 pieces
-__device__ __forceinline__ void pieces(float2 v, int ns, uint32_t (&w)[3]) {
+template <int NS>
+__device__ __forceinline__ void pieces(float2 v, uint32_t (&w)[NS]) {
   float r0, r1, q0, q1;
   w[0] = piece(v.x, r0) | (piece(v.y, r1) << 16);
-  if (ns == 2) {
+  if constexpr (NS == 2) {
     w[1] = pack_bf16(r0, r1);
   } else {
     w[1] = piece(r0, q0) | (piece(r1, q1) << 16);
@@ -333,9 +334,9 @@ __device__ __forceinline__ void load_b(const LoraParams& p, const LoraTile& tl, 
 }
 
 // acc[q][j] += B rows x h of the tile's rows 8 (j0 + j) .. + 7, rank columns 32 rc .. 32 rc + 31
-template <int Q, int NT, int AT>
+template <int Q, int NT, int AT, int NS>
 __device__ __forceinline__ void expand_step(float (&acc)[NT][Q][4], const uint4 (&vb)[2 * Q], const uint16_t* hf, int hpitch,
-                                            int hsplit, int ns, int j0, int rows, int rc, int lane) {
+                                            int hsplit, int j0, int rows, int rc, int lane) {
   const int g = lane >> 2, t = lane & 3;
   // (fp16 adapters: a pair of B rows at a time is split into its two pieces, and h read again for it)
 #pragma unroll
@@ -349,18 +350,29 @@ __device__ __forceinline__ void expand_step(float (&acc)[NT][Q][4], const uint4 
     for (int j = 0; j < NT; ++j) {
       if (8 * (j0 + j) >= rows) continue;  // warp-uniform
       const uint16_t* hrow = hf + (8 * (j0 + j) + g) * hpitch + 32 * rc + 8 * t;
+      constexpr int QN = AT == AD_F16 ? 1 : Q;
+      // fp32 results: the MMA's own sums are cut off and not rounded, so it sums 32 ranks only, the small pieces
+      // first, and the rest is rounded adds
+      float sum[QN][4];
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
-        if (s >= ns) break;  // uniform
+      for (int q = 0; q < QN; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[q][i] = NS == 3 ? 0.f : acc[j][q0 + q][i];
+#pragma unroll
+      for (int s = NS - 1; s >= 0; --s) {
         const uint4 h = *reinterpret_cast<const uint4*>(hrow + s * hsplit);
         if (AT == AD_F16) {
-          mma_pair(acc[j][q0], h0, h1, h);
-          if (s < 2) mma_pair(acc[j][q0], l0, l1, h);  // (the third pieces' product is below 2^-24 of h b)
+          if (s < 2) mma_pair(sum[0], l0, l1, h);  // (the third pieces' product is below 2^-24 of h b)
+          mma_pair(sum[0], h0, h1, h);
         } else {
 #pragma unroll
-          for (int q = 0; q < Q; ++q) mma_pair(acc[j][q], vb[2 * q], vb[2 * q + 1], h);
+          for (int q = 0; q < QN; ++q) mma_pair(sum[q], vb[2 * q], vb[2 * q + 1], h);
         }
       }
+#pragma unroll
+      for (int q = 0; q < QN; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][q0 + q][i] = NS == 3 ? __fadd_rn(acc[j][q0 + q][i], sum[q][i]) : sum[q][i];
     }
   }
 }
@@ -375,7 +387,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int id, int r
   return tl;
 }
 
-template <int MT, int AT, bool VEC, bool Y32>
+template <int MT, int AT, bool VEC, bool Y32, bool O32>
 __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
   using C = LoraCfg<MT>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -386,7 +398,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t crank = cluster_rank(), csize = cluster_size();
-  const int ns = p.out_f32 ? 3 : 2;
+  constexpr int NS = O32 ? 3 : 2;  // pieces of h
   constexpr int HS = C::TM * C::HPITCH;  // elements of one piece
   // x (and the ids) may come from the kernel before the one that writes y, so they wait too unless the
   // launch says that only y does
@@ -496,9 +508,10 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
       // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
       v.x = r < tl.rank ? __fmul_rn(v.x, tl.scale) : 0.f;
       v.y = r + 1 < tl.rank ? __fmul_rn(v.y, tl.scale) : 0.f;
-      uint32_t w[3];
-      pieces(v, ns, w);
-      for (int s = 0; s < ns; ++s) reinterpret_cast<uint32_t*>(hf)[(s * HS + m * C::HPITCH + r) >> 1] = w[s];
+      uint32_t w[NS];
+      pieces<NS>(v, w);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) reinterpret_cast<uint32_t*>(hf)[(s * HS + m * C::HPITCH + r) >> 1] = w[s];
     }
     cluster_arrive();  // no CTA ends before the others have read its sums
     pending = true;
@@ -519,9 +532,9 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) ai
     if (nb != gw) yt.load(p, tok, tl.rows, nb * 64 + c8, 0, t);
     for (int rc = 0; rc < rchunks; ++rc) {
       if (nb != gw || rc != 0) load_b<4>(p, tl, nb * 64 + c8, 32 * rc + 8 * t, vb);
-      expand_step<4, 1, AT>(acc, vb, hf, C::HPITCH, HS, ns, 0, tl.rows, rc, lane);
+      expand_step<4, 1, AT, NS>(acc, vb, hf, C::HPITCH, HS, 0, tl.rows, rc, lane);
     }
-    finish_rows<4, Y32>(p, tok, tl.rows, nb * 64 + c8, 0, t, acc[0], yt);
+    finish_rows<4, Y32, O32>(p, tok, tl.rows, nb * 64 + c8, 0, t, acc[0], yt);
   }
   pdl_launch_dependents();
   if (pending) cluster_wait();
@@ -655,6 +668,11 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
     issue(c + S - 1);
     const uint32_t st = use * STAGE;
     if (++use == S) use = 0;
+    float sum[MT][4];  // (rounded adds from chunk to chunk: the MMA's own sums are cut off)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum[i][q] = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint32_t x[4];
@@ -669,14 +687,18 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
             uint32_t h0, l0, h1, l1;
             split_f16(w[2 * h], h0, l0);
             split_f16(w[2 * h + 1], h1, l1);
-            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], h0, h1);
-            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], l0, l1);
+            mma_bf16_16816(sum[i + h], x[0], x[1], x[2], x[3], l0, l1);
+            mma_bf16_16816(sum[i + h], x[0], x[1], x[2], x[3], h0, h1);
           } else {
-            mma_bf16_16816(acc[i + h], x[0], x[1], x[2], x[3], w[2 * h], w[2 * h + 1]);
+            mma_bf16_16816(sum[i + h], x[0], x[1], x[2], x[3], w[2 * h], w[2 * h + 1]);
           }
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[i][q] = __fadd_rn(acc[i][q], sum[i][q]);
   }
   cp_wait<0>();
   const int g = lane >> 2, t = lane & 3;
@@ -705,7 +727,7 @@ struct ExpandCfg {
   static constexpr int YBYTES = kTile * YPITCH;
 };
 
-template <int AT, bool Y32>
+template <int AT, bool Y32, bool O32>
 __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const __grid_constant__ LoraParams p) {
   using C = ExpandCfg<Y32>;
   constexpr int NT = kTile / 8;
@@ -723,7 +745,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   const LoraTile tl = {tile.x, tile.z, tile.w, 1.f};
   if (tid < kTile) tok[tid] = tid < tl.rows ? p.perm[tile.y + tid] : 0;
   __syncthreads();
-  const int ns = p.out_f32 ? 3 : 2;
+  constexpr int NS = O32 ? 3 : 2;  // pieces of h
   const int rchunks = (tl.rank + 31) / 32;
   const int hpitch = 32 * ((p.rp + 31) / 32) + 8, hs = kTile * hpitch;
   const int col0 = np * C::COLS, blocks = (min(C::COLS, p.N - col0) + 31) / 32;
@@ -785,10 +807,11 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
       if (e0 + u * kLoraThreads >= all) break;
       // past the rank the sums are 0, or NaN where x is not finite: they count for nothing
       const int left = tl.rank - r[u];
-      uint32_t w0[3], w1[3];
-      pieces(make_float2(left > 0 ? v[u].x : 0.f, left > 1 ? v[u].y : 0.f), ns, w0);
-      pieces(make_float2(left > 2 ? v[u].z : 0.f, left > 3 ? v[u].w : 0.f), ns, w1);
-      for (int s = 0; s < ns; ++s)
+      uint32_t w0[NS], w1[NS];
+      pieces<NS>(make_float2(left > 0 ? v[u].x : 0.f, left > 1 ? v[u].y : 0.f), w0);
+      pieces<NS>(make_float2(left > 2 ? v[u].z : 0.f, left > 3 ? v[u].w : 0.f), w1);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
         *reinterpret_cast<uint2*>(hf + s * hs + m[u] * hpitch + r[u]) = make_uint2(w0[s], w1[s]);
     }
   }
@@ -806,7 +829,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
         for (int i = 0; i < 4; ++i) acc[j][q][i] = -0.f;  // y + -0 is y, also for y = -0
     for (int rc = 0; rc < rchunks; ++rc) {
       if (bk != first || rc) load_b<2>(p, tl, n, 32 * rc + 8 * t, vb);
-      expand_step<2, NT, AT>(acc, vb, hf, hpitch, hs, ns, j0, rows, rc, lane);
+      expand_step<2, NT, AT, NS>(acc, vb, hf, hpitch, hs, j0, rows, rc, lane);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -814,7 +837,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
       YRows<2, Y32> y;
 #pragma unroll
       for (int e = 0; e < 2; ++e) y.put(e, smem + (8 * (j0 + j) + 2 * t + e) * C::YPITCH + c * (Y32 ? 4 : 2));
-      finish_rows<2, Y32>(p, tok, rows, n, j0 + j, t, acc[j], y);
+      finish_rows<2, Y32, O32>(p, tok, rows, n, j0 + j, t, acc[j], y);
     }
   }
 }
@@ -964,9 +987,9 @@ static int launch(const void* kern, int grid, int block, size_t smem, cudaStream
   return set_cuda_error(cudaLaunchKernelExC(&cfg, kern, args), what);
 }
 
-template <int MT, int AT, bool VEC, bool Y32>
+template <int MT, int AT, bool VEC, bool Y32, bool O32>
 static int direct_launch(LoraParams& p, cudaStream_t s, bool pdl) {
-  const void* kern = reinterpret_cast<const void*>(aipu_lora_kernel<MT, AT, VEC, Y32>);
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_kernel<MT, AT, VEC, Y32, O32>);
   static bool attr[64] = {false};
   const int rc = set_smem_attr_once(kern, LoraCfg<MT>::TOTAL, attr, "cudaFuncSetAttribute(lora)");
   if (rc) return rc;
@@ -975,14 +998,15 @@ static int direct_launch(LoraParams& p, cudaStream_t s, bool pdl) {
   const int tiles = std::min(p.M, p.M / kDirectTile + std::min(p.L + 1, p.M));
   return launch(kern, tiles * kDirectCtas, kLoraThreads, LoraCfg<MT>::TOTAL, s, pdl, args, "aipu_lora_kernel");
 }
+template <int MT, int AT, bool VEC>
+static int direct_launch_y(LoraParams& p, cudaStream_t s, bool pdl) {
+  if (!p.y_f32) return direct_launch<MT, AT, VEC, false, false>(p, s, pdl);
+  return p.out_f32 ? direct_launch<MT, AT, VEC, true, true>(p, s, pdl) : direct_launch<MT, AT, VEC, true, false>(p, s, pdl);
+}
 template <int MT>
 static int direct_launch_t(LoraParams& p, bool vec, cudaStream_t s, bool pdl) {
-  if (p.adtype == AD_F16) {
-    if (vec) return p.y_f32 ? direct_launch<MT, AD_F16, true, true>(p, s, pdl) : direct_launch<MT, AD_F16, true, false>(p, s, pdl);
-    return p.y_f32 ? direct_launch<MT, AD_F16, false, true>(p, s, pdl) : direct_launch<MT, AD_F16, false, false>(p, s, pdl);
-  }
-  if (vec) return p.y_f32 ? direct_launch<MT, AD_BF16, true, true>(p, s, pdl) : direct_launch<MT, AD_BF16, true, false>(p, s, pdl);
-  return p.y_f32 ? direct_launch<MT, AD_BF16, false, true>(p, s, pdl) : direct_launch<MT, AD_BF16, false, false>(p, s, pdl);
+  if (p.adtype == AD_F16) return vec ? direct_launch_y<MT, AD_F16, true>(p, s, pdl) : direct_launch_y<MT, AD_F16, false>(p, s, pdl);
+  return vec ? direct_launch_y<MT, AD_BF16, true>(p, s, pdl) : direct_launch_y<MT, AD_BF16, false>(p, s, pdl);
 }
 
 template <int MT, int AT, bool VEC>
@@ -1002,16 +1026,22 @@ static int shrink_launch_t(LoraParams& p, bool vec, cudaStream_t s) {
   return vec ? shrink_launch<MT, AD_BF16, true>(p, s) : shrink_launch<MT, AD_BF16, false>(p, s);
 }
 
-template <int AT, bool Y32>
+template <int AT, bool Y32, bool O32>
 static int expand_launch(LoraParams& p, cudaStream_t s, bool pdl) {
-  const int smem = ExpandCfg<Y32>::YBYTES + (p.out_f32 ? 3 : 2) * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
-  const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, Y32>);
+  constexpr int pieces = O32 ? 3 : 2;
+  const int smem = ExpandCfg<Y32>::YBYTES + pieces * kTile * (32 * ((p.rp + 31) / 32) + 8) * 2;
+  const void* kern = reinterpret_cast<const void*>(aipu_lora_expand_kernel<AT, Y32, O32>);
   static bool attr[64] = {false};
-  const int rc = set_smem_attr_once(kern, ExpandCfg<Y32>::YBYTES + 3 * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
+  const int rc = set_smem_attr_once(kern, ExpandCfg<Y32>::YBYTES + pieces * kTile * 136 * 2, attr, "cudaFuncSetAttribute(lora expand)");
   if (rc) return rc;
   void* args[1] = {&p};
   return launch(kern, static_cast<int>(max_tiles(p.M, p.L)) * p.nsplit, kLoraThreads, smem, s, pdl, args,
                 "aipu_lora_expand_kernel");
+}
+template <int AT>
+static int expand_launch_t(LoraParams& p, cudaStream_t s, bool pdl) {
+  if (!p.y_f32) return expand_launch<AT, false, false>(p, s, pdl);
+  return p.out_f32 ? expand_launch<AT, true, true>(p, s, pdl) : expand_launch<AT, true, false>(p, s, pdl);
 }
 
 // widest load (elements of 16 bits) of rows `ld` elements apart from `ptr`
@@ -1070,8 +1100,7 @@ int lora_finish(LoraParams& p, cudaStream_t s, bool pdl) {
       default: return direct_launch_t<8>(p, vec, s, pdl);
     }
   }
-  if (p.adtype == AD_F16) return p.y_f32 ? expand_launch<AD_F16, true>(p, s, pdl) : expand_launch<AD_F16, false>(p, s, pdl);
-  return p.y_f32 ? expand_launch<AD_BF16, true>(p, s, pdl) : expand_launch<AD_BF16, false>(p, s, pdl);
+  return p.adtype == AD_F16 ? expand_launch_t<AD_F16>(p, s, pdl) : expand_launch_t<AD_BF16>(p, s, pdl);
 }
 
 }  // namespace aipu
