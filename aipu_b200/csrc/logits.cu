@@ -278,58 +278,85 @@ __global__ void __launch_bounds__(T, T == 256 ? 4 : 1) aipu_logits_kernel(const 
         const int lb = lb0 + d * nw;
         if (lb >= mine) break;
         const int v0 = first(b0, lb);
-        uint32_t live = Group<F32>::inside(v0, p.V);  // tokens of the group that are finished here
-        const uint32_t ok = cur[d].ok;
+        const uint32_t in = Group<F32>::inside(v0, p.V), ok = cur[d].ok;
         float z[G];
 #pragma unroll
-        for (int j = 0; j < G; ++j) z[j] = (ok >> j & 1u) ? cur[d].get(j) : -INFINITY;
+        for (int j = 0; j < G; ++j) z[j] = cur[d].get(j);
+        if (ok != kAll) {
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+            if (!(ok >> j & 1u)) z[j] = -INFINITY;
+        }
         if (out) {
-          if (live == kAll && ovec) {
+          if (in == kAll && ovec) {
 #pragma unroll
             for (int j = 0; j < G; j += 4) *reinterpret_cast<float4*>(out + v0 + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
           } else {
 #pragma unroll
             for (int j = 0; j < G; ++j)
-              if (live >> j & 1u) out[v0 + j] = z[j];
+              if (in >> j & 1u) out[v0 + j] = z[j];
           }
         }
         if (penal || some) {
+          // the group's fields: two of 16 bits a word, or one of 32
+          uint32_t w[G];
           const uint32_t* f = cnt + (lb * 32 + lane) * (wide ? G : G / 2);
+          if (wide) {
+#pragma unroll
+            for (int j = 0; j < G; j += 4) {
+              const uint4 c = *reinterpret_cast<const uint4*>(f + j);
+              w[j] = c.x; w[j + 1] = c.y; w[j + 2] = c.z; w[j + 3] = c.w;
+            }
+          } else {
+            uint32_t h[G / 2];
+            if constexpr (F32) {
+              const uint2 c = *reinterpret_cast<const uint2*>(f);
+              h[0] = c.x; h[1] = c.y;
+            } else {
+              const uint4 c = *reinterpret_cast<const uint4*>(f);
+              h[0] = c.x; h[1] = c.y; h[G / 2 - 2] = c.z; h[G / 2 - 1] = c.w;
+            }
+#pragma unroll
+            for (int j = 0; j < G; ++j) w[j] = (j & 1) ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu;
+          }
           uint32_t any = 0;
 #pragma unroll
-          for (int j = 0; j < G / 2; ++j) any |= f[j];
-          if (wide)
-#pragma unroll
-            for (int j = G / 2; j < G; ++j) any |= f[j];
+          for (int j = 0; j < G; ++j) any |= w[j];
           if (any) {
+            // finished one by one, or (with a bias) after the pass; masked ones and those past the row are finished
             uint32_t todo = 0;
+            float keep[G];
 #pragma unroll
-            for (int j = 0; j < G; ++j)
-              todo |= static_cast<uint32_t>((wide ? f[j] : f[j >> 1] & (0xFFFFu << (16 * (j & 1)))) != 0) << j;
-            live &= ~todo;
-            todo &= ok;  // (masked ones are finished)
+            for (int j = 0; j < G; ++j) {
+              keep[j] = z[j];
+              if (w[j]) {
+                todo |= (w[j] & biased) ? 0u : 1u << j;
+                z[j] = -INFINITY;
+              }
+            }
+            todo &= ok;
 #pragma unroll 1
             while (todo) {
               const int j = __ffs(todo) - 1;
               todo &= todo - 1;
-              const uint32_t n = wide ? f[j] : f[j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
-              if (n & biased) continue;
-              float v = z[0];
+              float v = keep[0];
 #pragma unroll
-              for (int i = 1; i < G; ++i) v = i == j ? z[i] : v;
-              v = penalise(v, n & (biased - 1), pen);
+              for (int i = 1; i < G; ++i) v = i == j ? keep[i] : v;
+              const uint32_t n = (wide ? f[j] : f[j >> 1] >> (16 * (j & 1)) & 0xFFFFu) & (biased - 1);
+              v = penalise(v, n, pen);
               take(best, v, v0 + j);
               if (out) out[v0 + j] = v;
             }
           }
         }
-        float top = -INFINITY;  // (the larger of a number and NaN is the number)
+        // (the larger of a number and NaN is the number; what is outside the row is -inf)
+        float top = z[0];
 #pragma unroll
-        for (int j = 0; j < G; ++j) top = fmaxf(top, (live >> j & 1u) ? z[j] : -INFINITY);
+        for (int j = 1; j < G; ++j) top = fmaxf(top, z[j]);
         if (top >= best.z && top > -INFINITY) {
 #pragma unroll
           for (int j = G - 1; j >= 0; --j)
-            if ((live >> j & 1u) && z[j] == top) take(best, top, v0 + j);
+            if (z[j] == top) take(best, top, v0 + j);
         }
       }
 #pragma unroll
