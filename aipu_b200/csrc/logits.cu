@@ -19,9 +19,9 @@
 // neighbours, and their counting should not fall to one CTA). The counts of a CTA's blocks are built in its
 // shared memory from the row's context, which each CTA scans whole (from L2 after the first): no table of
 // counts in global memory, nothing to reset or to keep from call to call, and rows may share a context (the
-// rows of a verify pass do). (Sharing the scan out and counting by atomics in distributed shared memory was
-// slower from 400 tokens to 8000: a remote atomic costs more than the seven compares it saves.) Integer
-// atomics only, so the order changes nothing.
+// rows of a verify pass do). (Sharing the scan out and counting by atomics in distributed shared memory was no
+// faster: 64 rows with contexts of 4000 to 8000 tokens 34.5 us against 32.4. A remote atomic costs about what the
+// compares that it saves do.) Integer atomics only, so the order changes nothing.
 // The tokens that a penalty changes are few among the vocabulary: the pass over it stores a lane's tokens as
 // they are and then finishes those with a count one by one (a branch for each would be taken by most warps
 // for the sake of a lane). Tokens with a bias are finished by the entries of the bias list after that.

@@ -18,11 +18,12 @@
 //   3. CTA c and its warps each take 64-column blocks of N. The MMA's rows are columns of y, ordered so
 //      that a lane ends with 8 consecutive columns of a row: y is read and written 16 bytes at a time.
 //   h never leaves the chip, and the reads of B and y do not wait for the sums of A.
-//   (4096 x 4096, device time in a graph: 1 row of rank 16 7.6 us, 128 rows on eight adapters 9.1 us.)
+//   (4096 x 4096, device time in a graph: 1 row of rank 16 5.8 us, 64 rows of 32 adapters of rank 16 to 64 9.2 us.)
 // More rows: a plan (rows ordered by adapter, tiles of up to 64 of them), the first product (a tile and a
 // share of K a CTA: x and A stream through a ring of asynchronous copies in shared memory, partial sums to
-// global memory), the second product (a tile and a share of N a CTA: step 3 above). As one cluster kernel
-// this took 119 us for 4096 rows, because its phases followed one another with one CTA an SM.
+// global memory), the second product (a tile and a share of N a CTA: step 3 above, 32 columns a warp). 4096 rows of
+// eight adapters of rank 32, 6144 x 2048: 33 us, 88 MB at 2.7 TB/s; as one cluster kernel 119 us, because its
+// phases followed one another with one CTA an SM.
 //
 // Rounding: bf16 x and A products are exact in the MMA, sums are fp32. h is not rounded to 16 bits: it
 // enters the second product as 2 (bf16 result) or 3 (fp32 result) bf16 pieces, 16 and 24 bits. fp16
@@ -956,11 +957,11 @@ static int k_split(int64_t M, int64_t L) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 296 / tiles)));
 }
 
-// The one launch: up to 256 rows, whose adapters it reads once for every 8 rows. 4096 x 4096, rank 16 / 64, eight
-// adapters: 128 rows 9.1 / 12.6 us against 10.4 / 14.2 us with the plan, one adapter 9.0 / 12.4 against 17.1 / 35.1
-// (the tiles are few), 256 rows on 64 adapters 23 / 30 against 24 / 30. Ranks above 64 leave one CTA an SM: as long as
-// all tiles fit at once (64 rows on eight adapters of rank 128 17 us; 96 rows 32 against 21.5 with the plan, 64 rows on
-// 64 adapters 113 against 58). 16 rows or fewer always go this way.
+// The one launch: up to 256 rows, whose adapters it reads once for every 8 rows. 4096 x 4096 in us, against the plan: rank
+// 16, 128 rows on 1 / 8 / 64 adapters 7.6 / 7.5 / 15.6 (17.1 / 12.9 / 25.7), 256 rows 9.5 / 11.4 / 19.8 (17.2 / 14.4 / 26.2);
+// rank 64, 256 rows 12.5 / 13.7 / 24.5 (22.4 / 17.6 / 32.2). Ranks above 64 leave one CTA an SM: as long as all tiles fit
+// at once (rank 128, 64 rows on eight adapters 11.5 (17.8); 64 rows on 64 adapters took twice the plan's time). 16 rows
+// or fewer always go this way.
 static bool lora_direct(int64_t M, int64_t L, int64_t R) {
   return M <= kDirectRows && (R <= 64 || M / kDirectTile + std::min<int64_t>(L + 1, M) <= 148 / kDirectCtas);
 }

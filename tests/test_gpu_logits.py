@@ -274,6 +274,29 @@ def test_captured_replayed_two_streams_and_equal_bits():
         assert np.array_equal(out.cpu().numpy(), z) and np.array_equal(tok.cpu().numpy(), t)
 
 
+def test_penalties_of_every_kind():
+    """Zero, negative, infinite and NaN penalties act as the steps say."""
+    d = _dev()
+    rng = np.random.default_rng(4)
+    vals = [0.0, -1.5, np.inf, -np.inf, np.nan, 1.0, 1e-38, 3e38]
+    pen = np.array([[a, b, c] for a in vals for b in (0.0, np.inf, -2.0) for c in (0.0, np.nan, 1e30)], F32)
+    M, V = len(pen), 90
+    x, x_np = _logits(rng, M, V, torch.float32, d)
+    x[:, 7], x_np[:, 7] = 0.0, 0.0
+    tokens = rng.integers(0, V // 2, M * 20).astype(np.int32)
+    at = 20 * np.arange(M)
+    c = dict(tokens=tokens, spans=np.stack([at, at + 8, at + 20], 1).astype(np.int64), penalties=pen)
+    out, tok = ops.process_logits(x, _dev_controls(c, d))
+    with np.errstate(all="ignore"):
+        z, t = oracle(x_np, **c)
+    np.testing.assert_array_equal(out.cpu().numpy(), z)
+    np.testing.assert_array_equal(tok.cpu().numpy(), t)
+
+
+def test_thousands_of_rows():
+    _run(3000, 130, history=40, bias=3, masks=7)
+
+
 def test_no_rows():
     d = _dev()
     out, tok = ops.process_logits(torch.empty((0, 10), device=d))

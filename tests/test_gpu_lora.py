@@ -198,6 +198,18 @@ def test_up_to_16_rows_do_not_depend_on_what_shares_the_call():
             assert torch.equal(ops.lora_add(A, ids[m:m + 1], x[m:m + 1], y[m:m + 1]), o[m:m + 1])
 
 
+@pytest.mark.parametrize("M,L", [(20, 32768), (300, 32768), (5000, 3), (70001, 40)])
+def test_many_adapters_and_many_rows(M, L):
+    A, ids, x = _case(M, 16, 8, 1, L)
+    y = torch.randn((M, 8), device=x.device)
+    i = ids.long().clamp_min(0)
+    h = (x.double() * A.a.double()[i, 0]).sum(1, keepdim=True)
+    size = (x.double() * A.a.double()[i, 0]).abs().sum(1, keepdim=True)
+    f = torch.where(ids >= 0, A.scale.double()[i], 0.0).view(M, 1)
+    b = A.b.double()[i, :, 0]
+    _check(ops.lora_add(A, ids, x, y), y.double().cpu(), (f * h * b).cpu(), (f * size * b.abs()).cpu(), 16)
+
+
 def test_no_rows():
     A, _, x = _case(2, 64, 32, 4, 1)
     e = torch.empty((0,), dtype=torch.int32, device=x.device)
@@ -361,10 +373,11 @@ def test_two_streams_at_once():
     assert all(torch.equal(o, want) for o in outs)
 
 
-def test_programmatic_launch_flag_keeps_the_results():
-    A, ids, x = _case(20, 512, 256, 16, 4)
+@pytest.mark.parametrize("M", [20, 300])
+def test_programmatic_launch_flag_keeps_the_results(M):
+    A, ids, x = _case(M, 512, 256, 16, 4)
     ctx = ops.Context(x.device).set_flags(pdl=True)
-    y = torch.randn((20, 256), device=x.device)
+    y = torch.randn((M, 256), device=x.device)
     want = ops.lora_add(A, ids, x, y + 0)
     for _ in range(20):
         z = y + 0  # a kernel right before, whose output is read
