@@ -270,7 +270,7 @@ __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok,
     }
     if (O32) {
       float* op = static_cast<float*>(p.out) + row * p.ldo + n;
-      if (p.vo && cols >= C) {
+      if (p.vo == 2 && cols >= C) {
 #pragma unroll
         for (int i = 0; i < C; i += 4) *reinterpret_cast<float4*>(op + i) = make_float4(d[i], d[i + 1], d[i + 2], d[i + 3]);
       } else {
@@ -283,9 +283,12 @@ __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok,
       uint32_t o[Q];
 #pragma unroll
       for (int i = 0; i < Q; ++i) o[i] = pack_bf16(d[2 * i], d[2 * i + 1]);
-      if (p.vo && cols >= C) {
+      if (p.vo == 2 && cols >= C) {
         if constexpr (Q == 2) *reinterpret_cast<uint2*>(op) = make_uint2(o[0], o[1]);
         else *reinterpret_cast<uint4*>(op) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else if (p.vo == 1 && cols >= C) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) reinterpret_cast<uint32_t*>(op)[i] = o[i];
       } else {
 #pragma unroll
         for (int i = 0; i < C; ++i)
@@ -389,7 +392,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int id, int r
 }
 
 template <int MT, int AT, bool VEC, bool Y32, bool O32>
-__global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads, 2) aipu_lora_kernel(const __grid_constant__ LoraParams p) {
   using C = LoraCfg<MT>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int tok[C::TM];
@@ -957,17 +960,14 @@ static int k_split(int64_t M, int64_t L) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 296 / tiles)));
 }
 
-// The one launch: up to 256 rows, whose adapters it reads once for every 8 rows. 4096 x 4096 in us, against the plan: rank
-// 16, 128 rows on 1 / 8 / 64 adapters 7.6 / 7.5 / 15.6 (17.1 / 12.9 / 25.7), 256 rows 9.5 / 11.4 / 19.8 (17.2 / 14.4 / 26.2);
-// rank 64, 256 rows 12.5 / 13.7 / 24.5 (22.4 / 17.6 / 32.2). Ranks above 64 leave one CTA an SM: as long as all tiles fit
-// at once (rank 128, 64 rows on eight adapters 11.5 (17.8); 64 rows on 64 adapters took twice the plan's time). 16 rows
-// or fewer always go this way.
-static bool lora_direct(int64_t M, int64_t L, int64_t R) {
-  return M <= kDirectRows && (R <= 64 || M / kDirectTile + std::min<int64_t>(L + 1, M) <= 148 / kDirectCtas);
-}
+// The one launch: up to 256 rows (a thread each finds the tiles), whose adapters it reads once for every 8 rows.
+// 4096 x 4096 in us, against the plan: rank 16, 128 rows on 1 / 8 / 64 adapters 7.6 / 7.5 / 15.6 (17.1 / 12.9 / 25.7), 256
+// rows 9.5 / 11.4 / 19.8 (17.2 / 14.4 / 26.2); rank 64, 256 rows 12.5 / 13.7 / 24.5 (22.4 / 17.6 / 32.2); rank 128, 256 rows
+// 17.0 / 17.9 / 42 (32.6 / 24.7 / 51), fp16 with fp32 results 29 / 29 / 64 (50 / 40 / 140).
+static bool lora_direct(int64_t M) { return M <= kDirectRows; }
 
 size_t lora_plan_bytes(int64_t M, int64_t L, int64_t R) {
-  if (lora_direct(M, L, R)) return 0;
+  if (lora_direct(M)) return 0;
   return 256 + al256l(4 * M) + al256l(16 * max_tiles(M, L)) +
          al256l(static_cast<size_t>(4) * M * padded_rank(R) * k_split(M, L));
 }
@@ -1065,9 +1065,9 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * esz % 16 == 0;
   };
   p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2);
-  p.vo = rows16(p.out, p.ldo, p.out_f32 ? 4 : 2);
+  p.vo = rows16(p.out, p.ldo, p.out_f32 ? 4 : 2) ? 2 : (!p.out_f32 && load_width(p.out, p.ldo) >= 2) ? 1 : 0;
   p.tiles = nullptr;
-  if (lora_direct(p.M, p.L, p.R)) return OK;
+  if (lora_direct(p.M)) return OK;
   uint8_t* b = static_cast<uint8_t*>(plan);
   p.n_tiles = reinterpret_cast<int32_t*>(b);
   p.perm = reinterpret_cast<int32_t*>(b + 256);

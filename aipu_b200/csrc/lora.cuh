@@ -34,7 +34,7 @@ struct LoraParams {
   int rp;                // padded rank: 16, 32, 64 or 128
   int skip_plain;        // 1: in-place, rows without an adapter are not touched
   int wa, wx, wb;        // widest aligned load of A rows, x rows, B rows (elements: 8, 2 or 1)
-  int vy, vo;            // 1: 16-byte loads of y, stores of out
+  int vy, vo;            // 1: 16-byte loads of y; 2: 16-byte stores of out, 1: 4-byte stores
 };
 
 // bytes of the scratch of M rows (0 when the one launch takes them)

@@ -20,7 +20,7 @@ rows share the pass (M = K + 1 rows give the same bits as K + 1 single-row passe
 A Request carries what one request asks of its tokens: its adapter on the LM head (ops.lora_add), and
 penalties, biases and a mask on the logits before the argmax (ops.greedy_tokens). Row j of a pass is
 then judged by the request's context with the drafts before it, so the committed stream equals greedy
-decoding under the same controls (the adapter's bits are those of a single row in passes of up to 16).
+decoding under the same controls (the adapter's bits are those of a single row in passes of up to 256).
 """
 from __future__ import annotations
 

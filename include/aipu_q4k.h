@@ -280,7 +280,8 @@ typedef struct aipu_lora {
  * columns of a wider tensor can be passed.
  * ws: device scratch of aipu_lora_workspace(M, n_adapters, rank) bytes (NULL when that is 0), in use until
  * the call's work on `stream` is done. Nothing else is shared, so calls with their own ws may run at the
- * same time. Equal calls give equal bits. No counterpart in the reference. */
+ * same time. Equal calls give equal bits; in calls of up to 256 rows a row's bits do not depend on the other
+ * rows. No counterpart in the reference. */
 int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
                   const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,

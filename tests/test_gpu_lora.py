@@ -189,12 +189,12 @@ def test_equal_calls_give_equal_bits_whatever_shares_the_batch():
         assert torch.equal(ops.lora_add(A, ids, x, y), o)
 
 
-def test_up_to_16_rows_do_not_depend_on_what_shares_the_call():
+def test_up_to_256_rows_do_not_depend_on_what_shares_the_call():
     for R in (16, 100):
-        A, ids, x = _case(16, 512, 300, R, 9)
-        y = torch.randn((16, 300), device=x.device)
+        A, ids, x = _case(256, 512, 300, R, 9)
+        y = torch.randn((256, 300), device=x.device)
         o = ops.lora_add(A, ids, x, y)
-        for m in range(16):
+        for m in range(0, 256, 7):
             assert torch.equal(ops.lora_add(A, ids[m:m + 1], x[m:m + 1], y[m:m + 1]), o[m:m + 1])
 
 
