@@ -1422,6 +1422,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   p.ldx = K;
   p.y = y32;
   p.ldy = gemm_lora_ld(N);
+  p.y_cols = static_cast<int>(p.ldy);
   p.ldo = N;
   p.out = y;
   p.y_f32 = 1;

@@ -335,9 +335,10 @@ static int dense_launch(DenseParams& p, int parts, cudaStream_t s) {
 static int token_tile(int64_t M) { return M <= 64 ? 64 : M <= 128 ? 128 : 256; }
 
 int dense_parts(int64_t N, int64_t K, int64_t M) {
-  // as many shares of K (of four steps at least) as still leave a CTA an SM (148)
+  // As many shares of K as still leave a CTA an SM (148), of four steps of 64 at least; of sixteen where there are rows
+  // enough for the plan (256), whose last kernel pays more for adding shares than a short GEMM gains.
   const int64_t tiles = ((N + 127) / 128) * ((M + token_tile(M) - 1) / token_tile(M));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / 256), 148 / tiles)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / (M > 256 ? 1024 : 256)), 148 / tiles)));
 }
 
 template <int WT>

@@ -212,24 +212,34 @@ struct YRows {
   }
   // rows 8 j + 2 t (+ 1) of the tile from global memory, columns n on (where whole 16-byte pieces may be read)
   __device__ __forceinline__ void load(const LoraParams& p, const int* tok, int rows, int n, int j, int t) {
-    if (!p.vy || n + 2 * Q > p.N) return;
+    if (n + 2 * Q > p.vy) return;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int m = 8 * j + 2 * t + e;
       if (m >= rows) continue;
       put(e, static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2));
-      if (Y32)
-        for (int s = 1; s < p.yparts; ++s) {
-          const float* o = static_cast<const float*>(p.y) + (static_cast<int64_t>(s) * p.M + tok[m]) * p.ldy + n;
+      if (Y32 && p.yparts > 1) {
+        const float* o = static_cast<const float*>(p.y) + static_cast<int64_t>(tok[m]) * p.ldy + n;
+        const int64_t share = static_cast<int64_t>(p.M) * p.ldy;
+        for (int s = 1; s < p.yparts; s += 4) {  // the loads of four shares are in flight together
+          float4 v[4][W / 4];
 #pragma unroll
-          for (int i = 0; i < W; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(o + i);
-            w[e][i] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i]), v.x));
-            w[e][i + 1] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 1]), v.y));
-            w[e][i + 2] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 2]), v.z));
-            w[e][i + 3] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][i + 3]), v.w));
+          for (int u = 0; u < 4; ++u)
+            if (s + u < p.yparts)
+#pragma unroll
+              for (int i = 0; i < W / 4; ++i) v[u][i] = *reinterpret_cast<const float4*>(o + (s + u) * share + 4 * i);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (s + u >= p.yparts) break;
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) {
+              const float d[4] = {v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[e][4 * i + k] = __float_as_uint(__fadd_rn(__uint_as_float(w[e][4 * i + k]), d[k]));
+            }
           }
         }
+      }
     }
   }
   __device__ __forceinline__ float get(int e, int i) const {
@@ -238,10 +248,10 @@ struct YRows {
   }
 };
 
-// out rows 8 j + 2 t (+ 1) of the tile, columns n on: y + acc, rounded once
+// out rows 8 j + 2 t (+ 1) of the tile, columns n on: y + acc, rounded once (y: loaded, or read here a column at a time)
 template <int Q, bool Y32, bool O32>
 __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok, int rows, int n, int j, int t,
-                                            const float (&acc)[Q][4], const YRows<Q, Y32>& y) {
+                                            const float (&acc)[Q][4], const YRows<Q, Y32>& y, bool loaded) {
   constexpr int C = 2 * Q;
   const int cols = p.N - n;
   if (cols <= 0) return;
@@ -253,19 +263,16 @@ __device__ __forceinline__ void finish_rows(const LoraParams& p, const int* tok,
     float d[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) d[i] = acc[i >> 1][e + 2 * (i & 1)];
-    if (p.vy && cols >= C) {
+    if (loaded) {
 #pragma unroll
       for (int i = 0; i < C; ++i) d[i] = __fadd_rn(y.get(e, i), d[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         if (i >= cols) break;
-        float v = Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
-                      : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]);
-        if (Y32)
-          for (int s = 1; s < p.yparts; ++s)
-            v = __fadd_rn(v, static_cast<const float*>(p.y)[(static_cast<int64_t>(s) * p.M + row) * p.ldy + n + i]);
-        d[i] = __fadd_rn(v, d[i]);
+        d[i] = __fadd_rn(Y32 ? static_cast<const float*>(p.y)[row * p.ldy + n + i]
+                             : bf16_bits_to_f32(static_cast<const uint16_t*>(p.y)[row * p.ldy + n + i]),
+                         d[i]);
       }
     }
     if (O32) {
@@ -538,7 +545,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads, 2)
       if (nb != gw || rc != 0) load_b<4>(p, tl, nb * 64 + c8, 32 * rc + 8 * t, vb);
       expand_step<4, 1, AT, NS>(acc, vb, hf, C::HPITCH, HS, 0, tl.rows, rc, lane);
     }
-    finish_rows<4, Y32, O32>(p, tok, tl.rows, nb * 64 + c8, 0, t, acc[0], yt);
+    finish_rows<4, Y32, O32>(p, tok, tl.rows, nb * 64 + c8, 0, t, acc[0], yt, nb * 64 + c8 + 8 <= p.vy);
   }
   pdl_launch_dependents();
   if (pending) cluster_wait();
@@ -759,24 +766,59 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
   const int j0 = halves && warp >= kLoraWarps / 2 ? NT / 2 : 0;
   const int rows = halves && warp < kLoraWarps / 2 ? kTile / 2 : tl.rows;
   auto load_y = [&]() {
-    if (p.vy) {  // 16 bytes a copy, whole rows of the tile
-      constexpr int per = C::COLS * (Y32 ? 4 : 2) / 16, each = Y32 ? 4 : 8;
-      for (int i = tid; i < tl.rows * per; i += kLoraThreads) {
-        const int m = i / per, n = col0 + (i % per) * each;
-        if (n + each > p.N) continue;
-        uint8_t* dst = smem + m * C::YPITCH + (i % per) * 16;
-        const uint8_t* src = static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[m]) * p.ldy + n) * (Y32 ? 4 : 2);
-        if (Y32 && p.yparts > 1) {
-          float4 v = *reinterpret_cast<const float4*>(src);
-#pragma unroll 4
-          for (int s = 1; s < p.yparts; ++s) {
-            const float4 o = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * p.M * p.ldy * 4);
-            v = make_float4(__fadd_rn(v.x, o.x), __fadd_rn(v.y, o.y), __fadd_rn(v.z, o.z), __fadd_rn(v.w, o.w));
+    constexpr int each = Y32 ? 4 : 8, esz = Y32 ? 4 : 2;  // columns of a 16-byte piece
+    const int cols = min(C::COLS, p.N - col0);
+    // columns read in whole pieces (all of them where the rows are padded), and the pieces of a row, as a power of two
+    const int whole = min((cols + each - 1) / each * each, max(0, p.vy - col0) / each * each);
+    const int lg = whole > each ? 32 - __clz(whole / each - 1) : 0, per = 1 << lg;
+    const int pieces = whole > 0 ? tl.rows << lg : 0;
+    auto at = [&](int i) { return (i & (per - 1)) * each; };
+    auto source = [&](int i) {
+      return static_cast<const uint8_t*>(p.y) + (static_cast<int64_t>(tok[i >> lg]) * p.ldy + col0 + at(i)) * esz;
+    };
+    auto place = [&](int i) { return smem + (i >> lg) * C::YPITCH + at(i) * esz; };
+    if (Y32 && p.yparts > 1) {
+      const int64_t share = static_cast<int64_t>(p.M) * p.ldy;
+      for (int i0 = tid; i0 < pieces; i0 += 2 * kLoraThreads) {
+        float4 sum[2];
+        for (int s0 = 0; s0 < p.yparts; s0 += 4) {  // the loads of four shares of two pieces are in flight together
+          float4 v[2][4];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * kLoraThreads;
+            const bool in = i < pieces && at(i) < whole;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              if (in && s0 + s < p.yparts) v[u][s] = *reinterpret_cast<const float4*>(source(i) + 4 * (s0 + s) * share);
           }
-          *reinterpret_cast<float4*>(dst) = v;
-        } else {
-          cp_async16(smem_u32(dst), src, 16);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              if (s0 + s >= p.yparts) break;
+              const float4 o = v[u][s];
+              sum[u] = s0 + s == 0 ? o
+                                   : make_float4(__fadd_rn(sum[u].x, o.x), __fadd_rn(sum[u].y, o.y), __fadd_rn(sum[u].z, o.z),
+                                                 __fadd_rn(sum[u].w, o.w));
+            }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * kLoraThreads;
+          if (i < pieces && at(i) < whole) *reinterpret_cast<float4*>(place(i)) = sum[u];
+        }
+      }
+    } else {
+      for (int i = tid; i < pieces; i += kLoraThreads)
+        if (at(i) < whole) cp_async16(smem_u32(place(i)), source(i), 16);
+      // the other columns one at a time, neighbours on neighbouring threads
+      const int left = max(0, cols - whole);
+#pragma unroll 4
+      for (int i = tid; i < tl.rows * left; i += kLoraThreads) {
+        const int m = i / left, c = whole + i - m * left;
+        const int64_t from = static_cast<int64_t>(tok[m]) * p.ldy + col0 + c;
+        if (Y32) *reinterpret_cast<uint32_t*>(smem + m * C::YPITCH + 4 * c) = static_cast<const uint32_t*>(p.y)[from];
+        else *reinterpret_cast<uint16_t*>(smem + m * C::YPITCH + 2 * c) = static_cast<const uint16_t*>(p.y)[from];
       }
     }
     cp_commit();
@@ -841,7 +883,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) aipu_lora_expand_kernel(const
       YRows<2, Y32> y;
 #pragma unroll
       for (int e = 0; e < 2; ++e) y.put(e, smem + (8 * (j0 + j) + 2 * t + e) * C::YPITCH + c * (Y32 ? 4 : 2));
-      finish_rows<2, Y32, O32>(p, tok, rows, n, j0 + j, t, acc[j], y);
+      finish_rows<2, Y32, O32>(p, tok, rows, n, j0 + j, t, acc[j], y, true);
     }
   }
 }
@@ -1064,7 +1106,7 @@ int lora_begin(LoraParams& p, void* plan, cudaStream_t s, bool pdl) {
   auto rows16 = [](const void* q, int64_t ld, int esz) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * esz % 16 == 0;
   };
-  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2);
+  p.vy = rows16(p.y, p.ldy, p.y_f32 ? 4 : 2) ? (p.y_cols ? p.y_cols : p.N) : 0;
   p.vo = rows16(p.out, p.ldo, p.out_f32 ? 4 : 2) ? 2 : (!p.out_f32 && load_width(p.out, p.ldo) >= 2) ? 1 : 0;
   p.tiles = nullptr;
   if (lora_direct(p.M)) return OK;

@@ -22,7 +22,8 @@ struct LoraParams {
   void* out;             // bf16, or fp32 when y is
   int64_t ldo;
   int y_f32, out_f32;
-  int yparts;            // shares of fp32 y to be summed, M * ldy elements apart (0: one)
+  int yparts;            // shares of fp32 y to be summed, M * ldy elements apart (0: one; more need aligned, padded rows)
+  int y_cols;            // columns of y that may be read (0: N; more where its rows are padded)
   int* status;           // device status word (nullable)
   int wait_y;            // 1: y comes from the kernel launched just before lora_finish's (programmatic launch)
   // set by lora_begin
@@ -34,7 +35,8 @@ struct LoraParams {
   int rp;                // padded rank: 16, 32, 64 or 128
   int skip_plain;        // 1: in-place, rows without an adapter are not touched
   int wa, wx, wb;        // widest aligned load of A rows, x rows, B rows (elements: 8, 2 or 1)
-  int vy, vo;            // 1: 16-byte loads of y; 2: 16-byte stores of out, 1: 4-byte stores
+  int vy;                // columns of y that may be read in 16-byte pieces (0: rows not aligned)
+  int vo;                // 2: 16-byte stores of out, 1: 4-byte stores
 };
 
 // bytes of the scratch of M rows (0 when the one launch takes them)
