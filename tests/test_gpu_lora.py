@@ -219,6 +219,22 @@ def test_no_rows():
     assert ops.gemm_lora(F.Q4_K, w, 32, 256, x[:0], A, e).shape == (0, 32)
 
 
+@pytest.mark.parametrize("M", [6, 150, 300])
+@pytest.mark.parametrize("N", [1, 71, 259, 515])
+@pytest.mark.parametrize("t", [BF, FP])
+def test_odd_widths_in_aligned_rows(M, N, t):
+    """Rows that begin on 16 bytes and end inside a 16-byte piece: the columns behind them are neither read nor written."""
+    A, ids, x = _case(M, 128, N, 8, 2)
+    wide = torch.full((M, 520), float("nan"), dtype=t, device=x.device)
+    y = wide[:, :N]
+    y.copy_(torch.randn((M, N), device=x.device))
+    y64 = y.double().cpu()
+    d, s = _delta(A, ids, x)
+    ops.lora_add(A, ids, x, y, out=y)
+    _check(y, y64, d, s, 128)
+    assert wide[:, N:].isnan().all()
+
+
 @pytest.mark.parametrize("wt", [F.Q4_K, F.Q6_K, F.Q8_0, F.F16])
 @pytest.mark.parametrize("M,K,N,R", [(1, 1024, 512, 16), (1, 256, 1, 1), (2, 512, 100, 8), (8, 2048, 260, 32), (11, 768, 130, 5),
                                      (63, 512, 96, 16), (64, 512, 96, 16), (150, 1024, 333, 64)])
@@ -263,7 +279,7 @@ def test_gemm_lora_without_adapters_is_the_projection():
 
 @pytest.mark.parametrize("wt", [F.Q4_K, F.Q6_K, F.Q8_0, F.F16])
 @pytest.mark.parametrize("M,K,N", [(9, 256, 1), (64, 2048, 128), (65, 256, 129), (128, 512, 127), (129, 768, 300), (256, 512, 256),
-                                   (257, 256, 640), (700, 2304, 520)])
+                                   (257, 256, 640), (700, 2304, 520), (300, 5120, 5), (257, 8192, 259), (290, 2048, 1003)])
 def test_gemm_lora_many_rows_at_tile_borders(wt, M, K, N):
     """Weights of the extremes too: scales of zero, of fp16's smallest and of its largest numbers, in some rows."""
     A, ids, x = _case(M, K, N, 8, 2)
