@@ -335,10 +335,13 @@ static int dense_launch(DenseParams& p, int parts, cudaStream_t s) {
 static int token_tile(int64_t M) { return M <= 64 ? 64 : M <= 128 ? 128 : 256; }
 
 int dense_parts(int64_t N, int64_t K, int64_t M) {
-  // As many shares of K as still leave a CTA an SM (148), of four steps of 64 at least; of sixteen where there are rows
-  // enough for the plan (256), whose last kernel pays more for adding shares than a short GEMM gains.
+  // As many shares of K as still leave a CTA an SM (148), of eight steps of 64 at least; of sixteen above 256 rows, where
+  // the last kernel pays more for adding shares than a short GEMM gains. F16 in us, a call, shares of at least 4 / 8 / 16 /
+  // 32 steps: 300 rows, 512 x 1024 29.3 / 29.4 / 26.4 / 26.4, 1003 x 4096 46.5 / 46.5 / 37.2 / 40.8, 2048 x 6144 41.8 / 41.5 /
+  // 41.5 / 44.1. Fewer rows, 4 / 8 steps: 64 rows of 1024 x 2048 14.9 / 12.0, 256 rows of 512 x 1024 19.7 / 16.0, but 64
+  // rows of 64 x 1024 10.1 / 11.1.
   const int64_t tiles = ((N + 127) / 128) * ((M + token_tile(M) - 1) / token_tile(M));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / (M > 256 ? 1024 : 256)), 148 / tiles)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / (M > 256 ? 1024 : 512)), 148 / tiles)));
 }
 
 template <int WT>

@@ -730,7 +730,11 @@ __global__ void __launch_bounds__(kLoraThreads) aipu_lora_shrink_kernel(const __
 // where there are few columns), so every value of B is read and, where it has to be, split or moved into place once. The
 // tile's part of y, its rows and its B rows do not depend on the first product: they are on their way (y by
 // asynchronous copies) while that runs, so what follows it is the sums of the shares of K in order, the MMAs and
-// the stores.
+// the stores. All of y passes through shared memory, also where its rows are not aligned or end inside 16 bytes (512 rows
+// of 1003 columns, 4 shares of y: 19 us; 67 when the last columns were read by the threads that add to them). Behind a
+// GEMM the loads of the shares are what this waits for: several pieces and shares are in flight a thread (28 tiles of
+// 502 columns, 2 shares: 18 us; 47 with one after the other). The next B is not fetched ahead: with this many
+// accumulators it spills (4096 rows of rank 128, 4096 x 4096: 84 us without, 99 with).
 template <bool Y32>
 struct ExpandCfg {
   static constexpr int COLS = Y32 ? 256 : 512;
