@@ -1321,11 +1321,15 @@ extern "C" int aipu_q4k_gemm_tc(aipu_ctx* c, int wtype, const void* w, int64_t N
 }
 
 // ------------------------------------------------------------------ low-rank adapters
+static bool off(const void* q, int bytes) { return reinterpret_cast<uintptr_t>(q) % bytes != 0; }
+
 static int lora_params(const aipu_lora* ad, const int32_t* ids, int64_t M, LoraParams& p, const char* bad) {
   if (!ad || (M > 0 && !ids) || !ad->a || !ad->b || (ad->dtype != AIPU_DT_BF16 && ad->dtype != AIPU_DT_F16) || ad->n_adapters < 1 ||
       ad->n_adapters > 32768 || ad->rank < 1 || ad->rank > 128 || ad->in_features < 1 || ad->in_features > (1 << 24) ||
       ad->out_features < 1 || ad->out_features > (1 << 24) || M < 0 || M > (1 << 24))
     return set_error(EINVAL_, bad);
+  if (off(ad->a, 2) || off(ad->b, 2) || off(ad->scale, 4) || off(ad->ranks, 4) || off(ids, 4))
+    return set_error(EINVAL_, "lora: adapters, factors, ranks or ids not aligned to their type");
   p.a = ad->a;
   p.b = ad->b;
   p.scale = ad->scale;
@@ -1355,6 +1359,8 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
   if ((y_dtype != AIPU_DT_F32 && y_dtype != AIPU_DT_BF16) || (out_dtype != AIPU_DT_F32 && out_dtype != AIPU_DT_BF16) ||
       (y_dtype == AIPU_DT_BF16 && out_dtype == AIPU_DT_F32))
     return set_error(EINVAL_, "lora_add: y and out must be bf16, fp32, or fp32 and bf16");
+  if (off(x, 2) || off(y, y_dtype == AIPU_DT_F32 ? 4 : 2) || off(out, out_dtype == AIPU_DT_F32 ? 4 : 2))
+    return set_error(EINVAL_, "lora_add: rows not aligned to their type");
   if (out && out == y && (y_dtype != out_dtype || ldy != ldo))
     return set_error(EINVAL_, "lora_add: in place needs the same type and row stride");
   const int64_t need = aipu_lora_workspace(M, p.L, p.R);
@@ -1403,8 +1409,8 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   if (!w || (M > 0 && (!x || !y)) || wtype == AIPU_F32 || aipu_row_bytes(wtype, K) == 0 || K % 256 || ad->in_features != K ||
       ad->out_features != N)
     return set_error(EINVAL_, "gemm_lora: bad arguments (GGUF rows, K % 256 == 0, adapters of the same K and N)");
-  if ((reinterpret_cast<uintptr_t>(w) & 15u) || (reinterpret_cast<uintptr_t>(x) & 15u))
-    return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned");
+  if (off(w, 16) || off(x, 16) || off(y, 2))
+    return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned, the result to its type");
   if ((M > 0 && !ws) || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L, p.R))
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
   if (!c) return set_error(EINVAL_, "gemm_lora: null context");
@@ -1462,6 +1468,8 @@ extern "C" int aipu_logits_process(aipu_ctx* c, const void* logits, int dtype, i
     return set_error(EINVAL_, "logits_process: bad shape, type or pointer");
   if (out == logits && out && (dtype != AIPU_DT_F32 || ld != ldo))
     return set_error(EINVAL_, "logits_process: in place needs fp32 logits and one row stride");
+  if (off(logits, dtype == AIPU_DT_F32 ? 4 : 2) || off(out, 4) || off(token, 4))
+    return set_error(EINVAL_, "logits_process: logits, out or token not aligned to their type");
   if (ctl) {
     if ((ctl->spans != nullptr) != (ctl->penalties != nullptr) || ctl->n_tokens < 0 || ctl->n_tokens > INT32_MAX ||
         (ctl->n_tokens > 0 && !ctl->tokens))
@@ -1470,6 +1478,9 @@ extern "C" int aipu_logits_process(aipu_ctx* c, const void* logits, int dtype, i
       return set_error(EINVAL_, "logits_process: biases need ids and values");
     if ((ctl->mask != nullptr) != (ctl->mask_rows != nullptr) || (ctl->mask && (ctl->n_masks < 1 || ctl->n_masks > INT32_MAX)))
       return set_error(EINVAL_, "logits_process: masks need mask_rows and at least one mask");
+    if (off(ctl->tokens, 4) || off(ctl->spans, 8) || off(ctl->penalties, 4) || off(ctl->bias_begin, 8) || off(ctl->bias_ids, 4) ||
+        off(ctl->bias_vals, 4) || off(ctl->mask, 4) || off(ctl->mask_rows, 4))
+      return set_error(EINVAL_, "logits_process: controls not aligned to their type");
   }
   if (!c) return set_error(EINVAL_, "logits_process: null context");
   if (M == 0) return OK;

@@ -257,7 +257,7 @@ int aipu_ep_destroy(aipu_ep* ep);
 
 /* Low-rank adapters of one projection of K inputs and N outputs: adapter l has a[l] (R rows of K),
  * b[l] (N rows of R), a factor and a rank <= R (rows of a[l] and columns of b[l] from the rank on are
- * not used, whatever they hold). All device pointers, 2-byte aligned; a, b and the x rows used with them must be
+ * not used, whatever they hold). All device pointers, aligned to their type; a, b and the x rows used with them must be
  * readable to the 16-byte boundaries around them (rows that start on such boundaries are fastest). */
 typedef struct aipu_lora {
   int32_t dtype;        /* of a and b: AIPU_DT_BF16 or AIPU_DT_F16 */
@@ -289,10 +289,11 @@ int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const 
 
 /* The quantised projection with the adapters of its rows: y[m, n] (bf16) = bf16(x[m] W^T + the adapter
  * term of aipu_lora_add); x[M, K] bf16, 16-byte aligned, W = N GGUF rows of K weights (Q4_K, Q6_K, Q8_0,
- * F16; K a multiple of 256, 16-byte aligned). The projection's fp32 sums (those of AIPU_MODE_FAST, or of
- * the tcgen05 GEMM for many rows of Q4_K / Q6_K) are not rounded before the adapter term is added.
- * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Uses the context's
- * stream-K workspace (one context per concurrently used stream). No counterpart in the reference. */
+ * F16; K a multiple of 256, 16-byte aligned); y must not overlap the inputs. The projection's fp32 sums (up to 8
+ * rows those of AIPU_MODE_FAST, above them of a tcgen05 GEMM whose weights are rounded to fp16 once) are not
+ * rounded before the adapter term is added.
+ * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Up to 8 rows use the context's
+ * stream-K workspace too (one context per concurrently used stream). No counterpart in the reference. */
 int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,
                        const aipu_lora* ad, const int32_t* ids, void* y, void* ws, int64_t ws_bytes, void* stream);
@@ -322,7 +323,8 @@ typedef struct aipu_logit_ctl {
  * logits[M, V] (bf16 or fp32, ld elements between rows). Steps, each rounded to fp32:
  *   z = z > 0 ? z / repetition : z * repetition   if the token occurs in the row's context
  *   z = z - frequency * count, z = z - presence   if it occurs count > 0 times in the generated part
- *   z = z + bias                                  every entry of the row for the token, in list order
+ *   z = z + bias                                  every entry of the row for the token, in list order (ids
+ *                                                 outside 0 .. V - 1 count for nothing)
  *   z = -inf                                      if the row's mask does not allow it
  * token = the lowest index of the largest z (NaN is never the largest), -1 if no z is above -inf (a mask
  * that leaves nothing). ctl may be NULL. out may be logits (fp32, same stride). A span or bias range that

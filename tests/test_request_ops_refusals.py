@@ -168,6 +168,30 @@ def test_c_entry_refuses_logits(kw, text):
     assert text in _lib.lib().aipu_last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(a=17), dict(b=17), dict(scale=18), dict(ranks=18)])
+def test_c_entries_refuse_adapters_off_their_types_alignment(kw):
+    L = _lib.lib()
+    assert L.aipu_lora_add(None, _lora(**kw), 16, 16, 256, 4, 16, 1, 32, 32, 1, 32, 16, 1 << 30, None) == _lib.AIPU_EINVAL
+    assert b"not aligned" in L.aipu_last_error()
+    assert L.aipu_q4k_gemm_lora(None, 0, 16, 32, 256, 16, 4, _lora(**kw), 16, 16, 256, 1 << 40, None) == _lib.AIPU_EINVAL
+    assert b"not aligned" in L.aipu_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(x=17), dict(y=17), dict(out=33), dict(y=18, ydt=0), dict(y=16, ydt=0, out=34, odt=0)])
+def test_c_entry_refuses_rows_off_their_types_alignment(kw):
+    assert _add(**kw) == _lib.AIPU_EINVAL
+    assert b"not aligned" in _lib.lib().aipu_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=65), dict(x=66, dtype=0), dict(out=130), dict(token=18), dict(ctl=_ctl(tokens=18)), dict(ctl=_ctl(spans=20)),
+    dict(ctl=_ctl(penalties=18)), dict(ctl=_ctl(bias_begin=20)), dict(ctl=_ctl(bias_ids=18)), dict(ctl=_ctl(bias_vals=17)),
+    dict(ctl=_ctl(mask=18)), dict(ctl=_ctl(mask_rows=18))])
+def test_c_entry_refuses_logits_off_their_types_alignment(kw):
+    assert _process(**kw) == _lib.AIPU_EINVAL
+    assert b"not aligned" in _lib.lib().aipu_last_error()
+
+
 def test_structs_match_the_header():
     """Field for field in the header's order (all 8-byte fields but the adapters' first two)."""
     assert ctypes.sizeof(_lib.Lora) == 8 + 7 * 8 and _lib.Lora.rank.offset == 8 and _lib.Lora.ranks.offset == 56
