@@ -417,7 +417,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads, 2)
 
   // A row leads a tile if the number of earlier rows with its id is a multiple of a tile's rows; the tile is
   // that row and the following ones of the id, and this cluster's is the one of the cluster's number.
-  __shared__ int key[kDirectRows];
+  __shared__ __align__(16) int key[kDirectRows];  // (read four at a time)
   __shared__ uint32_t lead_bits[kDirectRows / 32];
   int mine = -2, prior = 0;  // this thread's row: its id and the earlier rows with it
   if (tid < p.M) {
