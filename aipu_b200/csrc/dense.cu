@@ -25,12 +25,15 @@
 namespace aipu {
 
 // ------------------------------------------------------------------ operands
-// power of two that brings a magnitude of at most `bound` into [2^13, 2^14) (0 and not finite: some scale)
+// s such that bound * 2^-s is in [2^top, 2^(top + 1)) (0 and not finite: some scale that is finite). Rows of magnitudes
+// below 2^(top - 126) are scaled by 2^126 only: bf16 values are multiples of 2^-133, so those stay exact in fp16.
 __device__ __forceinline__ int scale_shift(float bound, int top) {
   const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 0xFFu);
   const int s = bound == 0.f ? 0 : e - 127 - top;
-  return min(max(s, -100), 100);
+  return max(s, -126);  // (at most 128 - top: the factor 2^-s is a normal number)
 }
+// v * 2^e for |e| <= 252, in two steps of one sign, so that nothing is lost or overflows before the result does
+__device__ __forceinline__ float scale2(float v, int e) { return __fmul_rn(__fmul_rn(v, exp2i(e / 2)), exp2i(e - e / 2)); }
 
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           float* dst = p.y + (static_cast<int64_t>(blockIdx.z) * p.M + m0 + c0) * p.ldy + n;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c0 + j < cols) dst[j * p.ldy] = __fmul_rn(__fmul_rn(v[j], exp2i(xs[c0 + j])), exp2i(ws));
+            if (c0 + j < cols) dst[j * p.ldy] = scale2(v[j], xs[c0 + j] + ws);
         }
       }
     }
