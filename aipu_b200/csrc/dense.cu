@@ -3,17 +3,13 @@
 //   y32[m, n] = sum_k x[m, k] * w[n, k],  x bf16, w = GGUF rows (Q4_K, Q6_K, Q8_0, F16), fp32 out
 //
 // Two kernels: the weights and tokens as fp16 rows, and a GEMM of the two (TMA tiles with 128-byte swizzle,
-// tcgen05.mma kind::f16, fp32 accumulators in TMEM). Dequantising once per call and not once per token tile
-// is what makes this faster than a GEMM that dequantises its own tiles (2048 rows of 6144 x 2048: 65 us
-// against 145): the fp16 rows (2 bytes a weight) stay in L2 between the kernels. The GEMM of that case takes
-// 46 us (1.12 PFLOP/s, 0.69 of the measured bf16 peak); the tensor pipe is busy 68 % of the time on the 128
-// SMs that have a tile, the rest is the first copies and the last tile's store.
+// tcgen05.mma kind::f16, fp32 accumulators in TMEM).
 //
 // Rounding: a token row is scaled by a power of two and is then exact in fp16 (bf16 has 8 bits; values below
 // 2^-24 of the row's largest lose bits). A weight is dequantised in fp32 as ggml defines it, scaled by a
-// power of two per row, and rounded to fp16: 2^-11 of the weight at most, independent from weight to weight,
-// so that a result differs by about 2^-12 of its typical size, a tenth of its own rounding to bf16. F16
-// weights are used as they are stored. Products are exact, sums fp32.
+// power of two per row, and enters as two fp16 halves, 22 bits (2^-38 of the row's bound where it is small), whose
+// products go to accumulators of their own and are added once. One half alone would round it by 2^-11 and change every
+// tenth bf16 result. F16 weights are used as they are stored, in one product. Products are exact, sums fp32.
 #include <algorithm>
 
 #include "deq.cuh"
@@ -32,12 +28,24 @@ __device__ __forceinline__ int scale_shift(float bound, int top) {
   const int s = bound == 0.f ? 0 : e - 127 - top;
   return max(s, -126);  // (at most 128 - top: the factor 2^-s is a normal number)
 }
+// shift of a token row with an infinite value (top = 9): all its results are infinite or NaN by the upper halves alone (a
+// lower half of 0 or of the other sign would make NaN of an infinity)
+constexpr int kNotFinite = 255 - 127 - 9;
 // v * 2^e for |e| <= 252, in two steps of one sign, so that nothing is lost or overflows before the result does
 __device__ __forceinline__ float scale2(float v, int e) { return __fmul_rn(__fmul_rn(v, exp2i(e / 2)), exp2i(e - e / 2)); }
 
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// a and b as fp16 pairs hi + lo: hi rounded, lo the rest (exact in fp32) rounded, 2^-22 of the value together. A value
+// that is not finite is hi alone.
+__device__ __forceinline__ void two_halves(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = half2_bits(fabsf(f.x) < INFINITY ? __fsub_rn(a, f.x) : 0.f, fabsf(f.y) < INFINITY ? __fsub_rn(b, f.y) : 0.f);
 }
 
 // 8 bytes from a 2-byte aligned address
@@ -126,14 +134,16 @@ __global__ void __launch_bounds__(256) aipu_dense_operands_kernel(const uint8_t*
       const float f = exp2i(-s);
       if (t == 0) wshift[n] = s;
       uint4* dst = reinterpret_cast<uint4*>(w16 + static_cast<int64_t>(n) * K) + lane;
+      uint4* rest = reinterpret_cast<uint4*>(w16 + (static_cast<int64_t>(N) + n) * K) + lane;
 #pragma unroll 2
       for (int u = warp; u < units; u += 4) {
         float v[8];
         unit_weights<WT>(row, u, lane, v);
-        uint32_t o[4];
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = half2_bits(__fmul_rn(v[2 * k], f), __fmul_rn(v[2 * k + 1], f));
-        dst[32 * u] = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 4; ++k) two_halves(__fmul_rn(v[2 * k], f), __fmul_rn(v[2 * k + 1], f), hi[k], lo[k]);
+        dst[32 * u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        rest[32 * u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
   } else {
@@ -176,7 +186,7 @@ __global__ void __launch_bounds__(256) aipu_dense_operands_kernel(const uint8_t*
 
 // ------------------------------------------------------------------ GEMM
 struct DenseParams {
-  alignas(64) CUtensorMap wmap;  // [N][K] fp16, box 128 rows x 64 k, 128-byte swizzle
+  alignas(64) CUtensorMap wmap;  // [N][K] fp16, behind it the lower halves' [N][K]; box 128 rows x 64 k, 128-byte swizzle
   alignas(64) CUtensorMap xmap;  // [M][K] fp16, box NT rows x 64 k
   const int* wshift;             // [N] or nullptr (0)
   const int* xshift;             // [M]
@@ -188,11 +198,12 @@ struct DenseParams {
 
 constexpr int kDenseThreads = 320;  // 8 epilogue warps, the copy warp, the MMA warp
 
-template <int NT>
+// P: 2 where the weights are two halves, 1 where they are stored as fp16
+template <int NT, int P>
 struct DenseCfg {
-  static constexpr int A = 128 * 128, B = NT * 128;  // bytes of a stage: 64 k of 128 weight rows and NT token rows
-  static constexpr int STAGE = A + B;
-  static constexpr int S = 196608 / STAGE;           // stages in 192 KB: 4, 6 or 8
+  static constexpr int A = 128 * 128, B = NT * 128;  // bytes of a stage: 64 k of 128 weight rows (P times) and NT token rows
+  static constexpr int STAGE = P * A + B;
+  static constexpr int S = std::min(8, 196608 / STAGE);  // stages in 192 KB: 3 to 8
   static constexpr int TOTAL = S * STAGE + 1024;     // (tiles start on 1024 bytes)
 };
 
@@ -213,9 +224,9 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, int x
 // MMA warp: four K = 16 steps a stage, one thread; a commit releases the stage. Epilogue: TMEM lane =
 // weight row, so a warp's store is 32 neighbouring results of a token. Every wait is bounded: on expiry the
 // status word is set, the roles leave, copies and MMAs in flight are waited for (bounded), TMEM is freed.
-template <int NT>
+template <int NT, int P>
 __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const __grid_constant__ DenseParams p) {
-  using C = DenseCfg<NT>;
+  using C = DenseCfg<NT, P>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ DenseBars bars;
   __shared__ int xs[NT];
@@ -231,7 +242,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
     bars.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(&bars.tmem, NT);
+  if (warp == 9) tmem_alloc(&bars.tmem, P * NT);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -252,8 +263,9 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           break;
         }
         mbar_arrive_expect_tx(&bars.full[s], C::STAGE);
-        tma_load_2d(base + s * C::STAGE, &p.wmap, 64 * (k0 + i), n0, &bars.full[s]);
-        tma_load_2d(base + s * C::STAGE + C::A, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
+        tma_load_2d(base + s * C::STAGE, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
+        for (int h = 0; h < P; ++h)  // (rows past N are of the other half or 0: their results are not stored)
+          tma_load_2d(base + s * C::STAGE + C::B + h * C::A, &p.wmap, 64 * (k0 + i), h * p.N + n0, &bars.full[s]);
       }
       // no copy may land after the CTA has ended: the MMAs have read them all, or (abort) they are waited for
       mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL);
@@ -271,10 +283,13 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           break;
         }
         tc_fence_after();
-        const uint32_t a = base + s * C::STAGE, b = a + C::A;
+        const uint32_t b = base + s * C::STAGE, a = b + C::B;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f16(tmem, umma_desc_sw128(a + 32 * k, 1024), umma_desc_sw128(b + 32 * k, 1024), idesc, (i | k) ? 1u : 0u);
+        for (int h = 0; h < P; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem + h * NT, umma_desc_sw128(a + h * C::A + 32 * k, 1024), umma_desc_sw128(b + 32 * k, 1024), idesc,
+                     (i | k) ? 1u : 0u);
         umma_commit(&bars.empty[s]);
       }
       umma_commit(&bars.done);
@@ -290,8 +305,14 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
       const int cols = min(NT, p.M - m0);
 #pragma unroll 1
       for (int c0 = (warp >> 2) * 16; c0 < cols; c0 += 32) {
-        float v[16];
+        float v[16], lo[16];
         tmem_ld16(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0, v);
+        if (P == 2) {
+          tmem_ld16(tmem + (static_cast<uint32_t>(32 * q) << 16) + NT + c0, lo);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < cols && xs[c0 + j] < kNotFinite) v[j] = __fadd_rn(v[j], lo[j]);
+        }
         if (n < p.N) {
           float* dst = p.y + (static_cast<int64_t>(blockIdx.z) * p.M + m0 + c0) * p.ldy + n;
 #pragma unroll
@@ -306,7 +327,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
   if (warp == 9) {
     mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL, 200000000LL);  // the MMAs in flight (after an abort too)
     tc_fence_after();
-    tmem_dealloc(tmem, NT);
+    tmem_dealloc(tmem, P * NT);
     tmem_relinquish();
   }
 }
@@ -315,24 +336,29 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
 static size_t al1k(size_t v) { return (v + 1023) & ~static_cast<size_t>(1023); }
 
 size_t dense_bytes(int wt, int64_t N, int64_t K, int64_t M) {
-  const size_t w = wt == WT_F16 ? 0 : al1k(static_cast<size_t>(2) * N * K) + al1k(4 * N);
+  const size_t w = wt == WT_F16 ? 0 : al1k(static_cast<size_t>(4) * N * K) + al1k(4 * N);
   return w + al1k(static_cast<size_t>(2) * M * K) + al1k(4 * M);
 }
 
-static int rows_map(CUtensorMap* map, const void* base, int rows, int K, int box) {
+static int rows_map(CUtensorMap* map, const void* base, int64_t rows, int K, int box) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
   const cuuint32_t bx[2] = {64, static_cast<cuuint32_t>(box)};
   return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, bx, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+template <int NT, int P>
+static int dense_launch_p(DenseParams& p, int parts, cudaStream_t s) {
+  using C = DenseCfg<NT, P>;
+  const void* kern = reinterpret_cast<const void*>(aipu_dense_gemm_kernel<NT, P>);
+  static bool attr[64] = {false};
+  const int rc = set_smem_attr_once(kern, C::TOTAL, attr, "cudaFuncSetAttribute(dense)");
+  if (rc) return rc;
+  return launch_kernel(kern, dim3((p.N + 127) / 128, (p.M + NT - 1) / NT, parts), dim3(kDenseThreads), C::TOTAL, s, true, &p);
+}
 template <int NT>
 static int dense_launch(DenseParams& p, int parts, cudaStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(aipu_dense_gemm_kernel<NT>);
-  static bool attr[64] = {false};
-  const int rc = set_smem_attr_once(kern, DenseCfg<NT>::TOTAL, attr, "cudaFuncSetAttribute(dense)");
-  if (rc) return rc;
-  return launch_kernel(kern, dim3((p.N + 127) / 128, (p.M + NT - 1) / NT, parts), dim3(kDenseThreads), DenseCfg<NT>::TOTAL, s, true, &p);
+  return p.wshift ? dense_launch_p<NT, 2>(p, parts, s) : dense_launch_p<NT, 1>(p, parts, s);
 }
 
 static int token_tile(int64_t M) { return M <= 64 ? 64 : M <= 128 ? 128 : 256; }
@@ -372,7 +398,7 @@ int dense_gemm(int wt, const uint8_t* w, int N, int K, const uint16_t* x, int M,
   int* wshift = nullptr;
   if (wt != WT_F16) {
     w16 = reinterpret_cast<uint16_t*>(b);
-    b += al1k(static_cast<size_t>(2) * N * K);
+    b += al1k(static_cast<size_t>(4) * N * K);
     wshift = reinterpret_cast<int*>(b);
     b += al1k(4 * static_cast<size_t>(N));
   }
@@ -389,7 +415,7 @@ int dense_gemm(int wt, const uint8_t* w, int N, int K, const uint16_t* x, int M,
   if (rc) return rc;
   const int nt = token_tile(M), parts = dense_parts(N, K, M);
   DenseParams p = {};
-  rc = rows_map(&p.wmap, wt == WT_F16 ? static_cast<const void*>(w) : w16, N, K, 128);
+  rc = wt == WT_F16 ? rows_map(&p.wmap, w, N, K, 128) : rows_map(&p.wmap, w16, 2 * static_cast<int64_t>(N), K, 128);
   if (!rc) rc = rows_map(&p.xmap, x16, M, K, nt);
   if (rc) return rc;
   p.wshift = wshift;

@@ -49,3 +49,65 @@ def test_rows_of_extreme_magnitudes_above_8_rows(wt, M):
     bad = fits & ~((got - want).abs() <= tol + (want.abs() + tol) * 2.0 ** -8 + 2.0 ** -126)
     assert not bad.any(), (shift[bad.any(1)].tolist(), got[bad][:4], want[bad][:4])
     assert fits[shift.view(M, 1).expand(M, N) <= 117].float().mean() > 0.95
+
+
+def _residual(wt, w, N, K, x, y64):
+    """gemm_lora's sums less bf16(y64), through an adapter for each row (x[:, 0] is 1): what the result's rounding hides."""
+    M, d = x.shape[0], x.device
+    a = torch.zeros((M, 1, K), dtype=BF, device=d)
+    a[:, 0, 0] = 1
+    near = y64.to(BF).contiguous()
+    A = ops.LoraAdapters(a, -near.view(M, N, 1))
+    return ops.gemm_lora(wt, w, N, K, x, A, torch.arange(M, dtype=torch.int32, device=d)).double(), y64 - near.double()
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 65, 129, 300])
+def test_weights_keep_their_bits_at_every_row_count(wt, M):
+    """One weight a result, as x picks it, less its bf16 value: off by the rounding of the rest (2^-8 of it) and by 2^-19
+    of the row's largest weight (fp16 halves: 2^-22 of the weight; Q4_K's two terms in fp32; one row: x to 2^-21)."""
+    d, K, N = _dev(), 512, 200
+    w, wd = _weights(wt, N, K, M, d)
+    x = torch.zeros((M, K), dtype=BF, device=d)
+    x[:, 0] = 1
+    k = torch.randint(1, K, (M,), generator=torch.Generator().manual_seed(M)).to(d)
+    x[torch.arange(M, device=d), k] = 1
+    y64 = wd[:, 0].view(1, N) + wd[:, k].t()
+    got, want = _residual(wt, w, N, K, x, y64)
+    tol = want.abs() * 2.0 ** -8 + 2.0 ** -19 * 2 * wd.abs().amax(1)
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("M,K", [(16, 4096), (40, 2048), (300, 6144)])
+def test_the_projections_sums_have_32_bits(wt, M, K):
+    """Root mean square of the sums' error: K / 16 steps of the MMA, each cut off by at most 2^-23 of a running sum that is at
+    most about the result, and the rounding of the rest to bf16 (2^-9 of up to 2^-9, rms). Weights of 11 bits would give 2^-12
+    / sqrt(3), 1.4e-4."""
+    d, N = _dev(), 264
+    w, wd = _weights(wt, N, K, M, d)
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(K)).to(BF)
+    x[:, 0] = 1
+    y64 = x.double() @ wd.t()
+    got, want = _residual(wt, w, N, K, x, y64)
+    err = (got - want).square().mean().sqrt() / y64.square().mean().sqrt()
+    assert err <= K / 16 * 2.0 ** -23 + 2.0 ** -18, float(err)
+
+
+@pytest.mark.parametrize("wt", [F.Q8_0, F.F16])
+@pytest.mark.parametrize("M", [9, 150, 300])
+def test_an_infinite_token_keeps_its_signs(wt, M):
+    """An infinite value times weights that are not 0 is infinite with the weight's sign, whatever the weight's bits."""
+    d, K, N = _dev(), 256, 140
+    w, wd = _weights(wt, N, K, 9, d)
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(M)).to(BF)
+    ids = torch.full((M,), -1, dtype=torch.int32, device=d)
+    clean = ops.gemm_lora(wt, w, N, K, x, _plain(d, K, N), ids)
+    x[1, 7], x[4, 30], x[5, 2] = float("inf"), float("-inf"), float("nan")
+    got = ops.gemm_lora(wt, w, N, K, x, _plain(d, K, N), ids)
+    keep = [m for m in range(M) if m not in (1, 4, 5)]
+    assert torch.equal(got[keep], clean[keep]) and got[5].isnan().all()
+    for m, k, s in ((1, 7, 1), (4, 30, -1)):
+        live = wd[:, k] != 0
+        assert torch.equal(got[m, live].double(), (s * wd[live, k].sign()) * float("inf"))
+        assert got[m, ~live].isnan().all()
