@@ -1384,9 +1384,9 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
   return lora_finish(p, s, pdl || p.tiles);
 }
 
-// rows from which the projection dequantises its weights once and runs as an fp16 GEMM: above the rows of one
-// decode GEMV launch
-static bool gemm_lora_dense(int64_t M) { return M > 8; }
+// whether the projection dequantises its weights once and runs as an fp16 GEMM: above the rows of one decode GEMV
+// launch, and where a row does not fit the GEMV
+static bool gemm_lora_dense(int64_t M, int64_t K) { return M > 8 || K > kGemvMaxK; }
 // row stride of its fp32 sums: rows start on 32 bytes
 static int64_t gemm_lora_ld(int64_t N) { return (N + 7) & ~static_cast<int64_t>(7); }
 
@@ -1394,9 +1394,9 @@ extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K,
   if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
       n_adapters > 32768 || rank < 1 || rank > 128)
     return 0;
-  const size_t parts = gemm_lora_dense(M) ? dense_parts(N, K, M) : 1;
+  const size_t parts = gemm_lora_dense(M, K) ? dense_parts(N, K, M) : 1;
   size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * parts * M * gemm_lora_ld(N));
-  if (gemm_lora_dense(M)) b += dense_bytes(wtype, N, K, M);
+  if (gemm_lora_dense(M, K)) b += dense_bytes(wtype, N, K, M);
   return static_cast<int64_t>(b);
 }
 
@@ -1415,14 +1415,13 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
   if (!c) return set_error(EINVAL_, "gemm_lora: null context");
   if (M == 0) return OK;
-  if (!gemm_lora_dense(M) && (N + 15) / 16 > c->ws[0].max_tiles) return set_error(EINVAL_, "gemm_lora: N too large for the workspace");
   DeviceGuard dg(c->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* b = static_cast<uint8_t*>(ws);
   void* plan = b;
   b += al256x(lora_plan_bytes(M, p.L, p.R));
   float* y32 = reinterpret_cast<float*>(b);
-  if (gemm_lora_dense(M)) p.yparts = dense_parts(N, K, M);
+  if (gemm_lora_dense(M, K)) p.yparts = dense_parts(N, K, M);
   b += al256x(4 * static_cast<size_t>(std::max(p.yparts, 1)) * M * gemm_lora_ld(N));
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = K;
@@ -1434,26 +1433,35 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   p.y_f32 = 1;
   p.status = c->status;
   if ((rc = lora_begin(p, plan, s, false))) return rc;
-  if (gemm_lora_dense(M)) {
+  if (gemm_lora_dense(M, K)) {
     // (beside the first product of the adapters, which was launched just before where there are many rows)
     rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, p.ldy, b, c->status, s, p.tiles != nullptr);
   } else {
-    GemvParams g = {};
-    g.w0 = static_cast<const uint8_t*>(w);
-    g.row_bytes = row_bytes_of(wtype, K);
-    g.n_groups = 1;
-    g.N = p.N;
-    g.K = p.K;
-    g.x = p.x;
-    g.M = p.M;
-    g.y32 = y32;
-    g.y32_ld = p.ldy;
-    g.partials = c->ws[0].partials;
-    g.counters = c->ws[0].counters;
-    g.status = c->status;
-    // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
-    // kernel behind it may read x, the ids and the adapters without waiting for it
-    rc = gemv_launch(wtype, XT_BF16, EPI_STORE32, g, c->num_sms, s, false);
+    // as many launches as the GEMV's tile counters (of N) and its shared memory (of tokens of K) ask for
+    const int64_t step = static_cast<int64_t>(c->ws[0].max_tiles) * 16;
+    for (int64_t n0 = 0; n0 < N && !rc; n0 += step) {
+      GemvParams g = {};
+      g.row_bytes = row_bytes_of(wtype, K);
+      g.w0 = static_cast<const uint8_t*>(w) + n0 * g.row_bytes;
+      g.n_groups = 1;
+      g.N = static_cast<int>(std::min(step, N - n0));
+      g.K = p.K;
+      g.y32_ld = p.ldy;
+      g.partials = c->ws[0].partials;
+      g.counters = c->ws[0].counters;
+      g.status = c->status;
+      const int fit = gemv_rows(wtype, g.w0, g.N, g.K, c->num_sms);
+      if (fit < 1) return set_error(EINVAL_, "gemm_lora: a token does not fit the GEMV");
+      const int launches = (p.M + fit - 1) / fit, rows = (p.M + launches - 1) / launches;
+      for (int m0 = 0; m0 < p.M && !rc; m0 += rows) {
+        g.M = std::min(rows, p.M - m0);
+        g.x = p.x + static_cast<int64_t>(m0) * K;
+        g.y32 = y32 + m0 * p.ldy + n0;
+        // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
+        // kernel behind it may read x, the ids and the adapters without waiting for it
+        rc = gemv_launch(wtype, XT_BF16, EPI_STORE32, g, c->num_sms, s, false);
+      }
+    }
   }
   if (rc) return rc;
   p.wait_y = 1;

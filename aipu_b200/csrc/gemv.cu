@@ -1428,20 +1428,24 @@ static int launch_one(GemvParams p, int grid, int nw, int smem, cudaStream_t str
 // (at most 2: the kernel processes a chunk as one or two straight-line units)
 static int gemv_upc(int wt) { return wt == WT_Q4K ? 2 : wt == WT_Q6K ? 2 : wt == WT_Q80 ? 2 : 1; }
 
-int gemv_launch(int wt, int xt, int epi, GemvParams p, int num_sms, cudaStream_t stream, bool pdl, int min_smem) {
+struct GemvShape {
+  int grid, nw, smem;
+  bool engi;  // the integer dot engine
+};
+
+// Launch shape of p's sizes and addresses (p.upc .. p.cta_mode and the tensor map's box are set; no map is encoded).
+static int gemv_shape(int wt, int xt, int epi, GemvParams& p, int num_sms, int min_smem, GemvShape& out) {
   if (p.K % 256 != 0 || p.K <= 0 || p.N <= 0 || p.M <= 0 || ((xt == XT_F32) ? 2 * p.M : p.M) > 8)
     return set_error(-1, "gemv: bad shape");
+  const int ne_map = p.n_experts > 0 ? p.n_experts : p.n_groups;
+  // tiled TMA path when rows (and experts) start on 16-byte boundaries
+  const bool aligned = (p.row_bytes % 16 == 0) && (reinterpret_cast<uintptr_t>(p.w0) % 16 == 0) &&
+                       (!p.w1 || reinterpret_cast<uintptr_t>(p.w1) % 16 == 0) &&
+                       (ne_map <= 1 || p.expert_stride % 16 == 0);
   // the integer dot engine for Q4_K and Q6_K rows and one token (the decode GEMV); the f16 engine
   // otherwise
   // (Q6_K: only with tiled copies, where every row of a slot starts at the same offset)
-  const bool tiled_rows = (p.row_bytes % 16 == 0) && (reinterpret_cast<uintptr_t>(p.w0) % 16 == 0) &&
-                          (!p.w1 || reinterpret_cast<uintptr_t>(p.w1) % 16 == 0) &&
-                          ((p.n_experts > 0 ? p.n_experts : p.n_groups) <= 1 || p.expert_stride % 16 == 0);
-  const bool engi = (wt == WT_Q4K || (wt == WT_Q6K && tiled_rows)) && p.M == 1 && (epi == EPI_STORE || xt == XT_BF16);
-  const int ncols = engi ? 8 : ((xt == XT_F32) ? 2 * p.M : p.M);
-  if (epi == EPI_SWIGLU && xt != XT_BF16) return set_error(-1, "gemv: swiglu needs bf16 activations");
-  if (epi == EPI_STORE32 && (xt != XT_BF16 || !p.y32 || p.n_groups != 1)) return set_error(-1, "gemv: fp32 sums need bf16 activations of one group");
-  if ((reinterpret_cast<uintptr_t>(p.x) & 15u) != 0) return set_error(-1, "gemv: activations must be 16-byte aligned");
+  const bool engi = (wt == WT_Q4K || (wt == WT_Q6K && aligned)) && p.M == 1 && (epi == EPI_STORE || xt == XT_BF16);
   const int rpt = (epi == EPI_SWIGLU) ? 8 : 16;
   const int64_t upg = static_cast<int64_t>((p.N + rpt - 1) / rpt) * (p.K / 256);
   const int64_t U = static_cast<int64_t>(p.n_groups) * upg;
@@ -1451,30 +1455,12 @@ int gemv_launch(int wt, int xt, int epi, GemvParams p, int num_sms, cudaStream_t
   if (grid < 1) grid = 1;
   p.upc = gemv_upc(wt);
   p.pitch = gemv_slot_pitch(wt, p.upc);
-  // tiled TMA path when rows (and experts) start on 16-byte boundaries
-  const int ne_map = p.n_experts > 0 ? p.n_experts : p.n_groups;
-  const bool aligned = (p.row_bytes % 16 == 0) && (reinterpret_cast<uintptr_t>(p.w0) % 16 == 0) &&
-                       (!p.w1 || reinterpret_cast<uintptr_t>(p.w1) % 16 == 0) &&
-                       (ne_map <= 1 || p.expert_stride % 16 == 0);
   p.use_tmap = aligned ? 1 : 0;
   if (p.use_tmap) {
     p.tm_esz = (wt == WT_Q6K) ? 2 : 8;
     p.tm_box = (wt == WT_Q4K) ? 18 * p.upc : (wt == WT_Q6K) ? 240 : 68;
     p.pitch = p.tm_box * p.tm_esz;
-    const int ne = ne_map;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.row_bytes / p.tm_esz), static_cast<cuuint64_t>(p.N),
-                                static_cast<cuuint64_t>(ne)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.row_bytes),
-                                   static_cast<cuuint64_t>(ne > 1 ? p.expert_stride : p.row_bytes * p.N)};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(p.tm_box), static_cast<cuuint32_t>(rpt), 1};
-    const CUtensorMapDataType dt = (wt == WT_Q6K) ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT64;
-    int rc = encode_tiled(&p.tmap0, dt, 3, p.w0, dims, strides, box);
-    if (!rc && epi == EPI_SWIGLU) rc = encode_tiled(&p.tmap1, dt, 3, p.w1, dims, strides, box);
-    if (rc) return rc;
   }
-  // f16 engine: K fp16 values per column; integer engine: K bytes per column, +32 so that the 8 columns
-  // read by a half-warp start 8 banks apart
-  p.xpitch = engi ? p.K + 32 : ((p.K * 2 + 127) & ~127) + 64;
   // at least ~4 units per worker: fewer pieces per tile when a launch has few units
   const int64_t want_w = std::max<int64_t>(4, std::min<int64_t>(16, U / (4 * static_cast<int64_t>(grid))));
   // A launch with few units per CTA (a single decode GEMV) is latency-bound: its weights are on the
@@ -1499,28 +1485,68 @@ int gemv_launch(int wt, int xt, int epi, GemvParams p, int num_sms, cudaStream_t
     if (p.xg > GEMV_MAXXG) return set_error(-1, "gemv: too many activation groups per CTA");
   }
   const int full_limit = 232448 - 1024 - 2 * GEMV_MAXW * 4;  // dynamic smem limit minus static
-  int limit = full_limit;
-  int nw = 0, ns = 0;
-  // small launches try half an SM first (unless the caller asks for a minimum), then the whole SM
-  for (int pass = (small && min_smem == 0) ? 0 : 1; pass < 2 && !nw; ++pass) {
-    limit = pass == 0 ? 232448 / 2 - 1024 - 2 * GEMV_MAXW * 4 : full_limit;
-    for (int cand_w : {16, 12, 8, 4}) {
-      if (!small && cand_w > want_w && cand_w > 4) continue;
-      if (small && cand_w > small_w) continue;
-      for (int cand_s = GEMV_MAXS; cand_s >= (small ? 1 : 2); --cand_s) {
-        if (gemv_layout(wt, ncols, p.K, p.xg, cand_w, cand_s, p.pitch, p.xpitch, p.cta_mode ? cand_w : 0).total <=
-            limit) {
-          nw = cand_w;
-          ns = cand_s;
-          break;
+  // (long rows of one token: the integer engine's eight columns are 8 K bytes, the f16 engine's column 2 K)
+  for (int eng = engi ? 1 : 0; eng >= 0; --eng) {
+    const int ncols = eng ? 8 : ((xt == XT_F32) ? 2 * p.M : p.M);
+    // f16 engine: K fp16 values per column; integer engine: K bytes per column, +32 so that the 8 columns
+    // read by a half-warp start 8 banks apart
+    p.xpitch = eng ? p.K + 32 : ((p.K * 2 + 127) & ~127) + 64;
+    // small launches try half an SM first (unless the caller asks for a minimum), then the whole SM
+    for (int pass = (small && min_smem == 0) ? 0 : 1; pass < 2; ++pass) {
+      const int limit = pass == 0 ? 232448 / 2 - 1024 - 2 * GEMV_MAXW * 4 : full_limit;
+      for (int cand_w : {16, 12, 8, 4}) {
+        if (!small && cand_w > want_w && cand_w > 4) continue;
+        if (small && cand_w > small_w) continue;
+        for (int cand_s = GEMV_MAXS; cand_s >= (small ? 1 : 2); --cand_s) {
+          const int total = gemv_layout(wt, ncols, p.K, p.xg, cand_w, cand_s, p.pitch, p.xpitch, p.cta_mode ? cand_w : 0).total;
+          if (total > limit) continue;
+          p.nslots = cand_s;
+          out = {grid, cand_w, std::min(limit, std::max(min_smem, total)), eng != 0};
+          return OK;
         }
       }
-      if (nw) break;
     }
   }
-  if (!nw) return set_error(-1, "gemv: activation block too large for shared memory");
-  p.nslots = ns;
-  const int smem = std::min(limit, std::max(min_smem, gemv_layout(wt, ncols, p.K, p.xg, nw, ns, p.pitch, p.xpitch, p.cta_mode ? nw : 0).total));
+  return set_error(-1, "gemv: activation block too large for shared memory");
+}
+
+int gemv_rows(int wt, const uint8_t* w, int N, int K, int num_sms) {
+  for (int M = K <= kGemvMaxK ? 8 : 0; M > 0; --M) {
+    GemvParams p = {};
+    p.w0 = w;
+    p.row_bytes = row_bytes_of(wt, K);
+    p.n_groups = 1;
+    p.N = N;
+    p.K = K;
+    p.M = M;
+    GemvShape g;
+    if (gemv_shape(wt, XT_BF16, EPI_STORE32, p, num_sms, 0, g) == OK) return M;
+  }
+  return 0;
+}
+
+int gemv_launch(int wt, int xt, int epi, GemvParams p, int num_sms, cudaStream_t stream, bool pdl, int min_smem) {
+  GemvShape g;
+  const int src = gemv_shape(wt, xt, epi, p, num_sms, min_smem, g);
+  if (src) return src;
+  const bool engi = g.engi;
+  const int grid = g.grid, nw = g.nw, smem = g.smem;
+  if (epi == EPI_SWIGLU && xt != XT_BF16) return set_error(-1, "gemv: swiglu needs bf16 activations");
+  if (epi == EPI_STORE32 && (xt != XT_BF16 || !p.y32 || p.n_groups != 1)) return set_error(-1, "gemv: fp32 sums need bf16 activations of one group");
+  if ((reinterpret_cast<uintptr_t>(p.x) & 15u) != 0) return set_error(-1, "gemv: activations must be 16-byte aligned");
+  if (p.use_tmap) {
+    const int rpt = (epi == EPI_SWIGLU) ? 8 : 16;
+    const int ne = p.n_experts > 0 ? p.n_experts : p.n_groups;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.row_bytes / p.tm_esz), static_cast<cuuint64_t>(p.N),
+                                static_cast<cuuint64_t>(ne)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.row_bytes),
+                                   static_cast<cuuint64_t>(ne > 1 ? p.expert_stride : p.row_bytes * p.N)};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(p.tm_box), static_cast<cuuint32_t>(rpt), 1};
+    const CUtensorMapDataType dt = (wt == WT_Q6K) ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT64;
+    int rc = encode_tiled(&p.tmap0, dt, 3, p.w0, dims, strides, box);
+    if (!rc && epi == EPI_SWIGLU) rc = encode_tiled(&p.tmap1, dt, 3, p.w1, dims, strides, box);
+    if (rc) return rc;
+  }
   if (engi && wt == WT_Q4K) {
     if (xt == XT_F32) return launch_one<WT_Q4K, XT_F32, EPI_STORE, 1>(p, grid, nw, smem, stream, pdl);
     if (xt == XT_BF16 && epi == EPI_STORE) return launch_one<WT_Q4K, XT_BF16, EPI_STORE, 1>(p, grid, nw, smem, stream, pdl);

@@ -78,6 +78,12 @@ struct GemvParams {
   alignas(64) CUtensorMap tmap1;  // same over w1 (EPI_SWIGLU)
 };
 
+// Longest K that one bf16 token always fits: 2 K bytes of it and K / 4 of its sub-block sums beside two ring slots of
+// four warps (70 KB for the widest rows) in an SM's 226 KB.
+constexpr int kGemvMaxK = 65536;
+// Most bf16 tokens (0 .. 8) that one launch takes of rows w [N, K]: all of them are staged in shared memory.
+int gemv_rows(int wt, const uint8_t* w, int N, int K, int num_sms);
+
 __host__ __device__ inline int gemv_slot_pitch(int wt, int upc) {
   // room for the unit bytes plus a possible 16-byte-alignment head, rounded so that rows start
   // 32 or 96 bytes mod 128 (rows g = 0..3 of a half-warp then hit distinct banks)

@@ -111,3 +111,72 @@ def test_an_infinite_token_keeps_its_signs(wt, M):
         live = wd[:, k] != 0
         assert torch.equal(got[m, live].double(), (s * wd[live, k].sign()) * float("inf"))
         assert got[m, ~live].isnan().all()
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("K", [11008, 14336, 28672])
+@pytest.mark.parametrize("N", [80, 2400])
+def test_few_rows_of_long_weights(wt, K, N):
+    """Tokens that do not all fit the shared memory of one GEMV launch. Sums of K products by steps of 16, each off by at
+    most 2^-23 of the magnitudes (Q4_K: of d sc q and dmin m apart); one row: x to 2^-21 of its largest."""
+    d = _dev()
+    w, wd = _weights(wt, N, K, 3, d)
+    x = torch.randn((8, K), device=d, generator=torch.Generator(d).manual_seed(K)).to(BF)
+    g = torch.Generator(d).manual_seed(N)
+    A = ops.LoraAdapters((torch.randn((2, 8, K), device=d, generator=g) * K ** -0.5).to(BF),
+                         (torch.randn((2, N, 8), device=d, generator=g) * float(wd.square().mean().sqrt()) * K ** 0.5).to(BF))
+    ids = torch.tensor([0, 1, -1, 1, 0, 0, -1, 1], dtype=torch.int32, device=d)
+    h = torch.einsum("mk,lrk->mlr", x.double(), A.a.double())
+    size = torch.einsum("mk,lrk->mlr", x.double().abs(), A.a.double().abs())
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    if wt == F.Q4_K:
+        dm = w.view(-1, 144)[:, 2:4].contiguous().view(HF).double().view(N, K // 256)
+        mag = mag + 2 * 63 * (x.double().abs().view(8, -1, 256).sum(2) @ dm.abs().t())
+    for m in range(8):
+        if ids[m] >= 0:
+            n = int(ids[m])
+            want[m] += A.b[n].double() @ h[m, n]
+            mag[m] += A.b[n].double().abs() @ size[m, n] + (A.b[n].double().abs() @ h[m, n].abs()) * 2.0 ** -15 / (K / 16 * 2.0 ** -23)
+    tol = mag * (K / 16 * 2.0 ** -23)
+    for M in (1, 2, 3, 5, 6, 7, 8):
+        got = ops.gemm_lora(wt, w, N, K, x[:M], A, ids[:M]).double()
+        t = tol[:M] + (2.0 ** -21 * x[:1].double().abs().amax() * wd.abs().sum(1) if M == 1 else 0)
+        t = t + (want[:M].abs() + t) * 2.0 ** -8
+        assert ((got - want[:M]).abs() <= t).all(), (M, ((got - want[:M]).abs() / t).max())
+    assert torch.equal(ops.gemm_lora(wt, w, N, K, x[2:3], A, ids[2:3]), ops.gemm(wt, w, N, K, x[2:3]))
+
+
+@pytest.mark.parametrize("wt", [F.Q4_K, F.F16])
+@pytest.mark.parametrize("M", [1, 5])
+def test_few_rows_of_weights_longer_than_the_gemv_takes(wt, M):
+    """K above 65536: the fp16 GEMM takes any number of rows."""
+    d, K, N = _dev(), 65536 + 512, 40
+    w, wd = _weights(wt, N, K, 3, d)
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(K)).to(BF)
+    ids = torch.full((M,), -1, dtype=torch.int32, device=d)
+    got = ops.gemm_lora(wt, w, N, K, x, _plain(d, K, N), ids).double()
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    assert ((got - want).abs() <= mag * (K / 16 * 2.0 ** -23) + want.abs() * 2.0 ** -7).all()
+
+
+@pytest.mark.parametrize("M", [1, 8])
+def test_few_rows_of_more_weight_rows_than_the_gemv_counts(M):
+    """N above 2^20, an LM head's rows of many vocabularies in one: results on both sides of the border and at the end."""
+    d, K, N = _dev(), 256, (1 << 20) + 1000
+    w = torch.randint(0, 256, (N, 8, 34), dtype=torch.uint8, device=d, generator=torch.Generator(d).manual_seed(1))
+    w[:, :, 0] = 0
+    w[:, :, 1] = 0x1C  # fp16 2^-8
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(M)).to(BF)
+    A = _plain(d, K, N)
+    A.a[0, 0, 0] = 1
+    A.b[0, :, 0] = torch.arange(N, device=d) % 128
+    ids = torch.tensor([0, -1] * 4, dtype=torch.int32, device=d)[:M]
+    got = ops.gemm_lora(F.Q8_0, w, N, K, x, A, ids).double()
+    wd = w[:, :, 2:].view(torch.int8).reshape(N, K)
+    for a, b in ((0, 3000), ((1 << 20) - 3000, (1 << 20) + 500), (N - 600, N)):
+        v = wd[a:b].double() * 2.0 ** -8
+        want, mag = x.double() @ v.t(), x.double().abs() @ v.abs().t()
+        add = x[:, :1].double() * A.b[0, a:b, 0].double() * (ids >= 0).view(M, 1)
+        tol = mag * (16 * 2.0 ** -23) + add.abs() * 2.0 ** -15
+        tol = tol + ((want + add).abs() + tol) * 2.0 ** -8
+        assert ((got[:, a:b] - want - add).abs() <= tol).all()
