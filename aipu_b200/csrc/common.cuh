@@ -214,7 +214,7 @@ __device__ __forceinline__ uint16_t bf16_rne_bits(float x) {
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 __device__ __forceinline__ float bf16_round_f(float x) { return bf16_bits_to_f32(bf16_rne_bits(x)); }
 
-// exact power-of-two scale 2^e for |e| <= 126
+// exact power-of-two scale 2^e for -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 }  // namespace aipu

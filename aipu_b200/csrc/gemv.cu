@@ -467,10 +467,9 @@ __device__ void gemv_stage_x_i8(const GemvParams& p, uint8_t* smem, const GemvLa
   float m = 0.f;
   for (int w = 0; w < NW; ++w) m = fmaxf(m, red[w]);
   // max * 2^-s in [2^21, 2^22): |X| <= 2^22 after rounding, so d2 stays within [-65, 65] and every
-  // integer sum below stays exact
+  // integer sum below stays exact (rows of magnitudes below 2^-105 are scaled by 2^126 only)
   const int e = static_cast<int>((__float_as_uint(m) >> 23) & 0xFFu);
-  int sh = (m == 0.f) ? 0 : (e - 127 - 21);
-  sh = sh < -100 ? -100 : (sh > 100 ? 100 : sh);
+  const int sh = (m == 0.f) ? 0 : max(e - 127 - 21, -126);
   if (tid == 0) {
     misc[0] = sh;
     misc[1] = sh;
@@ -819,10 +818,10 @@ __device__ __forceinline__ float vec_absmax(const uint4 q, bool f32, float mx) {
 }
 
 __device__ __forceinline__ int prescale_shift(float mx) {
-  // max * 2^-s in [2^9, 2^10): sub-block sums of 32 values stay below 2^15 (fp16-safe)
+  // max * 2^-s in [2^9, 2^10): sub-block sums of 32 values stay below 2^15 (fp16-safe); rows of magnitudes below 2^-117 are
+  // scaled by 2^126 only
   const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu);
-  int s = (mx == 0.f) ? 0 : (e - 127 - 9);
-  return s < -100 ? -100 : (s > 100 ? 100 : s);
+  return mx == 0.f ? 0 : max(e - 127 - 9, -126);
 }
 
 // Stage the activations of group `grp` into shared memory as fp16 columns (see gemv.cuh). Tokens

@@ -180,3 +180,25 @@ def test_few_rows_of_more_weight_rows_than_the_gemv_counts(M):
         tol = mag * (16 * 2.0 ** -23) + add.abs() * 2.0 ** -15
         tol = tol + ((want + add).abs() + tol) * 2.0 ** -8
         assert ((got[:, a:b] - want - add).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("e", [0, 100, 105, 111, 116, 121, 124, -90, -100])
+def test_rows_of_extreme_magnitudes_up_to_8_rows(wt, M, e):
+    """As above 8 rows; Q4_K's sums of d sc q and of dmin m apart, and one row's x is rounded to 2^-21 of its largest."""
+    d, K, N = _dev(), 512, 130
+    w, wd = _weights(wt, N, K, 5, d)
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(M)).clamp_(-3.9, 3.9)
+    x = (x.double() * 2.0 ** e).to(BF)
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    if wt == F.Q4_K:
+        dm = w.view(-1, 144)[:, 2:4].contiguous().view(HF).double().view(N, K // 256)
+        mag = mag + 2 * 63 * (x.double().abs().view(M, -1, 256).sum(2) @ dm.abs().t())
+    tol = mag * (K * 2.0 ** -23) + (2.0 ** -21 * x.double().abs().amax() * wd.abs().sum(1) if M == 1 else 0)
+    ids = torch.full((M,), -1, dtype=torch.int32, device=d)
+    got = ops.gemm_lora(wt, w, N, K, x, _plain(d, K, N), ids)
+    fits = want.abs() + tol < 3e38
+    bad = fits & ~((got.double() - want).abs() <= tol + (want.abs() + tol) * 2.0 ** -8)
+    assert not bad.any(), (got[bad][:4], want[bad][:4])
+    assert torch.equal(ops.gemm(wt, w, N, K, x), got)
