@@ -475,6 +475,7 @@ __device__ void gemv_stage_x_i8(const GemvParams& p, uint8_t* smem, const GemvLa
     misc[1] = sh;
   }
   const float sc = exp2i(-sh);
+  uint32_t over = 0;  // upper byte set: an X of more than 24 bits, from an infinity or NaN, which have no digits
   auto stage8 = [&](int v, const float (&f)[8]) {
     int sum = 0;
     // balanced base-256 digits of X at once: the bytes of X + 0x808080 (in [0, 2^24) for |X| <= 2^22)
@@ -488,6 +489,7 @@ __device__ void gemv_stage_x_i8(const GemvParams& p, uint8_t* smem, const GemvLa
       sum += X;
       e[i] = (static_cast<uint32_t>(X) + 0x808080u) ^ 0x808080u;
     }
+    over |= (e[0] | e[1] | e[2]) | (e[3] | e[4] | e[5]) | (e[6] | e[7]);
     // digit planes: byte c of elements 0..3 and 4..7
     uint32_t dig[3][2];
 #pragma unroll
@@ -530,7 +532,11 @@ __device__ void gemv_stage_x_i8(const GemvParams& p, uint8_t* smem, const GemvLa
       stage8(v, f);
     }
   }
-  __syncthreads();
+  // a row that is not finite: the first sub-block's sum, which enters every result, is NaN
+  if (__syncthreads_or((over >> 24) != 0u)) {
+    if (tid == 0) sxs[0] = NAN;
+    __syncthreads();
+  }
 }
 
 // Q4_K unit (16 rows g, g + 8 x one super-block) on the integer engine, one token. acc[0] / acc[2]:

@@ -202,3 +202,19 @@ def test_rows_of_extreme_magnitudes_up_to_8_rows(wt, M, e):
     bad = fits & ~((got.double() - want).abs() <= tol + (want.abs() + tol) * 2.0 ** -8)
     assert not bad.any(), (got[bad][:4], want[bad][:4])
     assert torch.equal(ops.gemm(wt, w, N, K, x), got)
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("v", ["inf", "-inf", "nan"])
+def test_tokens_that_are_not_finite_up_to_8_rows(wt, M, v):
+    """No finite result of such a row, and none of the others' changes."""
+    d, K, N = _dev(), 512, 130
+    w, _ = _weights(wt, N, K, 5, d)
+    x = torch.randn((M, K), device=d, generator=torch.Generator(d).manual_seed(M)).to(BF)
+    A, ids = _plain(d, K, N), torch.full((M,), -1, dtype=torch.int32, device=d)
+    clean = ops.gemm_lora(wt, w, N, K, x, A, ids)
+    x[M - 1, 300] = float(v)
+    got = ops.gemm_lora(wt, w, N, K, x, A, ids)
+    assert torch.equal(got[:M - 1], clean[:M - 1]) and not torch.isfinite(got[M - 1]).any()
+    assert not torch.isfinite(ops.gemm(wt, w, N, K, x)[M - 1]).any()
