@@ -85,27 +85,21 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int valid) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Two floats as packed bf16 pieces: hi truncated (never overflows), lo = the exact rest rounded or
-// truncated. A value that is not finite has no rest.
-__device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
+// v as bf16 pieces: hi = v cut off (to the next value towards 0 where nothing would be left) and the rest, which is exact.
+// So no piece of a value other than 0 is 0 or has another sign, and infinity = the largest number + infinity: pieces
+// times an infinite or NaN factor sum to what the value times it is. (A value of less than 2^-132 has pieces of 0.)
+__device__ __forceinline__ uint32_t upper(float v) { return (__float_as_uint(v) - (v != 0.f ? 1u : 0u)) & 0xFFFF0000u; }
 __device__ __forceinline__ uint32_t piece(float v, float& rest) {
-  if (not_finite(v)) {
-    rest = 0.f;
-    // a NaN keeps a bit that the upper half shows
-    return (v != v) ? 0x7FC0u : __float_as_uint(v) >> 16;
-  }
-  const uint32_t hi = __float_as_uint(v) & 0xFFFF0000u;
+  const uint32_t hi = upper(v);
   rest = __fsub_rn(v, __uint_as_float(hi));
   return hi >> 16;
 }
-// packed pair of fp16 -> packed bf16 hi and lo (exact: 11 bits)
+// packed pair of fp16 -> packed bf16 hi and lo (11 bits: lo is exact too)
 __device__ __forceinline__ void split_f16(uint32_t w, uint32_t& hi, uint32_t& lo) {
   const float a = f16_bits_to_f32(w), b = f16_bits_to_f32(w >> 16);
-  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  const uint32_t ua = upper(a), ub = upper(b);
   hi = prmt(ua, ub, 0x7632u);
-  float ra = __fsub_rn(a, __uint_as_float(ua & 0xFFFF0000u)), rb = __fsub_rn(b, __uint_as_float(ub & 0xFFFF0000u));
-  if (not_finite(a)) ra = 0.f;
-  if (not_finite(b)) rb = 0.f;
+  const float ra = __fsub_rn(a, __uint_as_float(ua)), rb = __fsub_rn(b, __uint_as_float(ub));
   lo = prmt(__float_as_uint(ra), __float_as_uint(rb), 0x7632u);
 }
 

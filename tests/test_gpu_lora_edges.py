@@ -218,3 +218,43 @@ def test_tokens_that_are_not_finite_up_to_8_rows(wt, M, v):
     got = ops.gemm_lora(wt, w, N, K, x, A, ids)
     assert torch.equal(got[:M - 1], clean[:M - 1]) and not torch.isfinite(got[M - 1]).any()
     assert not torch.isfinite(ops.gemm(wt, w, N, K, x)[M - 1]).any()
+
+
+@pytest.mark.parametrize("ad", [BF, HF])
+@pytest.mark.parametrize("M", [6, 70, 270])
+@pytest.mark.parametrize("t", [BF, FP])
+def test_infinite_values_keep_their_signs_in_adapters(ad, M, t):
+    """x, A, B or h infinite, beside values of few significant bits (1, powers of two, zero pieces): the infinity or NaN that
+    the definition gives, in the rows, ranks and columns that it has them in."""
+    d, K, N, R = _dev(), 72, 48, 5
+    g = torch.Generator(d).manual_seed(M)
+    pick = torch.tensor([1.0, 2.0, -1.0, 0.5, 1.5, -0.375, 3.0, 1.0 + 2.0 ** -7], device=d)
+
+    def values(*s):
+        return pick[torch.randint(0, len(pick), s, device=d, generator=g)]
+
+    x, a, b = values(M, K).to(BF), values(2, R, K).to(ad), values(2, N, R).to(ad)
+    x[1, 3], x[2, 5], x[3, 9] = float("inf"), float("-inf"), float("nan")
+    a[1, 2, 7] = float("inf")
+    b[1, 4, 1], b[1, 5, 3], b[1, 6, 0] = float("inf"), float("-inf"), float("nan")
+    x[4, 7] = 0  # times the infinite value of A: NaN
+    ids = torch.zeros(M, dtype=torch.int32, device=d)
+    ids[4:] = 1
+    # one rank: an infinite x times one row of A; then several
+    for r in (1, R):
+        A = ops.LoraAdapters(a[:, :r].contiguous(), b[:, :, :r].contiguous())
+        y = torch.zeros((M, N), dtype=t, device=d)
+        out = ops.lora_add(A, ids, x, y).double()
+        h = torch.einsum("mk,mrk->mr", x.double(), A.a.double()[ids.long()])
+        want = torch.einsum("mr,mnr->mn", h, A.b.double()[ids.long()])
+        live = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(out), live)
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want.isposinf())
+        # finite: few significant bits; h of 16 bits for a bf16 result
+        size = 3 * torch.einsum("mk,mnr->mn", x.double().abs(), A.b.double()[ids.long()].abs())  # |a| is at most 3
+        assert ((out - want).abs()[live] <= (want.abs() * 2.0 ** -8 + size * 2.0 ** -15)[live]).all()
+    # the sum over K is infinite: a finite x and A
+    x = torch.full((M, K), 2.0 ** 120, device=d).to(BF)
+    A = ops.LoraAdapters(torch.full((1, 1, K), 2.0 ** 15, device=d).to(ad), values(1, N, 1).to(ad))
+    out = ops.lora_add(A, torch.zeros(M, dtype=torch.int32, device=d), x, torch.zeros((M, N), dtype=t, device=d))
+    assert torch.equal(out, (A.b[0, :, 0].double().sign() * float("inf")).to(t).expand(M, N))
