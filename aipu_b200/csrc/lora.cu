@@ -136,7 +136,9 @@ struct LoraTile {
 };
 
 // ------------------------------------------------------------------ first product: this warp's k range
-template <int MT, int AT, bool VEC>
+// JOIN (fp32 results): the MMA's own sums are cut off and not rounded, so it sums 64 k at most, the small pieces first, and
+// the rest is rounded adds, as in the first product of many rows.
+template <int MT, int AT, bool VEC, bool JOIN>
 __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, const LoraTile& tl, int c0, int c1, int lane,
                                        float (&acc)[MT][4]) {
   constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1;  // k chunks loaded ahead
@@ -158,20 +160,29 @@ __device__ __forceinline__ void shrink(const LoraParams& p, const int* tok, cons
         }
       vx[u] = load8<VEC>(xrow + k, g < tl.rows ? valid : 0);
     }
+    constexpr int V = JOIN ? (U < 2 ? U : 2) : U;  // chunks that the MMA sums
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u0 = 0; u0 < U; u0 += V)
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if (16 * i >= tl.rank) continue;  // warp-uniform
-        if (AT == AD_F16) {
-          uint4 ah, al, bh, bl;
-          split4_f16(va[u][i][0], ah, al);
-          split4_f16(va[u][i][1], bh, bl);
-          mma_pair(acc[i], ah, bh, vx[u]);
-          mma_pair(acc[i], al, bl, vx[u]);
-        } else {
-          mma_pair(acc[i], va[u][i][0], va[u][i][1], vx[u]);
+        float sum[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[q] = JOIN ? 0.f : acc[i][q];
+#pragma unroll
+        for (int u = u0; u < u0 + V; ++u) {
+          if (AT == AD_F16) {
+            uint4 ah, al, bh, bl;
+            split4_f16(va[u][i][0], ah, al);
+            split4_f16(va[u][i][1], bh, bl);
+            mma_pair(sum, al, bl, vx[u]);
+            mma_pair(sum, ah, bh, vx[u]);
+          } else {
+            mma_pair(sum, va[u][i][0], va[u][i][1], vx[u]);
+          }
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i][q] = JOIN ? __fadd_rn(acc[i][q], sum[q]) : sum[q];
       }
   }
 }
@@ -367,7 +378,7 @@ __device__ __forceinline__ void expand_step(float (&acc)[NT][Q][4], const uint4 
       for (int s = NS - 1; s >= 0; --s) {
         const uint4 h = *reinterpret_cast<const uint4*>(hrow + s * hsplit);
         if (AT == AD_F16) {
-          if (s < 2) mma_pair(sum[0], l0, l1, h);  // (the third pieces' product is below 2^-24 of h b)
+          mma_pair(sum[0], l0, l1, h);
           mma_pair(sum[0], h0, h1, h);
         } else {
 #pragma unroll
@@ -482,7 +493,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads, 2)
     const int chunks = (p.K + 31) / 32;
     const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * gw / nw);
     const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (gw + 1) / nw);
-    shrink<MT, AT, VEC>(p, tok, tl, c0, c1, lane, acc);
+    shrink<MT, AT, VEC, O32>(p, tok, tl, c0, c1, lane, acc);
     // the first block's B rows are on the way while the sums are joined
     if (gw < nblk) load_b<4>(p, tl, gw * 64 + c8, 8 * t, vb);
     // ---- sums over the warps of the CTA, in warp order

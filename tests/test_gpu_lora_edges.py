@@ -258,3 +258,46 @@ def test_infinite_values_keep_their_signs_in_adapters(ad, M, t):
     A = ops.LoraAdapters(torch.full((1, 1, K), 2.0 ** 15, device=d).to(ad), values(1, N, 1).to(ad))
     out = ops.lora_add(A, torch.zeros(M, dtype=torch.int32, device=d), x, torch.zeros((M, N), dtype=t, device=d))
     assert torch.equal(out, (A.b[0, :, 0].double().sign() * float("inf")).to(t).expand(M, N))
+
+
+@pytest.mark.parametrize("ad", [BF, HF])
+@pytest.mark.parametrize("M", [5, 256, 300])
+def test_single_products_have_all_bits(ad, M):
+    """x = 1, a = 1, y = 0: scale * b. h holds the factor's 24 bits, b is exact, so what is off is the last product's sum:
+    one unit of fp32, 2^-23, for the MMA that adds the largest pieces and cuts off, and 2^-23 of the pieces before it,
+    2^-7 of the value, for each of the five MMAs of two steps that may have gone before."""
+    d, K, N, L = _dev(), 64, 72, 5
+    g = torch.Generator(d).manual_seed(M)
+    x = torch.zeros((M, K), device=d).to(BF)
+    x[:, 11] = 1
+    a = torch.zeros((L, 1, K), device=d).to(ad)
+    a[:, 0, 11] = 1
+    b = (1 + torch.rand((L, N, 1), device=d, generator=g)).to(ad) * torch.where(torch.rand((L, N, 1), device=d, generator=g) < 0.5, 1, -1).to(ad)
+    scale = 1 + torch.rand(L, device=d, generator=g)
+    # the largest rests: upper bits 0, lower bits all set
+    scale[0] = 1 + 2.0 ** -15 - 2.0 ** -23
+    b[0, 0, 0] = 1 + 7 * 2.0 ** -10 if ad == HF else 1
+    ids = (torch.arange(M, device=d) % L).to(torch.int32)
+    out = ops.lora_add(ops.LoraAdapters(a, b, scale), ids, x, torch.zeros((M, N), device=d))
+    want = (scale.double().view(L, 1) * b[:, :, 0].double())[ids.long()]
+    rel = ((out.double() - want).abs() / want.abs()).max()
+    assert rel <= 2.0 ** -23 * (1 + 10 * 2.0 ** -7), float(rel * 2 ** 23)
+
+
+@pytest.mark.parametrize("ad", [BF, HF])
+@pytest.mark.parametrize("M,K", [(8, 65536), (8, 1 << 20), (300, 65536)])
+def test_long_sums_of_one_sign_are_rounded_not_cut_off(ad, M, K):
+    """All of x and a positive: sums that are cut off fall short by half a unit a step, K / 16 of them. Root mean square of
+    the results' error, in 2^-24 of them: blocks of 64 k by the MMA, four steps (eight with fp16 pieces) of at most 2^-23 of
+    the block; rounded adds at random, at most sqrt of their number (K / 64 / 64 in a warp of the few rows' 64, K / 64 / 8 in
+    a share of the many rows', and the joins) of 1; the second product 2."""
+    d, N, R = _dev(), 40, 4
+    g = torch.Generator(d).manual_seed(K)
+    x = torch.rand((M, K), device=d, generator=g).to(BF)
+    a = torch.rand((1, R, K), device=d, generator=g).to(ad)
+    b = (1 + torch.arange(N * R, device=d) % 97).view(1, N, R).to(ad)  # exact
+    out = ops.lora_add(ops.LoraAdapters(a, b), torch.zeros(M, dtype=torch.int32, device=d), x, torch.zeros((M, N), device=d)).double()
+    want = (x.double() @ a[0].double().t()) @ b[0].double().t()
+    rms = float(((out - want) / want).square().mean().sqrt()) * 2 ** 24
+    adds = (K / 4096 + 15) if M <= 256 else K / 512 + 8
+    assert rms <= (8 if ad == BF else 16) + adds ** 0.5 + 2, rms
