@@ -31,9 +31,6 @@ __device__ __forceinline__ int scale_shift(float bound, int top) {
 // shift of a token row with an infinite value (top = 9): all its results are infinite or NaN by the upper halves alone (a
 // lower half of 0 or of the other sign would make NaN of an infinity)
 constexpr int kNotFinite = 255 - 127 - 9;
-// v * 2^e for |e| <= 252, in two steps of one sign, so that nothing is lost or overflows before the result does
-__device__ __forceinline__ float scale2(float v, int e) { return __fmul_rn(__fmul_rn(v, exp2i(e / 2)), exp2i(e - e / 2)); }
-
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -263,9 +260,10 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           break;
         }
         mbar_arrive_expect_tx(&bars.full[s], C::STAGE);
-        tma_load_2d(base + s * C::STAGE, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
+#pragma unroll
         for (int h = 0; h < P; ++h)  // (rows past N are of the other half or 0: their results are not stored)
-          tma_load_2d(base + s * C::STAGE + C::B + h * C::A, &p.wmap, 64 * (k0 + i), h * p.N + n0, &bars.full[s]);
+          tma_load_2d(base + s * C::STAGE + h * C::A, &p.wmap, 64 * (k0 + i), h * p.N + n0, &bars.full[s]);
+        tma_load_2d(base + s * C::STAGE + P * C::A, &p.xmap, 64 * (k0 + i), m0, &bars.full[s]);
       }
       // no copy may land after the CTA has ended: the MMAs have read them all, or (abort) they are waited for
       mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL);
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           break;
         }
         tc_fence_after();
-        const uint32_t b = base + s * C::STAGE, a = b + C::B;
+        const uint32_t a = base + s * C::STAGE, b = a + P * C::A;
 #pragma unroll
         for (int h = 0; h < P; ++h)
 #pragma unroll
@@ -298,7 +296,8 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
     for (int i = tid; i < NT; i += 256) xs[i] = m0 + i < p.M ? p.xshift[m0 + i] : 0;
     named_bar_sync(1, 256);
     const int q = warp & 3, n = n0 + 32 * q + lane;
-    const int ws = (p.wshift && n < p.N) ? p.wshift[n] : 0;
+    // (the weights' factor first: finite ones have shifts of -41 to 13, so nothing is lost or overflows before the result does)
+    const float wf = exp2i((p.wshift && n < p.N) ? p.wshift[n] : 0);
     const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL)) && !*abort;
     if (ok) {
       tc_fence_after();
@@ -317,7 +316,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
           float* dst = p.y + (static_cast<int64_t>(blockIdx.z) * p.M + m0 + c0) * p.ldy + n;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c0 + j < cols) dst[j * p.ldy] = scale2(v[j], xs[c0 + j] + ws);
+            if (c0 + j < cols) dst[j * p.ldy] = __fmul_rn(__fmul_rn(v[j], wf), exp2i(xs[c0 + j]));
         }
       }
     }
