@@ -1384,9 +1384,15 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
   return lora_finish(p, s, pdl || p.tiles);
 }
 
-// whether the projection dequantises its weights once and runs as an fp16 GEMM: above the rows of one decode GEMV
-// launch, and where a row does not fit the GEMV
-static bool gemm_lora_dense(int64_t M, int64_t K) { return M > 8 || K > kGemvMaxK; }
+// Whether the projection dequantises its weights once and runs as an fp16 GEMM, or as launches of the decode GEMV of up to 8
+// rows each. Two launches read 1.1 bytes a weight (Q4_K) and the GEMM's halves take 4 to write and 4 to read: 9 / 16
+// rows by launches and by the GEMM, us: Q4_K 6144 x 2048 35 / 33 and 28 / 28, 4096 x 4096 28 / 36 and 33 / 34, 4096 x 11008 44 / 46
+// and 90 / 91, 8192 x 8192 60 / 58 and 116 / 116; Q6_K 4096 x 4096 33 / 40 and 37 / 38, 8192 x 8192 82 / 136 and 132 / 133;
+// Q8_0 4096 x 1003 23 / 28 and 16 / 17, 6144 x 6144 53 / 69 and 74 / 74. Three launches (24 rows): 51 against 35 at Q4_K 4096 x
+// 4096, 84 against 117 at 8192 x 8192, Q6_K 200 against 134. F16 weights are read as they are stored: 29 / 31 and 17 / 17.
+static bool gemm_lora_dense(int wtype, int64_t N, int64_t K, int64_t M) {
+  return K > kGemvMaxK || M > 16 || (M > 8 && (wtype == AIPU_F16 || N * K < (1 << 24)));
+}
 // row stride of its fp32 sums: rows start on 32 bytes
 static int64_t gemm_lora_ld(int64_t N) { return (N + 7) & ~static_cast<int64_t>(7); }
 
@@ -1394,9 +1400,9 @@ extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K,
   if (N <= 0 || K <= 0 || M <= 0 || M > (1 << 24) || N > (1 << 24) || aipu_row_bytes(wtype, K) == 0 || K % 256 || n_adapters < 1 ||
       n_adapters > 32768 || rank < 1 || rank > 128)
     return 0;
-  const size_t parts = gemm_lora_dense(M, K) ? dense_parts(N, K, M) : 1;
+  const size_t parts = gemm_lora_dense(wtype, N, K, M) ? dense_parts(N, K, M) : 1;
   size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * parts * M * gemm_lora_ld(N));
-  if (gemm_lora_dense(M, K)) b += dense_bytes(wtype, N, K, M);
+  if (gemm_lora_dense(wtype, N, K, M)) b += dense_bytes(wtype, N, K, M);
   return static_cast<int64_t>(b);
 }
 
@@ -1421,7 +1427,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   void* plan = b;
   b += al256x(lora_plan_bytes(M, p.L, p.R));
   float* y32 = reinterpret_cast<float*>(b);
-  if (gemm_lora_dense(M, K)) p.yparts = dense_parts(N, K, M);
+  if (gemm_lora_dense(wtype, N, K, M)) p.yparts = dense_parts(N, K, M);
   b += al256x(4 * static_cast<size_t>(std::max(p.yparts, 1)) * M * gemm_lora_ld(N));
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = K;
@@ -1433,7 +1439,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
   p.y_f32 = 1;
   p.status = c->status;
   if ((rc = lora_begin(p, plan, s, false))) return rc;
-  if (gemm_lora_dense(M, K)) {
+  if (gemm_lora_dense(wtype, N, K, M)) {
     // (beside the first product of the adapters, which was launched just before where there are many rows)
     rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, p.ldy, b, c->status, s, p.tiles != nullptr);
   } else {

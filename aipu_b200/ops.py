@@ -446,8 +446,8 @@ def lora_add(ad: LoraAdapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tens
 def gemm_lora(wtype: int, w: torch.Tensor, N: int, K: int, x: torch.Tensor, ad: LoraAdapters, ids: torch.Tensor,
               ctx: Optional[Context] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[m] bf16 = x[m] W^T + scale[l] * (x[m] a[l]^T) b[l]^T with l = ids[m]: a shared quantised projection (W = N GGUF rows
-    of K weights, as in gemm) and the adapters of its rows, rounded once. Up to 8 rows run on the decode GEMV, more on a
-    tensor-core GEMM that takes the weights as two fp16 halves (22 bits). out must not overlap the inputs."""
+    of K weights, as in gemm) and the adapters of its rows, rounded once. Up to 8 rows run on the decode GEMV (up
+    to 16 of large weights), more on a tensor-core GEMM that takes the weights as two fp16 halves (22 bits). out must not overlap the inputs."""
     M = _lora_inputs(ids, x)
     cs = ad.cstruct()
     if x.shape[1] != K or cs.in_features != K or cs.out_features != N:

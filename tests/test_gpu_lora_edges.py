@@ -301,3 +301,23 @@ def test_long_sums_of_one_sign_are_rounded_not_cut_off(ad, M, K):
     rms = float(((out - want) / want).square().mean().sqrt()) * 2 ** 24
     adds = (K / 4096 + 15) if M <= 256 else K / 512 + 8
     assert rms <= (8 if ad == BF else 16) + adds ** 0.5 + 2, rms
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("K,N", [(4096, 4096), (4096, 4088), (11008, 1600)])
+def test_9_to_17_rows_of_large_weights(wt, K, N):
+    """On both sides of the borders between launches of the GEMV and the fp16 GEMM, in the rows and in the weights. Tolerance
+    as for few rows of long weights."""
+    d = _dev()
+    w, wd = _weights(wt, N, K, 3, d)
+    x = torch.randn((17, K), device=d, generator=torch.Generator(d).manual_seed(K)).to(BF)
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    if wt == F.Q4_K:
+        dm = w.view(-1, 144)[:, 2:4].contiguous().view(HF).double().view(N, K // 256)
+        mag = mag + 2 * 63 * (x.double().abs().view(17, -1, 256).sum(2) @ dm.abs().t())
+    tol = mag * (K / 16 * 2.0 ** -23)
+    tol = tol + (want.abs() + tol) * 2.0 ** -8
+    for M in (9, 12, 16, 17):
+        ids = torch.full((M,), -1, dtype=torch.int32, device=d)
+        got = ops.gemm_lora(wt, w, N, K, x[:M], _plain(d, K, N), ids).double()
+        assert ((got - want[:M]).abs() <= tol[:M]).all(), M
