@@ -1485,12 +1485,13 @@ extern "C" int aipu_logits_process(aipu_ctx* c, const void* logits, int dtype, i
   if (off(logits, dtype == AIPU_DT_F32 ? 4 : 2) || off(out, 4) || off(token, 4))
     return set_error(EINVAL_, "logits_process: logits, out or token not aligned to their type");
   if (ctl) {
-    if ((ctl->spans != nullptr) != (ctl->penalties != nullptr) || ctl->n_tokens < 0 || ctl->n_tokens > INT32_MAX ||
+    // (no rows: an array of theirs has no elements and may be null)
+    if ((M > 0 && (ctl->spans != nullptr) != (ctl->penalties != nullptr)) || ctl->n_tokens < 0 || ctl->n_tokens > INT32_MAX ||
         (ctl->n_tokens > 0 && !ctl->tokens))
       return set_error(EINVAL_, "logits_process: penalties need spans, and tokens for them (at most 2^31 - 1)");
     if (ctl->n_bias < 0 || (ctl->bias_begin && ctl->n_bias > 0 && (!ctl->bias_ids || !ctl->bias_vals)))
       return set_error(EINVAL_, "logits_process: biases need ids and values");
-    if ((ctl->mask != nullptr) != (ctl->mask_rows != nullptr) || (ctl->mask && (ctl->n_masks < 1 || ctl->n_masks > INT32_MAX)))
+    if ((M > 0 && (ctl->mask != nullptr) != (ctl->mask_rows != nullptr)) || (ctl->mask && (ctl->n_masks < 1 || ctl->n_masks > INT32_MAX)))
       return set_error(EINVAL_, "logits_process: masks need mask_rows and at least one mask");
     if (off(ctl->tokens, 4) || off(ctl->spans, 8) || off(ctl->penalties, 4) || off(ctl->bias_begin, 8) || off(ctl->bias_ids, 4) ||
         off(ctl->bias_vals, 4) || off(ctl->mask, 4) || off(ctl->mask_rows, 4))

@@ -196,3 +196,10 @@ def test_structs_match_the_header():
     """Field for field in the header's order (all 8-byte fields but the adapters' first two)."""
     assert ctypes.sizeof(_lib.Lora) == 8 + 7 * 8 and _lib.Lora.rank.offset == 8 and _lib.Lora.ranks.offset == 56
     assert ctypes.sizeof(_lib.LogitCtl) == 11 * 8
+
+
+def test_no_rows_need_no_row_arrays():
+    """An empty batch: its per-row arrays have no elements and may be null, whatever else the controls hold."""
+    for kw in (dict(mask_rows=None), dict(spans=None, penalties=None), dict(spans=None), dict(penalties=None)):
+        assert _process(M=0, x=None, out=None, token=None, ctl=_ctl(**kw)) == _lib.AIPU_EINVAL
+        assert b"null context" in _lib.lib().aipu_last_error()  # the last thing that is checked
