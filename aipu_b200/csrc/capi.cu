@@ -1486,9 +1486,9 @@ extern "C" int aipu_logits_process(aipu_ctx* c, const void* logits, int dtype, i
     return set_error(EINVAL_, "logits_process: logits, out or token not aligned to their type");
   if (ctl) {
     // (no rows: an array of theirs has no elements and may be null)
-    if ((M > 0 && (ctl->spans != nullptr) != (ctl->penalties != nullptr)) || ctl->n_tokens < 0 || ctl->n_tokens > INT32_MAX ||
+    if ((M > 0 && (ctl->spans != nullptr) != (ctl->penalties != nullptr)) || ctl->n_tokens < 0 || ctl->n_tokens >= (1 << 30) ||
         (ctl->n_tokens > 0 && !ctl->tokens))
-      return set_error(EINVAL_, "logits_process: penalties need spans, and tokens for them (at most 2^31 - 1)");
+      return set_error(EINVAL_, "logits_process: penalties need spans, and tokens for them (fewer than 2^30)");
     if (ctl->n_bias < 0 || (ctl->bias_begin && ctl->n_bias > 0 && (!ctl->bias_ids || !ctl->bias_vals)))
       return set_error(EINVAL_, "logits_process: biases need ids and values");
     if ((M > 0 && (ctl->mask != nullptr) != (ctl->mask_rows != nullptr)) || (ctl->mask && (ctl->n_masks < 1 || ctl->n_masks > INT32_MAX)))

@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(T, T == 256 ? 4 : 1) aipu_logits_kernel(const 
   bool bad = false;
   // ---- the row's controls
   RowPenalty pen = {1.f, 0.f, 0.f};
-  int cb = 0, cg = 0, ce = 0;  // (at most 2^31 - 1 tokens)
+  int cb = 0, cg = 0, ce = 0;  // (fewer than 2^30 tokens: a count fits below the marks of a 32-bit field)
   if (p.spans) {
     const int64_t b = p.spans[3 * m], g = p.spans[3 * m + 1], e = p.spans[3 * m + 2];
     cb = static_cast<int>(min(max(b, static_cast<int64_t>(0)), p.n_tokens));

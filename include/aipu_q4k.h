@@ -302,7 +302,7 @@ int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64
 typedef struct aipu_logit_ctl {
   /* penalties: row m's context is tokens[begin, end), of which tokens[gen, end) were generated, with
    * (begin, gen, end) = spans[3 m ..]; contexts may overlap. penalties[3 m ..] = repetition, presence,
-   * frequency (1, 0, 0: none). Tokens outside 0 .. V - 1 count for nothing. */
+   * frequency (1, 0, 0: none). Tokens outside 0 .. V - 1 count for nothing. n_tokens is below 2^30. */
   const int32_t* tokens;
   int64_t n_tokens;
   const int64_t* spans;     /* [M, 3] */

@@ -203,3 +203,10 @@ def test_no_rows_need_no_row_arrays():
     for kw in (dict(mask_rows=None), dict(spans=None, penalties=None), dict(spans=None), dict(penalties=None)):
         assert _process(M=0, x=None, out=None, token=None, ctl=_ctl(**kw)) == _lib.AIPU_EINVAL
         assert b"null context" in _lib.lib().aipu_last_error()  # the last thing that is checked
+
+
+@pytest.mark.parametrize("n,text", [(1 << 30, b"penalties need"), ((1 << 30) - 1, b"null context")])
+def test_contexts_are_as_long_as_their_counts(n, text):
+    """A token's count has 30 bits."""
+    assert _process(ctl=_ctl(n_tokens=n)) == _lib.AIPU_EINVAL
+    assert text in _lib.lib().aipu_last_error()
