@@ -1419,6 +1419,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     return set_error(EINVAL_, "gemm_lora: weights and activations must be 16-byte aligned, the result to its type");
   if ((M > 0 && !ws) || (reinterpret_cast<uintptr_t>(ws) & 255u) || ws_bytes < aipu_q4k_gemm_lora_workspace(wtype, N, K, M, p.L, p.R))
     return set_error(EINVAL_, "gemm_lora: workspace missing, too small or not 256-byte aligned");
+  if (gemm_lora_dense(wtype, N, K, M) && M > kDenseMaxRows) return set_error(EINVAL_, "gemm_lora: too many rows for one launch");
   if (!c) return set_error(EINVAL_, "gemm_lora: null context");
   if (M == 0) return OK;
   DeviceGuard dg(c->device);

@@ -7,6 +7,8 @@
 
 namespace aipu {
 
+// token rows of one launch: 65535 tiles of 256
+constexpr int64_t kDenseMaxRows = 65535 * 256;
 // scratch of dense_gemm for N weight rows of type wt, K and M token rows
 size_t dense_bytes(int wt, int64_t N, int64_t K, int64_t M);
 // shares of K of the result of dense_gemm

@@ -210,3 +210,11 @@ def test_contexts_are_as_long_as_their_counts(n, text):
     """A token's count has 30 bits."""
     assert _process(ctl=_ctl(n_tokens=n)) == _lib.AIPU_EINVAL
     assert text in _lib.lib().aipu_last_error()
+
+
+@pytest.mark.parametrize("M,text", [(1 << 24, b"too many rows"), ((1 << 24) - 256, b"null context")])
+def test_projection_refuses_more_rows_than_its_grid(M, text):
+    """65535 tiles of 256 rows."""
+    L = _lib.lib()
+    assert L.aipu_q4k_gemm_lora(None, 0, 16, 32, 256, 16, M, _lora(), 16, 16, 256, 1 << 50, None) == _lib.AIPU_EINVAL
+    assert text in L.aipu_last_error()
