@@ -59,12 +59,18 @@ class SpecStats:
         return self.committed / self.passes if self.passes else 0.0
 
 
+def _allows(words: torch.Tensor, token: int) -> bool:
+    """Whether packed mask words allow a token."""
+    return 0 <= token < 32 * words.numel() and bool(int(words[token // 32]) >> (token % 32) & 1)
+
+
 @dataclass
 class Request:
     """One request: its context (the last token is the next pass's input), of which the first n_prompt tokens were
     given and the rest generated, and the controls of its tokens. mask(context) gives the packed mask words (int32
-    [ceil(V / 32)], ops.pack_mask) of the token that follows a context, or None for no mask. adapter: its row in the
-    verifier's head adapters, negative for none."""
+    [ceil(V / 32)], ops.pack_mask) of the token that follows a context, or None for no mask. It is asked about the context
+    and about the context with drafts that its own masks allow, and its words are read on the host where drafts follow.
+    adapter: its row in the verifier's head adapters, negative for none."""
 
     context: List[int]
     n_prompt: int = 0
@@ -91,13 +97,16 @@ class Request:
             c.bias_ids = torch.tensor(list(self.bias.keys()) * M, dtype=torch.int32, device=device)
             c.bias_vals = torch.tensor(list(self.bias.values()) * M, dtype=torch.float32, device=device)
         if self.mask is not None:
-            words = [self.mask(tokens[:n + j]) for j in range(M)]
-            live = [w for w in words if w is not None]
+            rows, live = [-1] * M, []
+            for j in range(M):
+                words = self.mask(tokens[:n + j])
+                if words is None:
+                    continue
+                rows[j] = len(live)
+                live.append(words)
+                if j < M - 1 and not _allows(words, tokens[n + j]):
+                    break  # that draft is not accepted, so the rows behind it count for nothing
             if live:
-                rows, at = [], 0
-                for w in words:
-                    rows.append(-1 if w is None else at)
-                    at += w is not None
                 c.mask = torch.stack([w.to(device) for w in live]).contiguous()
                 c.mask_rows = torch.tensor(rows, dtype=torch.int32, device=device)
         return c
