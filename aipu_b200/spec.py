@@ -84,6 +84,8 @@ class Request:
     def controls(self, drafts: Sequence[int], device) -> ops.LogitControls:
         """Controls of the rows {context, context + d_1, ..}: one shared run of tokens, each row's context ends at its
         own input token."""
+        if self.n_prompt < 0:
+            raise ValueError("n_prompt must not be negative")
         M, n = len(drafts) + 1, len(self.context)
         tokens = list(self.context) + [int(d) for d in drafts]
         spans = [[0, min(self.n_prompt, n), n + j] for j in range(M)]
@@ -145,13 +147,19 @@ class SpecVerifier:
 
     def greedy_tokens(self, rows: Sequence[int], request: Optional[Request] = None) -> List[int]:
         """m_j = argmax of the LM head over the stack's output for token row j (lowest index on ties); for a request, of
-        its adapted logits under its controls (-1 where its mask leaves nothing)."""
-        idx = torch.as_tensor(list(rows), dtype=torch.long, device=self.emb.device)
+        its adapted logits under its controls (-1 where its mask leaves nothing), whose context ends with the first row."""
+        rows = list(rows)
+        if request is not None:
+            if not request.context or not rows or request.context[-1] != rows[0]:
+                raise ValueError("a request's context must end with cur_tok")
+            if request.adapter >= 0 and (self.head_adapters is None or request.adapter >= self.head_adapters.a.shape[0]):
+                raise ValueError("the request names an adapter that the verifier does not have")
+        idx = torch.as_tensor(rows, dtype=torch.long, device=self.emb.device)
         h = self._stack(self.emb.index_select(0, idx).contiguous())
         logits = ops.bf16_dot_gemv(self.lm_head, h, ctx=self.ctx)
         if request is None:
             return [int(v) for v in logits.float().argmax(dim=1).cpu().tolist()]
-        if self.head_adapters is not None and request.adapter >= 0:
+        if request.adapter >= 0:
             ids = torch.full((len(rows),), request.adapter, dtype=torch.int32, device=h.device)
             logits = ops.lora_add(self.head_adapters, ids, h, logits, out=logits, ctx=self.ctx)
         return ops.greedy_tokens(logits, request.controls(rows[1:], h.device), ctx=self.ctx).cpu().tolist()
@@ -159,11 +167,6 @@ class SpecVerifier:
     def verify(self, cur_tok: int, drafts: Sequence[int], request: Optional[Request] = None):
         """One pass over {cur_tok, d_1..d_K}: returns (committed tokens m_1..m_{p+1}, p). A request's context must end
         with cur_tok; the committed tokens are added to it. Where its mask leaves no token, the committed ones end."""
-        if request is not None:
-            if not request.context or request.context[-1] != cur_tok:
-                raise ValueError("a request's context must end with cur_tok")
-            if request.adapter >= 0 and (self.head_adapters is None or request.adapter >= self.head_adapters.a.shape[0]):
-                raise ValueError("the request names an adapter that the verifier does not have")
         rows = [cur_tok] + list(drafts)
         truth = self.greedy_tokens(rows) if request is None else self.greedy_tokens(rows, request)
         p = longest_accepted_prefix(drafts, truth)

@@ -43,6 +43,19 @@ def test_a_context_without_a_mask_allows_every_draft():
     assert len(g.asked) == 3 and c.mask_rows.tolist() == [-1, 0, 1, -1, -1]
 
 
+def test_verify_rows_need_their_request():
+    e = torch.zeros((V, 8), dtype=torch.bfloat16)
+    v = SpecVerifier(e, e, lambda h: h)
+    ad = ops.LoraAdapters(torch.zeros((2, 1, 8), dtype=torch.bfloat16), torch.zeros((2, V, 1), dtype=torch.bfloat16))
+    w = SpecVerifier(e, e, lambda h: h, head_adapters=ad)
+    for sv, q in ((v, Request(context=[4])), (v, Request(context=[])), (v, Request(context=[3], adapter=0)), (w, Request(context=[3], adapter=2))):
+        for call in (lambda: sv.greedy_tokens([3, 5], q), lambda: sv.verify(3, [5], q)):
+            with pytest.raises(ValueError, match="context must end with|does not have"):
+                call()
+    with pytest.raises(ValueError, match="n_prompt"):
+        Request(context=[3], n_prompt=-1).controls([], "cpu")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [1, 3, 9])
 def test_drafts_that_the_grammar_refuses_change_nothing(k):
