@@ -154,6 +154,8 @@ class SpecVerifier:
                 raise ValueError("a request's context must end with cur_tok")
             if request.adapter >= 0 and (self.head_adapters is None or request.adapter >= self.head_adapters.a.shape[0]):
                 raise ValueError("the request names an adapter that the verifier does not have")
+        if not all(0 <= t < self.emb.shape[0] for t in rows):
+            raise ValueError("a token is outside the embedding")
         idx = torch.as_tensor(rows, dtype=torch.long, device=self.emb.device)
         h = self._stack(self.emb.index_select(0, idx).contiguous())
         logits = ops.bf16_dot_gemv(self.lm_head, h, ctx=self.ctx)

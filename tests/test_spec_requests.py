@@ -56,6 +56,17 @@ def test_verify_rows_need_their_request():
         Request(context=[3], n_prompt=-1).controls([], "cpu")
 
 
+@pytest.mark.parametrize("rows", [[V], [-1], [3, V], [3, 5, 1 << 40]])
+def test_tokens_outside_the_embedding_are_refused(rows):
+    """Before the device looks them up."""
+    e = torch.zeros((V, 8), dtype=torch.bfloat16)
+    v = SpecVerifier(e, e, lambda h: h)
+    with pytest.raises(ValueError, match="outside"):
+        v.greedy_tokens(rows)
+    with pytest.raises(ValueError, match="outside"):
+        v.verify(rows[0], rows[1:], Request(context=rows[:1]))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [1, 3, 9])
 def test_drafts_that_the_grammar_refuses_change_nothing(k):
