@@ -321,3 +321,53 @@ def test_9_to_17_rows_of_large_weights(wt, K, N):
         ids = torch.full((M,), -1, dtype=torch.int32, device=d)
         got = ops.gemm_lora(wt, w, N, K, x[:M], _plain(d, K, N), ids).double()
         assert ((got - want[:M]).abs() <= tol[:M]).all(), M
+
+
+@pytest.mark.parametrize("N", [32000, 128000, 50257])
+@pytest.mark.parametrize("M,R", [(1, 16), (5, 64), (8, 13), (9, 128)])
+@pytest.mark.parametrize("t", [BF, FP])
+def test_few_rows_of_one_adapter_on_a_vocabulary(N, M, R, t):
+    """The LM head's adapter in a verify pass, in place. Off by the result's rounding, by h's 16 bits (bf16 results) and by
+    the sums of K and R products, at most 2^-23 of the magnitudes for each 16 terms and join."""
+    d, K = _dev(), 512
+    g = torch.Generator(d).manual_seed(N + M)
+    a = (torch.randn((2, R, K), device=d, generator=g) * K ** -0.5).to(BF)
+    b = (torch.randn((2, N, R), device=d, generator=g) * R ** -0.5).to(BF)
+    x = torch.randn((M, K), device=d, generator=g).to(BF)
+    y = torch.randn((M, N), device=d, generator=g).to(t)
+    want, size = y.double(), (x.double().abs() @ a[1].double().abs().t()) @ b[1].double().abs().t()
+    want = want + (x.double() @ a[1].double().t()) @ b[1].double().t()
+    ids = torch.ones(M, dtype=torch.int32, device=d)
+    assert ops.lora_add(ops.LoraAdapters(a, b), ids, x, y, out=y) is y
+    tol = size * ((K / 16 + 64 + R) * 2.0 ** -23 + (2.0 ** -15 if t == BF else 0))
+    tol = tol + (want.abs() + tol) * (2.0 ** -8 if t == BF else 2.0 ** -23)
+    assert ((y.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M", [1, 8, 12, 20, 300])
+@pytest.mark.parametrize("wt", [F.Q4_K, F.F16])
+def test_projection_with_the_programmatic_flag(M, wt):
+    """Behind the kernel that writes x and before the next call that reads the result, on a context with the flag."""
+    d, K, N = _dev(), 1024, 512
+    w, _ = _weights(wt, N, K, 1, d)
+    g = torch.Generator(d).manual_seed(M)
+    A = ops.LoraAdapters((torch.randn((3, 16, K), device=d, generator=g) * K ** -0.5).to(BF), torch.randn((3, N, 16), device=d, generator=g).to(BF))
+    back = ops.LoraAdapters((torch.randn((3, 16, N), device=d, generator=g) * 1e-3).to(BF), torch.randn((3, K, 16), device=d, generator=g).to(BF))
+    x0 = torch.randn((M, K), device=d, generator=g).to(BF)
+    ids = (torch.arange(M, device=d) % 4 - 1).to(torch.int32)
+    ctx, flagged = ops.Context(d), ops.Context(d).set_flags(pdl=True)
+
+    def chain(c):
+        x = x0 + 0
+        for _ in range(4):
+            y = ops.gemm_lora(wt, w, N, K, x, A, ids, ctx=c)
+            x = ops.lora_add(back, ids, y, x0, ctx=c)
+        return y, x
+
+    want = chain(ctx)
+    for _ in range(10):
+        got = chain(flagged)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert ctx.status() == 0 and flagged.status() == 0
+    ctx.close()
+    flagged.close()
