@@ -992,7 +992,7 @@ __device__ __forceinline__ void stage_token_vec(const uint4 q, float sc, uint8_t
 // Four and more tokens (a kernel variant of its own: the code of fewer tokens stays as short as it is): a warp
 // per token, so that all tokens' loads are in flight at once and no barrier stands between the maxima and
 // the conversion, whose loads come from L1. The values are those of gemv_stage_x. 4096 x 4096, Q4_K, 8 / 4
-// tokens: 17.6 / 11.9 -> 15.5 / 11.0 us, 4 fp32 tokens 26.3 -> 19.0 (3 fp32 tokens would take 19 against 15).
+// tokens: 17.6 / 11.9 -> 15.5 / 11.0 us, 4 fp32 tokens 26.3 -> 18.7 (3 fp32 tokens would take 19 against 15).
 // Leaves with a __syncthreads.
 template <int WT, int XT>
 __device__ __forceinline__ void gemv_stage_tokens(const GemvParams& p, uint8_t* smem, const GemvLayout& L, int grp, int xs_slot,

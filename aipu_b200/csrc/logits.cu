@@ -12,8 +12,8 @@
 //
 // Bound: each logit is read once and each result written once; the rest (contexts, masks, biases) is
 // small, so the operator should be bound by memory for many rows and by latency for one. Measured (device time in
-// a graph): 64 bf16 rows of 128000 14.7 us without controls (3.3 TB/s), 33 us with contexts of 4000 to 8000
-// tokens, biases and masks; 256 fp32 rows of 50001 30 and 41 us; one row of 32000 3.6 and 7.0 us.
+// a graph): 64 bf16 rows of 128000 14.7 us without controls (3.3 TB/s), 31 us with contexts of 4000 to 8000
+// tokens, biases and masks; 256 fp32 rows of 50001 30 and 40 us; one row of 32000 3.6 and 6.9 us.
 //
 // One cluster of CTAs takes one row; blocks of tokens go to its CTAs in turn (frequent tokens are
 // neighbours, and their counting should not fall to one CTA). The counts of a CTA's blocks are built in its

@@ -25,7 +25,7 @@ struct LogitParams {
   int64_t ldo;
   int32_t* token;             // [M] greedy token (nullable)
   int* status;
-  int blocks;                 // set by the launch: blocks of 256 tokens of one CTA and window
+  int blocks;                 // set by the launch: blocks (256 bf16 or 128 fp32 tokens) of one CTA and window
 };
 
 int logits_launch(LogitParams p, int num_sms, cudaStream_t s, bool pdl);

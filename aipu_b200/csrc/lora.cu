@@ -18,16 +18,18 @@
 //   3. CTA c and its warps each take 64-column blocks of N. The MMA's rows are columns of y, ordered so
 //      that a lane ends with 8 consecutive columns of a row: y is read and written 16 bytes at a time.
 //   h never leaves the chip, and the reads of B and y do not wait for the sums of A.
-//   (4096 x 4096, device time in a graph: 1 row of rank 16 5.8 us, 64 rows of 32 adapters of rank 16 to 64 9.2 us.)
+//   (4096 x 4096, device time in a graph: 1 row of rank 16 5.8 us, 64 rows of 32 adapters of rank 16 to 64 9.1 us.)
 // More rows: a plan (rows ordered by adapter, tiles of up to 64 of them), the first product (a tile and a
 // share of K a CTA: x and A stream through a ring of asynchronous copies in shared memory, partial sums to
 // global memory), the second product (a tile and a share of N a CTA: step 3 above, 32 columns a warp). 4096 rows of
 // eight adapters of rank 32, 6144 x 2048: 33 us, 88 MB at 2.7 TB/s; as one cluster kernel 119 us, because its
 // phases followed one another with one CTA an SM.
 //
-// Rounding: bf16 x and A products are exact in the MMA, sums are fp32. h is not rounded to 16 bits: it
-// enters the second product as 2 (bf16 result) or 3 (fp32 result) bf16 pieces, 16 and 24 bits. fp16
-// adapters enter as two bf16 pieces (11 bits: exact).
+// Rounding: bf16 x and A products are exact in the MMA, sums are fp32: the MMA's own, which are cut off, over 64 k (and 32
+// ranks, fp32 results), then rounded adds. h enters the second product as 2 (bf16 result) or 3 (fp32 result) bf16 pieces, 16 and
+// 24 bits: for a bf16 result 2^-16 of h is 2^-8 of its own rounding, and a third piece would take Q6_K 2048 x 6144, 8
+// rows, from 19.4 to 21.9 us and 4096 rows of rank 128, 4096 x 4096, from 82 to 128. fp16 adapters enter as two bf16 pieces
+// (11 bits: exact).
 #include <algorithm>
 #include <cstdint>
 
@@ -556,7 +558,7 @@ __global__ void __cluster_dims__(kDirectCtas) __launch_bounds__(kLoraThreads, 2)
 
 // ------------------------------------------------------------------ many rows: first product
 constexpr int kTile = 64;    // rows of a tile
-// ring of 64-wide k chunks: two CTAs' rings fill an SM's shared memory (80 KB on their way an SM where rank <= 32)
+// ring of 64-wide k chunks: two CTAs' rings of 80 to 96 KB fill an SM's shared memory
 template <int MT>
 constexpr int kStages = MT == 1 ? 8 : MT == 2 ? 7 : MT == 4 ? 6 : 4;
 constexpr int kMaxSplit = 8; // shares of K
@@ -1003,7 +1005,8 @@ __global__ void __launch_bounds__(1024) aipu_lora_plan_kernel(const int32_t* __r
 static size_t al256l(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 static int64_t max_tiles(int64_t M, int64_t L) { return M / kTile + std::min<int64_t>(L + 1, M); }
 static int padded_rank(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
-// shares of K: about two CTAs an SM over the tiles that M rows and L adapters make (148 SMs)
+// shares of K: about two CTAs an SM over the tiles that M rows and L adapters make (a B200's 148 SMs: the workspace is
+// sized without a context)
 static int k_split(int64_t M, int64_t L) {
   const int64_t tiles = std::max<int64_t>(1, M / kTile + std::min<int64_t>(L, M) / 2);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 296 / tiles)));

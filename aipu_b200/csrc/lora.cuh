@@ -28,7 +28,7 @@ struct LoraParams {
   int wait_y;            // 1: y comes from the kernel launched just before lora_finish's (programmatic launch)
   // set by lora_begin
   int32_t* perm;         // rows ordered by adapter (more rows than one launch takes: tiles is set)
-  int4* tiles;           // {adapter or -1, first position in perm, rows, 0}
+  int4* tiles;           // {adapter or -1, first position in perm, rows, the adapter's rank}
   int32_t* n_tiles;
   float* sums;           // [ksplit][M][rp] shares of h by position
   int ksplit, nsplit;    // shares of K and of N

@@ -281,7 +281,8 @@ typedef struct aipu_lora {
  * ws: device scratch of aipu_lora_workspace(M, n_adapters, rank) bytes (NULL when that is 0), in use until
  * the call's work on `stream` is done. Nothing else is shared, so calls with their own ws may run at the
  * same time. Equal calls give equal bits; in calls of up to 256 rows a row's bits do not depend on the other
- * rows. No counterpart in the reference. */
+ * rows (above that K is shared out by the numbers of rows and adapters, and the order of its sums with it). No
+ * counterpart in the reference. */
 int64_t aipu_lora_workspace(int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const void* x, int64_t ldx, int64_t M,
                   const void* y, int y_dtype, int64_t ldy, void* out, int out_dtype, int64_t ldo, void* ws,
@@ -324,7 +325,8 @@ typedef struct aipu_logit_ctl {
  *   z = z > 0 ? z / repetition : z * repetition   if the token occurs in the row's context
  *   z = z - frequency * count, z = z - presence   if it occurs count > 0 times in the generated part
  *   z = z + bias                                  every entry of the row for the token, in list order (ids
- *                                                 outside 0 .. V - 1 count for nothing)
+ *                                                 outside 0 .. V - 1 count for nothing; an entry of a token
+ *                                                 that has several looks through the list)
  *   z = -inf                                      if the row's mask does not allow it
  * token = the lowest index of the largest z (NaN is never the largest), -1 if no z is above -inf (a mask
  * that leaves nothing). ctl may be NULL. out may be logits (fp32, same stride). A span or bias range that
