@@ -12,7 +12,8 @@
 // 2^-24 of the row's largest lose bits). A weight is dequantised in fp32 as ggml defines it, scaled by a
 // power of two per row, and enters as two fp16 halves, 22 bits (2^-38 of the row's bound where it is small), whose
 // products go to accumulators of their own and are added once. One half alone would round it by 2^-11 and change every
-// tenth bf16 result (and the call of that case would take 79 us for 111). F16 weights are used as they are stored, in one product. Products are exact, sums fp32.
+// tenth bf16 result (and the call of that case would take 79 us for 111). F16 weights are used as they are stored, in one
+// product. Products are exact, sums fp32.
 #include <algorithm>
 
 #include "deq.cuh"
@@ -34,6 +35,7 @@ __device__ __forceinline__ int scale_shift(float bound, int top) {
 // shift of a token row with an infinite value (top = 9): all its results are infinite or NaN by the upper halves alone (a
 // lower half of 0 or of the other sign would make NaN of an infinity)
 constexpr int kNotFinite = 255 - 127 - 9;
+
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kDenseThreads, 1) aipu_dense_gemm_kernel(const
     for (int i = tid; i < NT; i += 256) xs[i] = m0 + i < p.M ? p.xshift[m0 + i] : 0;
     named_bar_sync(1, 256);
     const int q = warp & 3, n = n0 + 32 * q + lane;
-    // (the weights' factor first: finite ones have shifts of -41 to 13, so nothing is lost or overflows before the result does)
+    // (the weights' factor first: finite ones have shifts of -32 to 13, so nothing is lost or overflows before the result does)
     const float wf = exp2i((p.wshift && n < p.N) ? p.wshift[n] : 0);
     const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.done, 0, p.status, ST_TIMEOUT_FULL)) && !*abort;
     if (ok) {
@@ -366,11 +368,11 @@ static int dense_launch(DenseParams& p, int parts, cudaStream_t s) {
 static int token_tile(int64_t M) { return M <= 64 ? 64 : M <= 128 ? 128 : 256; }
 
 int dense_parts(int64_t N, int64_t K, int64_t M) {
-  // As many shares of K as still leave a CTA an SM (a B200's 148: the workspace is sized without a context), of eight steps of 64 at least; of sixteen above 256 rows, where
-  // the last kernel pays more for adding shares than a short GEMM gains. F16 in us, a call, shares of at least 4 / 8 / 16 /
-  // 32 steps: 300 rows, 512 x 1024 29.3 / 29.4 / 26.4 / 26.4, 1003 x 4096 46.5 / 46.5 / 37.2 / 40.8, 2048 x 6144 41.8 / 41.5 /
-  // 41.5 / 44.1. Fewer rows, 4 / 8 steps: 64 rows of 1024 x 2048 14.9 / 12.0, 256 rows of 512 x 1024 19.7 / 16.0, but 64
-  // rows of 64 x 1024 10.1 / 11.1.
+  // As many shares of K as still leave a CTA an SM (a B200's 148: the workspace is sized without a context), of eight
+  // steps of 64 at least; of sixteen above 256 rows, where the last kernel pays more for adding shares than a short GEMM
+  // gains. F16 in us, a call, shares of at least 4 / 8 / 16 / 32 steps: 300 rows, 512 x 1024 29.3 / 29.4 / 26.4 / 26.4,
+  // 1003 x 4096 46.5 / 46.5 / 37.2 / 40.8, 2048 x 6144 41.8 / 41.5 / 41.5 / 44.1. Fewer rows, 4 / 8 steps: 64 rows of 1024 x
+  // 2048 14.9 / 12.0, 256 rows of 512 x 1024 19.7 / 16.0, but 64 rows of 64 x 1024 10.1 / 11.1.
   const int64_t tiles = ((N + 127) / 128) * ((M + token_tile(M) - 1) / token_tile(M));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, K / (M > 256 ? 1024 : 512)), 148 / tiles)));
 }

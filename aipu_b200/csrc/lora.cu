@@ -89,7 +89,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int valid) {
 
 // v as bf16 pieces: hi = v cut off (to the next value towards 0 where nothing would be left) and the rest, which is exact.
 // So no piece of a value other than 0 is 0 or has another sign, and infinity = the largest number + infinity: pieces
-// times an infinite or NaN factor sum to what the value times it is. (A value of less than 2^-132 has pieces of 0.)
+// times an infinite or NaN factor sum to what the value times it is. (Below 2^-110 a rest may be too small for the type.)
 __device__ __forceinline__ uint32_t upper(float v) { return (__float_as_uint(v) - (v != 0.f ? 1u : 0u)) & 0xFFFF0000u; }
 __device__ __forceinline__ uint32_t piece(float v, float& rest) {
   const uint32_t hi = upper(v);
