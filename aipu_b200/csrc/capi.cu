@@ -1386,13 +1386,18 @@ extern "C" int aipu_lora_add(aipu_ctx* c, const aipu_lora* ad, const int32_t* id
 
 // Whether the projection dequantises its weights once and runs as an fp16 GEMM, or as launches of the decode GEMV of up to 8
 // rows each. Two launches read 1.1 bytes a weight (Q4_K) and the GEMM's halves take 4 to write and 4 to read: 9 / 16
-// rows by launches and by the GEMM, us: Q4_K 6144 x 2048 35 / 33 and 28 / 28, 4096 x 4096 28 / 36 and 33 / 34, 4096 x 11008 44 / 46
-// and 90 / 91, 8192 x 8192 60 / 58 and 116 / 116; Q6_K 4096 x 4096 33 / 40 and 37 / 38, 8192 x 8192 82 / 136 and 132 / 133;
-// Q8_0 4096 x 1003 23 / 28 and 16 / 17, 6144 x 6144 53 / 69 and 74 / 74. Three launches (24 rows): 51 against 35 at Q4_K 4096 x
-// 4096, 84 against 117 at 8192 x 8192, Q6_K 200 against 134. F16 weights are read as they are stored: 29 / 31 and 17 / 17.
+// rows by launches and by the GEMM, us: Q4_K 6144 x 2048 38 / 37 and 28 / 28, 4096 x 4096 31 / 41 and 33 / 34, 4096 x 11008 48 / 50
+// and 90 / 91, 8192 x 8192 64 / 62 and 116 / 116; Q6_K 4096 x 4096 36 / 43 and 37 / 38, 8192 x 8192 86 / 140 and 132 / 133;
+// Q8_0 4096 x 1003 26 / 31 and 16 / 17, 6144 x 6144 56 / 72 and 74 / 74. Three launches (24 rows): 55 against 35 at Q4_K 4096 x
+// 4096, 88 against 117 at 8192 x 8192, Q6_K 204 against 134. F16 weights are read as they are stored: 32 / 34 and 17 / 17.
 static bool gemm_lora_dense(int wtype, int64_t N, int64_t K, int64_t M) {
-  return K > kGemvMaxK || M > 16 || (M > 8 && (wtype == AIPU_F16 || N * K < (1 << 24)));
+  return K > kGemvMaxK || M > 16 || (M > 8 && (wtype == AIPU_F16 || N * K <= (1 << 24)));
 }
+// Above 8 rows the GEMV launches take their partial sums and (zeroed) tile counters from the call's scratch, so that calls may
+// run at the same time as they may on the GEMM. Of so many SMs at most:
+static const int kLoraGemvSms = 160;
+static size_t gemm_lora_partials() { return al256x(sizeof(float) * gemv_partials_floats(kLoraGemvSms)); }
+static size_t gemm_lora_counters(int64_t N) { return 4 * static_cast<size_t>(std::min<int64_t>((N + 15) / 16, kMaxTiles)); }
 // row stride of its fp32 sums: rows start on 32 bytes
 static int64_t gemm_lora_ld(int64_t N) { return (N + 7) & ~static_cast<int64_t>(7); }
 
@@ -1403,6 +1408,7 @@ extern "C" int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K,
   const size_t parts = gemm_lora_dense(wtype, N, K, M) ? dense_parts(N, K, M) : 1;
   size_t b = al256x(lora_plan_bytes(M, n_adapters, rank)) + al256x(4 * parts * M * gemm_lora_ld(N));
   if (gemm_lora_dense(wtype, N, K, M)) b += dense_bytes(wtype, N, K, M);
+  else if (M > 8) b += gemm_lora_partials() + gemm_lora_counters(N);
   return static_cast<int64_t>(b);
 }
 
@@ -1445,7 +1451,16 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
     rc = dense_gemm(wtype, static_cast<const uint8_t*>(w), p.N, p.K, p.x, p.M, y32, p.ldy, b, c->status, s, p.tiles != nullptr);
   } else {
     // as many launches as the GEMV's tile counters (of N) and its shared memory (of tokens of K) ask for
-    const int64_t step = static_cast<int64_t>(c->ws[0].max_tiles) * 16;
+    const int64_t step = static_cast<int64_t>(kMaxTiles) * 16;
+    float* partials = c->ws[0].partials;
+    int* counters = c->ws[0].counters;
+    int sms = c->num_sms;
+    if (M > 8) {
+      partials = reinterpret_cast<float*>(b);
+      counters = reinterpret_cast<int*>(b + gemm_lora_partials());
+      sms = std::min(sms, kLoraGemvSms);
+      if ((rc = set_cuda_error(cudaMemsetAsync(counters, 0, gemm_lora_counters(N), s), "cudaMemsetAsync(gemm_lora)"))) return rc;
+    }
     for (int64_t n0 = 0; n0 < N && !rc; n0 += step) {
       GemvParams g = {};
       g.row_bytes = row_bytes_of(wtype, K);
@@ -1454,10 +1469,10 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
       g.N = static_cast<int>(std::min(step, N - n0));
       g.K = p.K;
       g.y32_ld = p.ldy;
-      g.partials = c->ws[0].partials;
-      g.counters = c->ws[0].counters;
+      g.partials = partials;
+      g.counters = counters;
       g.status = c->status;
-      const int fit = gemv_rows(wtype, g.w0, g.N, g.K, c->num_sms);
+      const int fit = gemv_rows(wtype, g.w0, g.N, g.K, sms);
       if (fit < 1) return set_error(EINVAL_, "gemm_lora: a token does not fit the GEMV");
       const int launches = (p.M + fit - 1) / fit, rows = (p.M + launches - 1) / launches;
       for (int m0 = 0; m0 < p.M && !rc; m0 += rows) {
@@ -1466,7 +1481,7 @@ extern "C" int aipu_q4k_gemm_lora(aipu_ctx* c, int wtype, const void* w, int64_t
         g.y32 = y32 + m0 * p.ldy + n0;
         // no programmatic launch: when this kernel starts, everything before it is done, so the adapter
         // kernel behind it may read x, the ids and the adapters without waiting for it
-        rc = gemv_launch(wtype, XT_BF16, EPI_STORE32, g, c->num_sms, s, false);
+        rc = gemv_launch(wtype, XT_BF16, EPI_STORE32, g, sms, s, false);
       }
     }
   }

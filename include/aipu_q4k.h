@@ -291,9 +291,9 @@ int aipu_lora_add(aipu_ctx* ctx, const aipu_lora* ad, const int32_t* ids, const 
 /* The quantised projection with the adapters of its rows: y[m, n] (bf16) = bf16(x[m] W^T + the adapter
  * term of aipu_lora_add); x[M, K] bf16, 16-byte aligned, W = N GGUF rows of K weights (Q4_K, Q6_K, Q8_0,
  * F16; K a multiple of 256, 16-byte aligned); y must not overlap the inputs. The projection's fp32 sums are not
- * rounded before the adapter term is added: up to 8 rows (16 of 2^24 quantised weights and more) those of
+ * rounded before the adapter term is added: up to 8 rows (16 of more than 2^24 quantised weights) those of
  * AIPU_MODE_FAST, above them, and for K above 65536, of a tcgen05 GEMM whose weights are two fp16 halves of 22 bits.
- * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Up to 16 rows may use the context's
+ * ws: device scratch of aipu_q4k_gemm_lora_workspace(...) bytes (256-byte aligned). Up to 8 rows use the context's
  * stream-K workspace too (one context per concurrently used stream). No counterpart in the reference. */
 int64_t aipu_q4k_gemm_lora_workspace(int wtype, int64_t N, int64_t K, int64_t M, int64_t n_adapters, int64_t rank);
 int aipu_q4k_gemm_lora(aipu_ctx* ctx, int wtype, const void* w, int64_t N, int64_t K, const void* x, int64_t M,

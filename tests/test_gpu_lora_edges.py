@@ -304,7 +304,7 @@ def test_long_sums_of_one_sign_are_rounded_not_cut_off(ad, M, K):
 
 
 @pytest.mark.parametrize("wt", TYPES)
-@pytest.mark.parametrize("K,N", [(4096, 4096), (4096, 4088), (11008, 1600)])
+@pytest.mark.parametrize("K,N", [(4096, 4096), (4096, 4104), (11008, 1600)])
 def test_9_to_17_rows_of_large_weights(wt, K, N):
     """On both sides of the borders between launches of the GEMV and the fp16 GEMM, in the rows and in the weights. Tolerance
     as for few rows of long weights."""
@@ -321,6 +321,31 @@ def test_9_to_17_rows_of_large_weights(wt, K, N):
         ids = torch.full((M,), -1, dtype=torch.int32, device=d)
         got = ops.gemm_lora(wt, w, N, K, x[:M], _plain(d, K, N), ids).double()
         assert ((got - want[:M]).abs() <= tol[:M]).all(), M
+
+
+@pytest.mark.parametrize("wt", [F.Q4_K, F.Q6_K])
+def test_9_to_16_rows_on_several_streams_at_once(wt):
+    """Calls of more than 8 rows share nothing of their context."""
+    d, K, N, M = _dev(), 4096, 8192, 13
+    w, _ = _weights(wt, N, K, 2, d)
+    x = torch.randn((3, M, K), device=d, generator=torch.Generator(d).manual_seed(1)).to(BF)
+    A, ids = _plain(d, K, N), torch.full((M,), -1, dtype=torch.int32, device=d)
+    want = [ops.gemm_lora(wt, w, N, K, x[i], A, ids) for i in range(3)]
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs.append((i, ops.gemm_lora(wt, w, N, K, x[i], A, ids)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = ops.gemm_lora(wt, w, N, K, x[0], A, ids)
+    for i in (1, 2):
+        x[0].copy_(x[i])
+        g.replay()
+        assert torch.equal(o, want[i])
 
 
 @pytest.mark.parametrize("N", [32000, 128000, 50257])
